@@ -79,21 +79,11 @@ def set_wgrad_side_stream(enabled):
     _SIDE["enabled"] = bool(enabled)
 
 
-# HIP stream priority of the weight-gradient stream: -1 (high, default) | 0 (normal).  Measured (round 6, same box, two A/B rounds): high
-# 127.0 / 127.2 ms, normal 127.5 / 127.6 — the full-chip weight-gradient launches finish sooner when the dispatcher favours them, and
-# the main stream's kernels were going to share the chip with them anyway.
-_SIDE_PRIORITY = os.environ.get("FFVC_SIDE_PRIORITY", "-1")
-
-
+# The weight-gradient stream has the default priority, as every stream of this package: work on streams of different priorities can hang the
+# device.  (High priority measured 0.4 % faster on the 127 ms step: not worth that.)
 def _side_stream():
     if _SIDE["stream"] is None:
-        if _SIDE_PRIORITY is not None:
-            try:
-                _SIDE["stream"] = torch.cuda.Stream(priority=int(_SIDE_PRIORITY))
-            except (RuntimeError, ValueError):
-                _SIDE["stream"] = torch.cuda.Stream()
-        else:
-            _SIDE["stream"] = torch.cuda.Stream()
+        _SIDE["stream"] = torch.cuda.Stream()
     return _SIDE["stream"]
 
 

@@ -1,5 +1,5 @@
 """Round 6: bitwise run-to-run reproducibility of the VitGAN-only kernels (16-token attention fwd / bwd, SLN fwd / bwd) at cfg3's geometry
-while a second, high-priority stream keeps the chip busy.  usage (GPU box): python tools/r6/vit_ops_stress.py"""
+while a second stream keeps the chip busy.  usage (GPU box): python tools/r6/vit_ops_stress.py"""
 import os
 import sys
 
@@ -10,7 +10,7 @@ from feed_forward_vqgan_clip_amd import kernels as K  # noqa: E402
 
 dev = torch.device("cuda:0")
 dt = torch.float16
-side = torch.cuda.Stream(priority=-1)
+side = torch.cuda.Stream()
 a = torch.randn(4096, 1024, device=dev).to(dt)
 b = torch.randn(512, 4096, device=dev).to(dt)
 wg = torch.zeros(4096, 1024, device=dev)
