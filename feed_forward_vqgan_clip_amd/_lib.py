@@ -107,6 +107,14 @@ class GemmDesc(Structure):
     ]
 
 
+class AttnPackedDesc(Structure):
+    """Mirror of `ffvc_attn_packed_desc` (include/ffvc.h)."""
+
+    _fields_ = ([(n, c_void_p) for n in ("q", "k", "v", "out", "lse", "cu", "dout", "dq", "dk", "dv", "delta")] + [("rows", c_int64)] +
+                [(f"{n}_{s}", c_int64) for n in ("q", "k", "v", "o", "do", "dq", "dk", "dv") for s in ("rs", "hs")] +
+                [(n, c_int32) for n in ("seqs", "heads", "kv_heads", "head_dim", "dtype", "zero_tail")] + [("scale", c_float)])
+
+
 _lib = None
 
 # name -> (restype, argtypes).  tests/test_abi.py checks every symbol declared in
@@ -229,6 +237,18 @@ _SIGNATURES = {
     "ffvc_tokmix_fwd": (c_int, [c_void_p] * 7 + [c_int, c_int, c_int, c_int, c_int, c_void_p]),
     "ffvc_tokmix_bwd_hidden": (c_int, [c_void_p] * 8 + [c_int, c_int, c_int, c_int, c_int, c_void_p]),
     "ffvc_tokmix_fwd_save": (c_int, [c_void_p] * 9 + [c_int, c_int, c_int, c_int, c_int, c_void_p]),
+    "ffvc_embed_fwd": (c_int, [c_void_p, c_int, c_int64, c_int64, c_void_p, c_float, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int, c_int64,
+                               c_int64, c_int, c_void_p]),
+    "ffvc_embed_bwd_ws_bytes": (c_int64, [c_int64, c_int]),
+    "ffvc_embed_bwd": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int64, c_int64, c_int, c_float, c_void_p, c_int, c_void_p, c_int64, c_void_p]),
+    "ffvc_attn_packed_fwd": (c_int, [POINTER(AttnPackedDesc), c_void_p]),
+    "ffvc_attn_packed_bwd": (c_int, [POINTER(AttnPackedDesc), c_void_p]),
+    "ffvc_int8_quant": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p]),
+    "ffvc_gemm_int8": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int64, c_void_p, c_int,
+                               c_int64, c_void_p, c_int, c_int, c_int, c_int, c_void_p]),
+    "ffvc_linear_int8_few_ok": (c_int, [c_int, c_int]),
+    "ffvc_linear_int8_few": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int64, c_void_p, c_int,
+                                     c_int64, c_void_p, c_int, c_int, c_int, c_void_p]),
     "ffvc_set_option": (c_int, [c_char_p, c_int]),
     "ffvc_last_error": (c_char_p, []),
     "ffvc_version": (c_int, []),

@@ -76,9 +76,9 @@ def _f(t):
 
 
 class _Block:
-    def __init__(self, sd, p, cdt, need_dgrad, act=ACT_QUICKGELU, fp8=False):
+    def __init__(self, sd, p, cdt, need_dgrad, act=ACT_QUICKGELU, fp8=False, int8=False):
         self.act = act
-        fz = lambda w, b: ops.Weights.frozen(sd[w], sd[b], cdt, need_dgrad, fp8=fp8)  # noqa: E731
+        fz = lambda w, b: ops.Weights.frozen(sd[w], sd[b], cdt, need_dgrad, fp8=fp8, int8=int8)  # noqa: E731
         self.ln1 = (_f(sd[p + ".ln_1.weight"]), _f(sd[p + ".ln_1.bias"]))
         self.ln2 = (_f(sd[p + ".ln_2.weight"]), _f(sd[p + ".ln_2.bias"]))
         self.in_proj = fz(p + ".attn.in_proj_weight", p + ".attn.in_proj_bias")
@@ -86,12 +86,15 @@ class _Block:
         self.c_fc = fz(p + ".mlp.c_fc.weight", p + ".mlp.c_fc.bias")
         self.c_proj = fz(p + ".mlp.c_proj.weight", p + ".mlp.c_proj.bias")
 
-    def __call__(self, x, heads, cdt, causal):
-        """cloob.py:202-205: x + attn(ln_1(x)); x + mlp(ln_2(x)). x: fp32 residual stream (N, L, D)."""
+    def __call__(self, x, heads, cdt, causal, cu_seqlens=None):
+        """cloob.py:202-205: x + attn(ln_1(x)); x + mlp(ln_2(x)). x: fp32 residual stream (N, L, D); with cu_seqlens packed rows (rows, D)."""
         f32 = torch.float32
         dh = x.shape[-1] // heads
         xn, xid = ops.layernorm_fork(x, *self.ln1, cdt, f8_for=self.in_proj)       # fp8 tower: LN writes the e4m3 operand of its linear
-        o = ops.attention(ops.linear(xn, self.in_proj), heads, dh ** -0.5, causal, f8_for=self.out_proj)
+        if cu_seqlens is not None:
+            o = ops.attention_packed(ops.linear(xn, self.in_proj), cu_seqlens, heads, scale=dh ** -0.5)
+        else:
+            o = ops.attention(ops.linear(xn, self.in_proj), heads, dh ** -0.5, causal, f8_for=self.out_proj)
         x = ops.linear(o, self.out_proj, residual=xid, out_dtype=f32)
         xn, xid = ops.layernorm_fork(x, *self.ln2, cdt, f8_for=self.c_fc)
         return ops.mlp(xn, self.c_fc, self.c_proj, self.act, residual=xid, out_dtype=f32)
@@ -164,9 +167,22 @@ class _TakeToken(torch.autograd.Function):
         return dx, None
 
 
+def pack_tokens(text):
+    """Padded prompts (B, L) int64 -> (ids [rows], cu_seqlens int32 [B + 1]), both on the host: every prompt up to and with its EOT (the largest
+    id, cloob.py:536).  What stands behind it cannot reach the features: the mask is causal and they are read at the EOT."""
+    if text.dtype != torch.long or text.dim() != 2 or text.shape[0] < 1 or text.shape[1] < 1:
+        raise TypeError("pack_tokens expects int64 token rows (B, L)")
+    text = text.cpu()
+    n = text.argmax(dim=-1) + 1
+    ids = torch.cat([row[:int(k)] for row, k in zip(text, n)])
+    cu = torch.zeros(len(n) + 1, dtype=torch.int32)
+    cu[1:] = n.cumsum(0)
+    return ids, cu
+
+
 class CLIP:
     def __init__(self, state_dict, cdt=torch.float16, vision_heads=None, text_heads=None, quick_gelu=True, fp8=False,
-                 text_exact=None):
+                 text_exact=None, int8=False, text_packed=False):
         """quick_gelu: OpenAI checkpoints and open_clip's `-quickgelu` architectures use x*sigmoid(1.702x) in the MLPs
         (cloob.py:179-181); the other open_clip architectures (ViT-B-32 / ViT-L-14 on LAION-2B, main.py:1323-1329) use
         the exact erf GELU.
@@ -176,11 +192,20 @@ class CLIP:
         text_exact: True = the text tower's Linear layers on the exact fp32 MFMA (v_mfma_f32_32x32x2_f32, 1/16 of the 16-bit
         rate; what round 2 shipped); False = split-precision f16 GEMMs (`_SplitLinear`, fp32-grade: features agree with the exact
         path to ~1e-6 relative, 7.4 -> ~2 ms per step at cfg2).  Default: exact in fp32 parity mode, split otherwise
-        (FFVC_TEXT_EXACT=1 forces the exact path)."""
+        (FFVC_TEXT_EXACT=1 forces the exact path).
+        int8: the same four Linear layers of the image tower (and of the packed text tower) in 8-bit integers, one scale per token and per
+        channel (kernels.linear_int8), forward only: gradients pass straight through to the 16-bit W^T.  Excludes fp8.
+        text_packed: also build the text tower over packed prompts in the compute dtype (encode_text_packed); encode_text then packs its
+        rows and uses it (16-bit activations, 8-bit Linear layers with int8, instead of the fp32-grade padded tower)."""
         if not torch.cuda.is_available():
             raise RuntimeError("CLIP needs a HIP device; there is no CPU fallback")
         sd, self.cdt = state_dict, cdt
         self.fp8 = bool(fp8)
+        self.int8, self.text_packed = bool(int8), bool(text_packed)
+        if self.int8 and self.fp8:
+            raise ValueError("CLIP: int8 and fp8 exclude each other")
+        if (self.int8 or self.text_packed) and cdt not in K.LOWP:
+            raise ValueError("CLIP: int8 / text_packed need a 16-bit compute dtype")
         act = ACT_QUICKGELU if quick_gelu else ACT_GELU
         w = sd["visual.conv1.weight"]
         self.width, self.patch = w.shape[0], w.shape[-1]
@@ -196,7 +221,7 @@ class CLIP:
         n = 0
         self.vblocks = []
         while f"visual.transformer.resblocks.{n}.ln_1.weight" in sd:
-            self.vblocks.append(_Block(sd, f"visual.transformer.resblocks.{n}", cdt, True, act, fp8=fp8))
+            self.vblocks.append(_Block(sd, f"visual.transformer.resblocks.{n}", cdt, True, act, fp8=fp8, int8=int8))
             n += 1
         self.vproj = ops.Weights.frozen(sd["visual.proj"].t().contiguous(), None, cdt)
         self.embed_dim = sd["visual.proj"].shape[1]
@@ -219,6 +244,9 @@ class CLIP:
         self.ln_final = (_f(sd["ln_final.weight"]), _f(sd["ln_final.bias"]))
         self.tproj = ops.Weights.frozen(sd["text_projection"].t().contiguous(), None, f32, False)
         self.logit_scale = _f(sd["logit_scale"]) if "logit_scale" in sd else torch.tensor(np.log(1 / 0.07)).cuda()
+        if self.text_packed:
+            self.pblocks = [_Block(sd, f"transformer.resblocks.{i}", cdt, True, act, int8=int8) for i in range(n)]
+            self.ptproj = ops.Weights.frozen(sd["text_projection"].t().contiguous(), None, f32, True)
         if not self.text_exact:
             self._probe_text_tower(sd, act)
 
@@ -231,7 +259,7 @@ class CLIP:
         g = torch.Generator().manual_seed(0)
         tok = torch.randint(1, max(2, V - 2), (4, L), generator=g)
         tok[:, -1] = V - 1
-        feats = self.encode_text(tok)
+        feats = self._encode_text_padded(tok)
         if not bool(torch.isfinite(feats).all()):
             self.text_exact = True
             f32 = torch.float32
@@ -265,6 +293,13 @@ class CLIP:
         """text: int64 (B, L) -> (B, embed_dim) fp32 (cloob.py:525-538)."""
         if text.dtype != torch.long:
             raise TypeError("encode_text expects int64 token ids (main.py:733 dispatches on torch.long)")
+        if self.text_packed:
+            ids, cu = pack_tokens(text)
+            return self.encode_text_packed(ids.cuda(), cu.cuda())
+        return self._encode_text_padded(text)
+
+    @torch.no_grad()
+    def _encode_text_padded(self, text):
         f32 = torch.float32
         text = text.cuda().contiguous()
         B, L = text.shape
@@ -274,6 +309,26 @@ class CLIP:
         xn = ops.layernorm(x, *self.ln_final, f32)                                  # :532
         eot = K.eot_gather(xn, text)                                                # :536
         return ops.linear(eot, self.tproj, out_dtype=f32)
+
+    def encode_text_packed(self, ids, cu_seqlens, table=None):
+        """Features of prompts packed behind one another (pack_tokens): ids int64 [rows], cu_seqlens int32 [B + 1], both on the device ->
+        (B, embed_dim) fp32.  Rows behind the last prompt are ignored, a prompt without tokens gives the features of a zero row.
+        table: a token embedding to use instead of the checkpoint's (vocab, width) fp32; gradients flow to it (and through the frozen tower)."""
+        if not self.text_packed:
+            raise RuntimeError("this CLIP was built without text_packed=True")
+        if ids.dtype != torch.long or ids.dim() != 1 or cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2:
+            raise TypeError("encode_text_packed expects int64 ids [rows] and int32 offsets [B + 1]")
+        f32 = torch.float32
+        first, end = cu_seqlens[:-1].long(), cu_seqlens[1:].long()
+        row = torch.arange(ids.numel(), device=ids.device)
+        seq = torch.searchsorted(end, row, right=True)                              # the prompt of a row; B behind the last one
+        behind = seq >= first.numel()
+        place = torch.where(behind, -1, row - first[seq.clamp(max=first.numel() - 1)])
+        x = ops.embedding(torch.where(behind, -1, ids), self.tok_emb if table is None else table, pos=self.tpos, pos_ids=place, out_dtype=f32)
+        for blk in self.pblocks:
+            x = blk(x, self.text_heads, self.cdt, True, cu_seqlens)
+        eot = ops.embedding(torch.where(end > first, end - 1, -1), x)               # the rows the features are read at
+        return ops.linear(ops.layernorm(eot, *self.ln_final, f32), self.ptproj, out_dtype=f32)
 
     def float(self):
         return self

@@ -1,0 +1,610 @@
+// attn_packed.hip — causal attention over PACKED sequences of different lengths with grouped heads, forward and backward.
+//
+// The rows cu[b] .. cu[b + 1] - 1 of q / k / v are sequence b.  With c = scale * log2(e), query i of a sequence and its keys j <= i:
+//     s_ij = q_i . k_j        m_i = max_j s_ij        l_i = sum_j 2^(c (s_ij - m_i))        p_ij = 2^(c (s_ij - m_i)) / l_i
+//     o_i  = sum_j p_ij v_j                           lse_i = c m_i + log2 l_i   (kept for the backward: p_ij = 2^(c s_ij - lse_i))
+//     dv_j = sum_i p_ij do_i      dp_ij = do_i . v_j      delta_i = do_i . o_i      ds_ij = scale p_ij (dp_ij - delta_i)
+//     dq_i = sum_j ds_ij k_j      dk_j = sum_i ds_ij q_i  (over the heads / kv_heads query heads that share key head j's group)
+//
+// Work is cut without knowing the lengths on the host: with tiles of BM rows, sequence b owns the tile slots from
+// cu[b] / BM + b on.  Consecutive sequences never overlap (floor((c + l) / BM) + 1 - floor(c / BM) >= ceil(l / BM)), so the grid is
+// rows / BM + seqs + 1 slots and a workgroup finds its sequence by a search over the slot starts; a slot past its sequence's last tile has
+// nothing to do.  The rows behind the last sequence are a pseudo-sequence of their own (zero-filled on request, otherwise left alone).
+// Offsets into a tensor are 64 bits wide; inside a tile the buffer descriptor's 32-bit offsets are enough, its record count ends with the
+// sequence, so rows past the end (and features past head_dim) read as zeros without a branch.
+#include "common.h"
+
+namespace {
+
+#define mma mma_lo<L>
+
+typedef __amdgpu_buffer_rsrc_t rsrc_t;
+typedef __attribute__((address_space(3))) void* lds_vp;
+typedef __attribute__((address_space(3))) s16x4_t* lds_tr;
+constexpr uint32_t OOB = 0xFFFFFFF0u;
+constexpr float LOG2E = 1.44269504088896341f;
+constexpr float NEG_BIG = -3.0e38f;
+constexpr int KB = 64;                      // rows of a staged tile
+
+// 64 lanes x 16 (4) bytes from a bounded buffer into consecutive LDS
+__device__ __forceinline__ void dma16(rsrc_t r, uint32_t off, unsigned char* lds) { __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_vp)lds, 16, off, 0, 0, 0); }
+__device__ __forceinline__ void dma4(rsrc_t r, uint32_t off, float* lds) { __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_vp)lds, 4, off, 0, 0, 0); }
+
+// ---- a tile of KB rows x DP features in LDS: rows of DP * 2 bytes in lines of 256, 16-byte chunks XOR-swizzled so that both the 16-byte
+// row reads (16 rows of one chunk column) and the transposing 8-byte reads (4 rows x 32 bytes) spread over all banks
+template <int DP>
+__device__ __forceinline__ int tile_off(int row, int chunk) {       // byte offset of 16-byte chunk `chunk` of row `row`
+  if constexpr (DP == 128) {
+    return row * 256 + ((chunk ^ (((row & 3) << 2) | ((row >> 2) & 3))) << 4);
+  } else {
+    const int line = row >> 1;
+    return line * 256 + (((((row & 1) << 3) | chunk) ^ (((line & 1) << 2) | ((line >> 1) & 3))) << 4);
+  }
+}
+template <int DP>
+__device__ __forceinline__ void tile_src(int pos, int& row, int& chunk) {   // the inverse: what 16-byte position `pos` of the tile holds
+  const int line = pos >> 4, slot = pos & 15;
+  if constexpr (DP == 128) {
+    row = line;
+    chunk = slot ^ (((row & 3) << 2) | ((row >> 2) & 3));
+  } else {
+    const int cp = slot ^ (((line & 1) << 2) | ((line >> 1) & 3));
+    row = 2 * line + (cp >> 3);
+    chunk = cp & 7;
+  }
+}
+
+// LDS-DMA of one tile by NW waves: piece i of a wave fills 64 consecutive chunk positions; the lane's source offset inside the tile is fixed
+template <int DP, int NW>
+struct TileDma {
+  static constexpr int NP = KB * DP / 8 / 64 / NW;
+  uint32_t off[NP];
+  __device__ __forceinline__ void init(int64_t rs, int D, int wave, int lane) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      int row, chunk;
+      tile_src<DP>((wave * NP + i) * 64 + lane, row, chunk);
+      off[i] = chunk * 8 < D ? (uint32_t)((row * rs + chunk * 8) * 2) : OOB;
+    }
+  }
+  // base: element (row0, feature 0) of the tile; live: rows of the sequence from row0 on (> 0)
+  __device__ __forceinline__ void issue(const uint16_t* base, int64_t rs, int D, int64_t live, unsigned char* tile, int wave) {
+    const int64_t bytes = ((live < KB ? live : KB) - 1) * rs * 2 + D * 2;
+    const rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)bytes, 0x00020000);
+#pragma unroll
+    for (int i = 0; i < NP; ++i)
+      dma16(r, off[i], tile + (wave * NP + i) * 1024);
+  }
+};
+
+// A fragment (rows of the tile): features 16 s + 8 h .. + 7 of row `row`
+template <int DP>
+__device__ __forceinline__ u32x4_t frag_rows(const unsigned char* tile, int row, int s, int h) {
+  return *(const u32x4_t*)(tile + tile_off<DP>(row, 2 * s + h));
+}
+// A fragment of the transposed tile: lane -> feature 32 dt + lane % 32, elements = rows r0 + 4 h + {0..3} and r0 + 8 + 4 h + {0..3}: the
+// order in which eight consecutive accumulator registers of a 32 x 32 product run over its rows, so those are the B fragment as they are
+template <int DP>
+__device__ __forceinline__ u32x4_t frag_cols(const unsigned char* tile, int dt, int r0, int lane) {
+  const int c = lane & 15, h = lane >> 5;
+  const int d = 32 * dt + 16 * ((lane >> 4) & 1) + 4 * (c & 3);
+  const int row = r0 + 4 * h + (c >> 2);
+  union {
+    s16x4_t x[2];
+    u32x4_t v;
+  } u;
+  u.x[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr)(tile + tile_off<DP>(row, d >> 3) + (d & 7) * 2));
+  u.x[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr)(tile + tile_off<DP>(row + 8, d >> 3) + (d & 7) * 2));
+  return u.v;
+}
+
+template <typename L>
+__device__ __forceinline__ u32x4_t pack8(const f32x16_t& t, int first) {
+  u32x4_t r;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) r[e] = lo_pack2<L>(t[first + 2 * e], t[first + 2 * e + 1]);
+  return r;
+}
+
+__device__ __forceinline__ void zero16(f32x16_t& t) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r) t[r] = 0.0f;
+}
+__device__ __forceinline__ int acc_row(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }
+
+// the other half-wave's value of the same column
+__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
+
+struct Place {
+  int64_t row0;      // first row of the sequence
+  int64_t len;       // its rows
+  int64_t tile;      // tile inside the sequence
+  bool tail;         // the rows behind the last sequence
+};
+
+__device__ __forceinline__ int64_t cu_at(const int32_t* cu, int b, int64_t rows) {
+  const int64_t c = cu[b];
+  return c < 0 ? 0 : (c > rows ? rows : c);
+}
+
+// slot -> (sequence, tile).  64 probes at a time; a cu that is not ascending gives some sequence's clamped rows, never one outside [0, rows).
+template <int BM>
+__device__ __forceinline__ Place find_slot(const int32_t* __restrict__ cu, int seqs, int64_t rows, int64_t slot) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, n = seqs + 1;                       // candidates lo .. lo + n - 1; sequence `seqs` is the tail
+  while (n > 1) {
+    const int step = (n + 63) / 64;
+    const int b = lo + lane * step;
+    const bool le = lane * step < n && cu_at(cu, b, rows) / BM + b <= slot;
+    const uint64_t m = __ballot(le) | 1ull;       // (candidate lo always holds)
+    const int k = 63 - __builtin_clzll(m);
+    lo += k * step;
+    n = min(step, n - k * step);
+  }
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  Place p;
+  p.row0 = cu_at(cu, lo, rows);
+  const int64_t end = lo < seqs ? cu_at(cu, lo + 1, rows) : rows;
+  p.len = end > p.row0 ? end - p.row0 : 0;
+  p.tile = slot - (p.row0 / BM + lo);
+  p.tail = lo == seqs;
+  return p;
+}
+
+// block -> (slot, head).  Consecutive workgroups go to the 8 XCDs in turn: with a multiple of 8 heads each XCD keeps heads / 8 neighbouring
+// heads, so the heads of one key / value group read it through one L2.  The last tiles of the sequences (the longest rows) go first.
+__device__ __forceinline__ void block_place(int64_t slots, int heads, int64_t& slot, int& head) {
+  const int64_t i = blockIdx.x;
+  const int j = (int)(i % heads);
+  head = heads % 8 == 0 ? (j & 7) * (heads >> 3) + (j >> 3) : j;
+  slot = slots - 1 - i / heads;
+}
+
+// o[row0 + lane % 32][32 dt + ...] = acc, rows < n; the wave's tile is transposed (lane = row, registers = features)
+template <typename L, int DP>
+__device__ __forceinline__ void store_rows(uint16_t* base, int64_t rs, int D, const f32x16_t (&acc)[DP / 32], int row, bool ok, int h) {
+  if (!ok) return;
+  uint16_t* p = base + row * rs;
+#pragma unroll
+  for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = 32 * dt + 8 * g + 4 * h;
+      if (d < D) {
+        u32x2_t v;
+        v[0] = lo_pack2<L>(acc[dt][4 * g], acc[dt][4 * g + 1]);
+        v[1] = lo_pack2<L>(acc[dt][4 * g + 2], acc[dt][4 * g + 3]);
+        *(u32x2_t*)(p + d) = v;
+      }
+    }
+}
+
+__device__ __forceinline__ void zero_rows(uint16_t* base, int64_t rs, int D, int64_t nrows, int tid, int threads) {
+  const int ch = D / 8;
+  const u32x4_t z = {0u, 0u, 0u, 0u};
+  for (int64_t i = tid; i < nrows * ch; i += threads) {
+    const int64_t r = i / ch;
+    *(u32x4_t*)(base + r * rs + (i - r * ch) * 8) = z;
+  }
+}
+
+// eight features of row `row` (16 s + 8 h ..) of one head; zeros past the sequence or past head_dim
+__device__ __forceinline__ u32x4_t row_frag(const uint16_t* base, int64_t rs, int64_t row, bool ok, int s, int h, int D) {
+  const u32x4_t z = {0u, 0u, 0u, 0u};
+  const int d = 16 * s + 8 * h;
+  return ok && d < D ? *(const u32x4_t*)(base + row * rs + d) : z;
+}
+
+// ---- forward -------------------------------------------------------------------------------------------------------------------
+// NW waves x 32 queries; key / value tiles of 64 rows, two LDS stages filled by LDS-DMA while the previous tile is multiplied.
+template <typename L, int DP, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void attn_packed_fwd_kernel(const ffvc_attn_packed_desc p, int64_t slots) {
+  constexpr int BM = 32 * NW, NS = DP / 16, ND = DP / 32, TB = KB * DP * 2;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int64_t slot;
+  int head;
+  block_place(slots, p.heads, slot, head);
+  const Place pl = find_slot<BM>(p.cu, p.seqs, p.rows, slot);
+  const int64_t q0 = pl.tile * BM;
+  if (q0 < 0 || q0 >= pl.len) return;
+  const int D = p.head_dim;
+  uint16_t* O = (uint16_t*)p.out + pl.row0 * p.o_rs + head * p.o_hs;
+  if (pl.tail) {
+    if (p.zero_tail) zero_rows(O + q0 * p.o_rs, p.o_rs, D, pl.len - q0 < BM ? pl.len - q0 : BM, tid, 64 * NW);
+    return;
+  }
+  const int kvh = head / (p.heads / p.kv_heads);
+  const uint16_t* Q = (const uint16_t*)p.q + pl.row0 * p.q_rs + head * p.q_hs;
+  const uint16_t* Kp = (const uint16_t*)p.k + pl.row0 * p.k_rs + kvh * p.k_hs;
+  const uint16_t* V = (const uint16_t*)p.v + pl.row0 * p.v_rs + kvh * p.v_hs;
+  const float c = p.scale * LOG2E;
+  TileDma<DP, NW> dk, dv;
+  dk.init(p.k_rs, D, wave, lane);
+  dv.init(p.v_rs, D, wave, lane);
+  const int64_t qend = q0 + BM < pl.len ? q0 + BM : pl.len;
+  const int nkb = (int)((qend + KB - 1) / KB);
+  auto issue = [&](int kb) {
+    const int64_t k0 = (int64_t)kb * KB;
+    unsigned char* st = smem + (kb & 1) * 2 * TB;
+    dk.issue(Kp + k0 * p.k_rs, p.k_rs, D, pl.len - k0, st, wave);
+    dv.issue(V + k0 * p.v_rs, p.v_rs, D, pl.len - k0, st + TB, wave);
+  };
+  issue(0);
+  const int64_t qw = q0 + 32 * wave;                       // this wave's first query
+  const int64_t qi = qw + l31;
+  const bool ok = qi < pl.len;
+  u32x4_t fq[NS];
+#pragma unroll
+  for (int s = 0; s < NS; ++s) fq[s] = row_frag(Q, p.q_rs, qi, ok, s, h, D);
+  f32x16_t acc[ND];
+#pragma unroll
+  for (int t = 0; t < ND; ++t) zero16(acc[t]);
+  float m = NEG_BIG, l = 0.0f;
+#pragma unroll 1
+  for (int kb = 0; kb < nkb; ++kb) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (kb + 1 < nkb) issue(kb + 1);
+    const int64_t k0 = (int64_t)kb * KB;
+    if (k0 > qw + 31 || qw >= pl.len) continue;            // every key of the tile is later than this wave's queries
+    const unsigned char* sk = smem + (kb & 1) * 2 * TB;
+    const unsigned char* sv = sk + TB;
+    f32x16_t S[2];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      zero16(S[kt]);
+#pragma unroll
+      for (int s = 0; s < NS; ++s) mma(S[kt], frag_rows<DP>(sk, 32 * kt + l31, s, h), fq[s]);
+    }
+    if (k0 + KB - 1 > qw) {                                // the diagonal crosses this tile
+      const int lim = (int)(qi - k0);                      // last visible key of this lane's query
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) S[kt][r] = 32 * kt + acc_row(r, h) <= lim ? S[kt][r] : -INFINITY;
+    }
+    float mx = m;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, S[kt][r]);
+    mx = fmaxf(mx, other_half(mx));
+    if (__any(mx > m)) {                                   // most tiles of a long row leave the maximum alone
+      const float a = __builtin_amdgcn_exp2f((m - mx) * c);
+      l *= a;
+#pragma unroll
+      for (int t = 0; t < ND; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[t][r] *= a;
+      m = mx;
+    }
+    const float mc = m * c;
+    float sum = 0.0f;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        S[kt][r] = __builtin_amdgcn_exp2f(fmaf(S[kt][r], c, -mc));
+        sum += S[kt][r];
+      }
+    l += sum;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int sg = 0; sg < 2; ++sg) {
+        const u32x4_t fp = pack8<L>(S[kt], 8 * sg);
+#pragma unroll
+        for (int t = 0; t < ND; ++t) mma(acc[t], frag_cols<DP>(sv, t, 32 * kt + 16 * sg, lane), fp);
+      }
+  }
+  l += other_half(l);
+  const float inv = 1.0f / l;
+#pragma unroll
+  for (int t = 0; t < ND; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[t][r] *= inv;
+  if (p.lse && ok && h == 0) p.lse[(int64_t)head * p.rows + pl.row0 + qi] = m * c + __builtin_amdgcn_logf(l);
+  store_rows<L, DP>(O + qw * p.o_rs, p.o_rs, D, acc, l31, ok, h);
+}
+
+// ---- backward: dq (and delta) ----------------------------------------------------------------------------------------------------
+template <typename L, int DP, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void attn_packed_dq_kernel(const ffvc_attn_packed_desc p, int64_t slots) {
+  constexpr int BM = 32 * NW, NS = DP / 16, ND = DP / 32, TB = KB * DP * 2;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int64_t slot;
+  int head;
+  block_place(slots, p.heads, slot, head);
+  const Place pl = find_slot<BM>(p.cu, p.seqs, p.rows, slot);
+  const int64_t q0 = pl.tile * BM;
+  if (q0 < 0 || q0 >= pl.len) return;
+  const int D = p.head_dim;
+  uint16_t* dQ = (uint16_t*)p.dq + pl.row0 * p.dq_rs + head * p.dq_hs;
+  if (pl.tail) {
+    if (p.zero_tail) zero_rows(dQ + q0 * p.dq_rs, p.dq_rs, D, pl.len - q0 < BM ? pl.len - q0 : BM, tid, 64 * NW);
+    return;
+  }
+  const int kvh = head / (p.heads / p.kv_heads);
+  const uint16_t* Q = (const uint16_t*)p.q + pl.row0 * p.q_rs + head * p.q_hs;
+  const uint16_t* Kp = (const uint16_t*)p.k + pl.row0 * p.k_rs + kvh * p.k_hs;
+  const uint16_t* V = (const uint16_t*)p.v + pl.row0 * p.v_rs + kvh * p.v_hs;
+  const uint16_t* Oh = (const uint16_t*)p.out + pl.row0 * p.o_rs + head * p.o_hs;
+  const uint16_t* dO = (const uint16_t*)p.dout + pl.row0 * p.do_rs + head * p.do_hs;
+  const float c = p.scale * LOG2E;
+  TileDma<DP, NW> dk, dv;
+  dk.init(p.k_rs, D, wave, lane);
+  dv.init(p.v_rs, D, wave, lane);
+  const int64_t qend = q0 + BM < pl.len ? q0 + BM : pl.len;
+  const int nkb = (int)((qend + KB - 1) / KB);
+  auto issue = [&](int kb) {
+    const int64_t k0 = (int64_t)kb * KB;
+    unsigned char* st = smem + (kb & 1) * 2 * TB;
+    dk.issue(Kp + k0 * p.k_rs, p.k_rs, D, pl.len - k0, st, wave);
+    dv.issue(V + k0 * p.v_rs, p.v_rs, D, pl.len - k0, st + TB, wave);
+  };
+  issue(0);
+  const int64_t qw = q0 + 32 * wave;
+  const int64_t qi = qw + l31;
+  const bool ok = qi < pl.len;
+  const int64_t stat = (int64_t)head * p.rows + pl.row0 + qi;
+  u32x4_t fq[NS], fo[NS];
+  float dl = 0.0f;
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    fq[s] = row_frag(Q, p.q_rs, qi, ok, s, h, D);
+    fo[s] = row_frag(dO, p.do_rs, qi, ok, s, h, D);
+    const f32x8 a = unpack8<L>(row_frag(Oh, p.o_rs, qi, ok, s, h, D)), b = unpack8<L>(fo[s]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dl = fmaf(a.v[e], b.v[e], dl);
+  }
+  dl += other_half(dl);
+  const float ls = ok ? p.lse[stat] : 0.0f;
+  if (ok && h == 0) p.delta[stat] = dl;
+  f32x16_t acc[ND];
+#pragma unroll
+  for (int t = 0; t < ND; ++t) zero16(acc[t]);
+#pragma unroll 1
+  for (int kb = 0; kb < nkb; ++kb) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (kb + 1 < nkb) issue(kb + 1);
+    const int64_t k0 = (int64_t)kb * KB;
+    if (k0 > qw + 31 || qw >= pl.len) continue;
+    const unsigned char* sk = smem + (kb & 1) * 2 * TB;
+    const unsigned char* sv = sk + TB;
+    const bool diag = k0 + KB - 1 > qw;
+    const int lim = (int)(qi - k0);
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      f32x16_t S, dP;
+      zero16(S);
+      zero16(dP);
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        mma(S, frag_rows<DP>(sk, 32 * kt + l31, s, h), fq[s]);
+        mma(dP, frag_rows<DP>(sv, 32 * kt + l31, s, h), fo[s]);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float pr = __builtin_amdgcn_exp2f(fmaf(S[r], c, -ls));
+        const float ds = pr * (dP[r] - dl) * p.scale;
+        dP[r] = diag && 32 * kt + acc_row(r, h) > lim ? 0.0f : ds;
+      }
+#pragma unroll
+      for (int sg = 0; sg < 2; ++sg) {
+        const u32x4_t fs = pack8<L>(dP, 8 * sg);
+#pragma unroll
+        for (int t = 0; t < ND; ++t) mma(acc[t], frag_cols<DP>(sk, t, 32 * kt + 16 * sg, lane), fs);
+      }
+    }
+  }
+  store_rows<L, DP>(dQ + qw * p.dq_rs, p.dq_rs, D, acc, l31, ok, h);
+}
+
+// ---- backward: dk, dv --------------------------------------------------------------------------------------------------------------
+// NW waves x 32 keys of one key / value head; walks the query tiles that see them, for every query head of the group.
+template <typename L, int DP, int NW>
+__global__ __launch_bounds__(64 * NW, 1) void attn_packed_dkv_kernel(const ffvc_attn_packed_desc p, int64_t slots) {
+  constexpr int BM = 32 * NW, NS = DP / 16, ND = DP / 32, TB = KB * DP * 2;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int64_t slot;
+  int kvh;
+  block_place(slots, p.kv_heads, slot, kvh);
+  slot = slots - 1 - slot;                                  // the first keys are seen by the most queries: they go first
+  const Place pl = find_slot<BM>(p.cu, p.seqs, p.rows, slot);
+  const int64_t k0 = pl.tile * BM;
+  if (k0 < 0 || k0 >= pl.len) return;
+  const int D = p.head_dim;
+  uint16_t* dK = (uint16_t*)p.dk + pl.row0 * p.dk_rs + kvh * p.dk_hs;
+  uint16_t* dV = (uint16_t*)p.dv + pl.row0 * p.dv_rs + kvh * p.dv_hs;
+  if (pl.tail) {
+    if (p.zero_tail) {
+      const int64_t n = pl.len - k0 < BM ? pl.len - k0 : BM;
+      zero_rows(dK + k0 * p.dk_rs, p.dk_rs, D, n, tid, 64 * NW);
+      zero_rows(dV + k0 * p.dv_rs, p.dv_rs, D, n, tid, 64 * NW);
+    }
+    return;
+  }
+  const uint16_t* Kp = (const uint16_t*)p.k + pl.row0 * p.k_rs + kvh * p.k_hs;
+  const uint16_t* V = (const uint16_t*)p.v + pl.row0 * p.v_rs + kvh * p.v_hs;
+  const int group = p.heads / p.kv_heads;
+  const float c = p.scale * LOG2E;
+  TileDma<DP, NW> dq, dd;
+  dq.init(p.q_rs, D, wave, lane);
+  dd.init(p.do_rs, D, wave, lane);
+  const int qb0 = (int)(k0 / KB);                            // first query tile that sees any of these keys
+  const int nqb = (int)((pl.len + KB - 1) / KB);
+  const int total = (nqb - qb0) * group;
+  float* stat = (float*)(smem + 4 * TB);                     // [2 stages][lse | delta][KB]
+  int head_i = kvh * group, qb_i = qb0;                      // the next tile to fetch
+  auto issue = [&](int st_i) {
+    const int64_t r0 = (int64_t)qb_i * KB;
+    unsigned char* st = smem + st_i * 2 * TB;
+    dq.issue((const uint16_t*)p.q + (pl.row0 + r0) * p.q_rs + head_i * p.q_hs, p.q_rs, D, pl.len - r0, st, wave);
+    dd.issue((const uint16_t*)p.dout + (pl.row0 + r0) * p.do_rs + head_i * p.do_hs, p.do_rs, D, pl.len - r0, st + TB, wave);
+    if (wave < 2) {                                          // their lse and delta, zeros past the end
+      const float* src = (wave ? p.delta : p.lse) + (int64_t)head_i * p.rows + pl.row0 + r0;
+      const int n = (int)(pl.len - r0 < KB ? pl.len - r0 : KB);
+      const rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)src, 0, n * 4, 0x00020000);
+      dma4(r, lane * 4, stat + (st_i * 2 + wave) * KB);
+    }
+    if (++qb_i == nqb) {
+      qb_i = qb0;
+      ++head_i;
+    }
+  };
+  issue(0);
+  const int64_t kw = k0 + 32 * wave;
+  const int64_t ki = kw + l31;
+  const bool ok = ki < pl.len;
+  u32x4_t fk[NS], fv[NS];
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    fk[s] = row_frag(Kp, p.k_rs, ki, ok, s, h, D);
+    fv[s] = row_frag(V, p.v_rs, ki, ok, s, h, D);
+  }
+  f32x16_t aK[ND], aV[ND];
+#pragma unroll
+  for (int t = 0; t < ND; ++t) {
+    zero16(aK[t]);
+    zero16(aV[t]);
+  }
+  int qb = qb0;
+#pragma unroll 1
+  for (int it = 0; it < total; ++it) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    const int64_t r0 = (int64_t)qb * KB;
+    if (++qb == nqb) qb = qb0;
+    if (it + 1 < total) issue((it + 1) & 1);
+    if (r0 + KB - 1 < kw || kw >= pl.len) continue;          // every query of the tile is earlier than this wave's keys
+    const unsigned char* sq = smem + (it & 1) * 2 * TB;
+    const unsigned char* sd = sq + TB;
+    const float* st = stat + (it & 1) * 2 * KB;
+    const bool diag = r0 < kw + 31;
+#pragma unroll
+    for (int qt = 0; qt < 2; ++qt) {
+      f32x16_t S, dP;
+      zero16(S);
+      zero16(dP);
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        mma(S, frag_rows<DP>(sq, 32 * qt + l31, s, h), fk[s]);
+        mma(dP, frag_rows<DP>(sd, 32 * qt + l31, s, h), fv[s]);
+      }
+      const int lim = (int)(ki - r0);                         // first query of the tile that sees this lane's key
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4_t l4 = *(const f32x4_t*)(st + 32 * qt + 8 * g + 4 * h);
+        const f32x4_t d4 = *(const f32x4_t*)(st + KB + 32 * qt + 8 * g + 4 * h);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int r = 4 * g + j;
+          const bool see = !diag || 32 * qt + 8 * g + 4 * h + j >= lim;
+          const float pr = __builtin_amdgcn_exp2f(fmaf(S[r], c, -l4[j]));
+          const float ds = pr * (dP[r] - d4[j]) * p.scale;
+          S[r] = see ? pr : 0.0f;
+          dP[r] = see ? ds : 0.0f;
+        }
+      }
+#pragma unroll
+      for (int sg = 0; sg < 2; ++sg) {
+        const u32x4_t fp = pack8<L>(S, 8 * sg), fs = pack8<L>(dP, 8 * sg);
+#pragma unroll
+        for (int t = 0; t < ND; ++t) {
+          mma(aV[t], frag_cols<DP>(sd, t, 32 * qt + 16 * sg, lane), fp);
+          mma(aK[t], frag_cols<DP>(sq, t, 32 * qt + 16 * sg, lane), fs);
+        }
+      }
+    }
+  }
+  store_rows<L, DP>(dK + kw * p.dk_rs, p.dk_rs, D, aK, l31, ok, h);
+  store_rows<L, DP>(dV + kw * p.dv_rs, p.dv_rs, D, aV, l31, ok, h);
+}
+
+int check_common(const ffvc_attn_packed_desc& d, const char* who) {
+  FFVC_CHECK_ARG(d.dtype == FFVC_BF16 || d.dtype == FFVC_F16, "%s: 16-bit storage only (bf16, f16)", who);
+  FFVC_CHECK_ARG(d.rows > 0 && d.seqs > 0 && d.cu, "%s: needs rows > 0, seqs > 0 and the sequence offsets", who);
+  FFVC_CHECK_ARG(d.rows < (1ll << 31), "%s: the row offsets are 32-bit integers: rows < 2^31", who);
+  FFVC_CHECK_ARG(d.heads > 0 && d.kv_heads > 0 && d.heads % d.kv_heads == 0, "%s: heads (%d) must be a multiple of kv_heads (%d)", who, d.heads, d.kv_heads);
+  FFVC_CHECK_ARG(d.head_dim >= 8 && d.head_dim <= 128 && d.head_dim % 8 == 0, "%s: head_dim %d unsupported (a multiple of 8, at most 128)", who, d.head_dim);
+  FFVC_CHECK_ARG(d.scale > 0.0f && d.scale < INFINITY, "%s: scale must be positive and finite", who);
+  return 0;
+}
+int check_tensor(const void* ptr, int64_t rs, int64_t hs, int D, const char* who, const char* what) {
+  FFVC_CHECK_ARG(ptr && (uintptr_t)ptr % 16 == 0, "%s: %s must be non-null and 16-byte aligned", who, what);
+  FFVC_CHECK_ARG(rs % 8 == 0 && hs % 8 == 0 && rs >= D && hs >= 0, "%s: %s strides must be multiples of 8 elements, rows at least head_dim apart (row %lld, head %lld)", who, what, (long long)rs, (long long)hs);
+  FFVC_CHECK_ARG(rs < (1ll << 23), "%s: %s row stride too long", who, what);       // a tile of 64 rows stays below 2 GiB
+  return 0;
+}
+
+// one launch of KERNEL (a template-id in parentheses) over slots x HEADS workgroups
+#define LAUNCH_PACKED(KERNEL, LDS, HEADS, THREADS)                                                                                              \
+  do {                                                                                                                                          \
+    static ffvc_lds_once once__;                                                                                                                \
+    const int64_t blocks__ = slots * (HEADS);                                                                                                   \
+    FFVC_CHECK_ARG(blocks__ > 0 && blocks__ < (1ll << 31), "ffvc_attn_packed: too many tiles for one launch (%lld)", (long long)blocks__);      \
+    const int rc__ = once__.set((const void*)KERNEL, LDS);                                                                                      \
+    if (rc__) return rc__;                                                                                                                      \
+    hipLaunchKernelGGL(KERNEL, dim3((unsigned)blocks__), dim3(THREADS), LDS, st, d, slots);                                                     \
+    FFVC_LAUNCH_CHECK();                                                                                                                        \
+  } while (0)
+
+template <typename L, int DP>
+int run_fwd(const ffvc_attn_packed_desc& d, hipStream_t st) {
+  constexpr int NW = 4;
+  const int64_t slots = d.rows / (32 * NW) + d.seqs + 1;
+  LAUNCH_PACKED((attn_packed_fwd_kernel<L, DP, NW>), 4 * KB * DP * 2, d.heads, 64 * NW);
+  return 0;
+}
+template <typename L, int DP>
+int run_bwd(const ffvc_attn_packed_desc& d, hipStream_t st) {
+  constexpr int NW = 4;
+  const int64_t slots = d.rows / (32 * NW) + d.seqs + 1;
+  LAUNCH_PACKED((attn_packed_dq_kernel<L, DP, NW>), 4 * KB * DP * 2, d.heads, 64 * NW);
+  LAUNCH_PACKED((attn_packed_dkv_kernel<L, DP, NW>), 4 * KB * DP * 2 + 4 * KB * 4, d.kv_heads, 64 * NW);
+  return 0;
+}
+
+}  // namespace
+
+extern "C" int ffvc_attn_packed_fwd(const ffvc_attn_packed_desc* dp, void* stream) {
+  FFVC_CHECK_ARG(dp, "ffvc_attn_packed_fwd: null descriptor");
+  const ffvc_attn_packed_desc& d = *dp;
+  const char* who = "ffvc_attn_packed_fwd";
+  int rc = check_common(d, who);
+  if (!rc) rc = check_tensor(d.q, d.q_rs, d.q_hs, d.head_dim, who, "q");
+  if (!rc) rc = check_tensor(d.k, d.k_rs, d.k_hs, d.head_dim, who, "k");
+  if (!rc) rc = check_tensor(d.v, d.v_rs, d.v_hs, d.head_dim, who, "v");
+  if (!rc) rc = check_tensor(d.out, d.o_rs, d.o_hs, d.head_dim, who, "out");
+  if (rc) return rc;
+  hipStream_t st = (hipStream_t)stream;
+  if (d.head_dim <= 64) return d.dtype == FFVC_F16 ? run_fwd<f16_t, 64>(d, st) : run_fwd<uint16_t, 64>(d, st);
+  return d.dtype == FFVC_F16 ? run_fwd<f16_t, 128>(d, st) : run_fwd<uint16_t, 128>(d, st);
+}
+
+extern "C" int ffvc_attn_packed_bwd(const ffvc_attn_packed_desc* dp, void* stream) {
+  FFVC_CHECK_ARG(dp, "ffvc_attn_packed_bwd: null descriptor");
+  const ffvc_attn_packed_desc& d = *dp;
+  const char* who = "ffvc_attn_packed_bwd";
+  int rc = check_common(d, who);
+  if (!rc) rc = check_tensor(d.q, d.q_rs, d.q_hs, d.head_dim, who, "q");
+  if (!rc) rc = check_tensor(d.k, d.k_rs, d.k_hs, d.head_dim, who, "k");
+  if (!rc) rc = check_tensor(d.v, d.v_rs, d.v_hs, d.head_dim, who, "v");
+  if (!rc) rc = check_tensor(d.out, d.o_rs, d.o_hs, d.head_dim, who, "out");
+  if (!rc) rc = check_tensor(d.dout, d.do_rs, d.do_hs, d.head_dim, who, "dout");
+  if (!rc) rc = check_tensor(d.dq, d.dq_rs, d.dq_hs, d.head_dim, who, "dq");
+  if (!rc) rc = check_tensor(d.dk, d.dk_rs, d.dk_hs, d.head_dim, who, "dk");
+  if (!rc) rc = check_tensor(d.dv, d.dv_rs, d.dv_hs, d.head_dim, who, "dv");
+  if (rc) return rc;
+  FFVC_CHECK_ARG(d.lse && d.delta, "ffvc_attn_packed_bwd: needs the forward's lse and the delta workspace");
+  hipStream_t st = (hipStream_t)stream;
+  if (d.head_dim <= 64) return d.dtype == FFVC_F16 ? run_bwd<f16_t, 64>(d, st) : run_bwd<uint16_t, 64>(d, st);
+  return d.dtype == FFVC_F16 ? run_bwd<f16_t, 128>(d, st) : run_bwd<uint16_t, 128>(d, st);
+}

@@ -3,6 +3,9 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <stdio.h>
+
+#include <atomic>
+
 #include "../../include/ffvc.h"
 
 #define FFVC_WAVE 64
@@ -35,6 +38,24 @@ void ffvc_set_error(const char* fmt, ...);
       return (int)e__;                                                   \
     }                                                                    \
   } while (0)
+
+// The dynamic-LDS limit of one kernel, raised once per device (a static of each launcher; launchers may run on several threads).
+struct ffvc_lds_once {
+  std::atomic<uint64_t> done{0};
+  int set(const void* kernel, int bytes) {
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    const uint64_t bit = 1ull << (dev & 63);
+    if (e == hipSuccess && (done.load(std::memory_order_relaxed) & bit)) return 0;
+    if (e == hipSuccess) e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != hipSuccess) {
+      ffvc_set_error("dynamic LDS limit: %s", hipGetErrorString(e));
+      return (int)e;
+    }
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return 0;
+  }
+};
 
 // ---- bf16 <-> f32 (round-to-nearest-even, NaN preserved) ------------------
 __device__ __forceinline__ float bf16_bits_to_f32(uint16_t b) {

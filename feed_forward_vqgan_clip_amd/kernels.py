@@ -1558,3 +1558,211 @@ def avgpool_patches_bwd(gout, N, S, out_size, patch, std):
     _call("ffvc_avgpool_patches_bwd", gout.data_ptr(), dtype_code(gout.dtype), dx.data_ptr(), N, S, out_size, patch, std[0],
           std[1], std[2], stream_ptr())
     return dx
+
+
+# ---------------------------------------------------------------------------
+# packed prompts: embedding, causal attention over sequences of different lengths, 8-bit integer Linear
+# ---------------------------------------------------------------------------
+def _same_device(*ts):
+    """Context in which these tensors' device is the current one (the launch goes to ITS current stream); they must share it."""
+    dev = None
+    for t in ts:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise _lib.FFVCError("ffvc kernels need CUDA(HIP) tensors; there is no CPU fallback")
+        if dev is not None and t.device != dev:
+            raise ValueError(f"ffvc launcher: tensors on {dev} and {t.device}")
+        dev = t.device
+    return torch.cuda.device(dev)
+
+
+def _rows2d(name, t):
+    """A 2-d tensor whose rows are contiguous; returns its row stride."""
+    if t.dim() != 2:
+        raise ValueError(f"{name}: expected a 2-d tensor, got {tuple(t.shape)}")
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name}: the elements of a row must be contiguous (strides {t.stride()})")
+    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], t.stride(0))
+
+
+def _ids(name, t, n=None):
+    if t.dtype != torch.int64 or not t.is_contiguous():
+        raise TypeError(f"{name}: expected contiguous int64 indices, got {t.dtype}")
+    if n is not None and t.numel() != n:
+        raise ValueError(f"{name}: {t.numel()} indices for {n} tokens")
+
+
+def embed_fwd(ids, table, scale=1.0, pos=None, pos_ids=None, out_dtype=None):
+    """scale * table[ids] (+ pos[pos_ids]; pos_ids None: row t for token t) -> [*ids.shape, dim].  Indices outside their table read zero rows."""
+    _ids("embed_fwd", ids)
+    if pos_ids is not None:
+        _ids("embed_fwd: pos_ids", pos_ids, ids.numel())
+    ld = _rows2d("embed_fwd: table", table)
+    V, dim = table.shape
+    pld = npos = 0
+    if pos is not None:
+        pld, npos = _rows2d("embed_fwd: pos", pos), pos.shape[0]
+        if pos.shape[1] != dim or pos.dtype != table.dtype:
+            raise ValueError("embed_fwd: pos must have the table's width and dtype")
+    code = dtype_code(table.dtype)
+    with _same_device(ids, table, pos, pos_ids):
+        out = torch.empty(*ids.shape, dim, dtype=out_dtype or table.dtype, device=table.device)
+        if out.numel():
+            if V < 1 or (pos is not None and npos < 1):
+                raise ValueError("embed_fwd: empty table")
+            _call("ffvc_embed_fwd", table.data_ptr(), code, ld, V, ids.data_ptr(), float(scale), _ptr(pos), pld, npos, _ptr(pos_ids), out.data_ptr(),
+                  dtype_code(out.dtype), dim, ids.numel(), dim, stream_ptr())
+    return out
+
+
+def embed_bwd(dout, ids, rows, scale=1.0, out_dtype=None):
+    """The gradient of a table of `rows` rows that was read with `ids`: scale * sum of the tokens' dout rows, every row written."""
+    _ids("embed_bwd", ids)
+    dim = dout.shape[-1]
+    if tuple(dout.shape[:-1]) != tuple(ids.shape):
+        raise ValueError(f"embed_bwd: dout {tuple(dout.shape)} for indices {tuple(ids.shape)}")
+    d2 = dout.reshape(-1, dim)
+    ld = _rows2d("embed_bwd: dout", d2)
+    n = ids.numel()
+    with _same_device(dout, ids):
+        dt = out_dtype or dout.dtype
+        if n == 0 or rows == 0 or dim == 0:
+            return torch.zeros(rows, dim, dtype=dt, device=dout.device)
+        grad = torch.empty(rows, dim, dtype=dt, device=dout.device)
+        nb = int(_lib.load().ffvc_embed_bwd_ws_bytes(n, dim))
+        ws = torch.empty(nb, dtype=torch.uint8, device=dout.device)
+        _call("ffvc_embed_bwd", d2.data_ptr(), dtype_code(d2.dtype), ld, ids.data_ptr(), n, rows, dim, float(scale), grad.data_ptr(), dtype_code(dt),
+              ws.data_ptr(), nb, stream_ptr())
+    return grad
+
+
+def _heads3d(name, t, like=None):
+    """(rows, heads, head_dim) with contiguous features; returns (row stride, head stride)."""
+    if t.dim() != 3 or (like is not None and tuple(t.shape) != tuple(like)):
+        raise ValueError(f"{name}: expected {'(rows, heads, head_dim)' if like is None else tuple(like)}, got {tuple(t.shape)}")
+    if t.stride(2) != 1 and t.shape[2] > 1:
+        raise ValueError(f"{name}: the features of a head must be contiguous (strides {t.stride()})")
+    T, H, D = t.shape
+    return (t.stride(0) if T > 1 else max(H * D, t.stride(0))), (t.stride(1) if H > 1 else D)
+
+
+def _attn_packed_desc(q, k, v, cu, scale):
+    if q.dtype not in LOWP:
+        raise TypeError(f"attn_packed: 16-bit tensors only (bf16, f16), got {q.dtype}")
+    for n, t in (("k", k), ("v", v)):
+        if t.dtype != q.dtype:
+            raise TypeError(f"attn_packed: {n} is {t.dtype}, q is {q.dtype}")
+    if cu.dtype != torch.int32 or cu.dim() != 1 or cu.numel() < 2 or not cu.is_contiguous():
+        raise TypeError("attn_packed: cu_seqlens must be a contiguous int32 vector of at least two offsets")
+    T, H, D = q.shape
+    d = _lib.AttnPackedDesc()
+    d.rows, d.seqs, d.heads, d.kv_heads, d.head_dim = T, cu.numel() - 1, H, k.shape[1], D
+    d.dtype, d.scale, d.cu = dtype_code(q.dtype), float(scale), cu.data_ptr()
+    d.q, (d.q_rs, d.q_hs) = q.data_ptr(), _heads3d("attn_packed: q", q)
+    d.k, (d.k_rs, d.k_hs) = k.data_ptr(), _heads3d("attn_packed: k", k, (T, k.shape[1], D))
+    d.v, (d.v_rs, d.v_hs) = v.data_ptr(), _heads3d("attn_packed: v", v, (T, k.shape[1], D))
+    return d
+
+
+def attn_packed_fwd(q, k, v, cu_seqlens, scale, out=None, want_lse=False):
+    """Causal attention over packed sequences: q (rows, heads, head_dim), k / v (rows, kv_heads, head_dim), views of one projection included;
+    cu_seqlens int32 [sequences + 1] on the device -> (out (rows, heads, head_dim), lse fp32 (heads, rows) or None).  Without `out` the rows
+    behind the last sequence come as zeros; a given `out` keeps what it holds there."""
+    d = _attn_packed_desc(q, k, v, cu_seqlens, scale)
+    T, H, D = q.shape
+    with _same_device(q, k, v, cu_seqlens, out):
+        d.zero_tail = int(out is None)
+        if out is None:
+            out = torch.empty(T, H, D, dtype=q.dtype, device=q.device)
+        elif out.dtype != q.dtype:
+            raise TypeError(f"attn_packed: out is {out.dtype}, q is {q.dtype}")
+        d.out, (d.o_rs, d.o_hs) = out.data_ptr(), _heads3d("attn_packed: out", out, (T, H, D))
+        lse = torch.empty(H, T, dtype=torch.float32, device=q.device) if want_lse else None
+        d.lse = _ptr(lse)
+        if T:
+            _call("ffvc_attn_packed_fwd", byref(d), stream_ptr())
+    return out, lse
+
+
+def attn_packed_bwd(q, k, v, out, dout, lse, cu_seqlens, scale, dq, dk, dv):
+    """Gradients of attn_packed_fwd into dq, dk, dv (views of one packed gradient included); rows behind the last sequence become zeros."""
+    d = _attn_packed_desc(q, k, v, cu_seqlens, scale)
+    T, H, D = q.shape
+    for n, t, like in (("out", out, q), ("dout", dout, q), ("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
+        if t.dtype != q.dtype:
+            raise TypeError(f"attn_packed_bwd: {n} is {t.dtype}, q is {q.dtype}")
+        f = "o" if n == "out" else ("do" if n == "dout" else n)
+        setattr(d, n, t.data_ptr())
+        rs, hs = _heads3d(f"attn_packed_bwd: {n}", t, tuple(like.shape))
+        setattr(d, f + "_rs", rs)
+        setattr(d, f + "_hs", hs)
+    _req_f32(lse)
+    if tuple(lse.shape) != (H, T):
+        raise ValueError("attn_packed_bwd: lse does not belong to these tensors")
+    with _same_device(q, k, v, out, dout, lse, cu_seqlens, dq, dk, dv):
+        delta = torch.empty_like(lse)
+        d.lse, d.delta, d.zero_tail = lse.data_ptr(), delta.data_ptr(), 1
+        if T:
+            _call("ffvc_attn_packed_bwd", byref(d), stream_ptr())
+
+
+def int8_quant(x):
+    """Rows of x [..., K] (K a multiple of 16) -> (int8 [..., K], fp32 scale [...]): scale = max |x| / 127, q = round-half-even(x / scale)."""
+    if x.dim() < 1 or x.shape[-1] % 16 or x.shape[-1] == 0:
+        raise ValueError(f"int8_quant: the row length must be a multiple of 16, got {tuple(x.shape)}")
+    K = x.shape[-1]
+    x2 = x.reshape(-1, K)
+    code = dtype_code(x.dtype)
+    ld = _rows2d("int8_quant", x2)
+    with _same_device(x):
+        if x2.data_ptr() % 16 or (ld * x2.element_size()) % 16:
+            x2, ld = x2.contiguous() if x2.data_ptr() % 16 == 0 else x2.clone(), K
+        q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+        s = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        if x2.shape[0]:
+            _call("ffvc_int8_quant", x2.data_ptr(), code, ld, q.data_ptr(), K, s.data_ptr(), x2.shape[0], K, stream_ptr())
+    return q, s
+
+
+def linear_int8(x, wq, ws, bias=None, act=ACT_NONE, residual=None, out_dtype=None, want_actgrad=False):
+    """act(x W^T + bias) (+ residual) with x [..., K] 16-bit and (wq, ws) = int8_quant(W) of a weight [N, K]: x is quantised row by row, the
+    products are summed exactly in 32-bit integers.  out_dtype: x's (default) or fp32.  want_actgrad: -> (y, act'(pre-activation))."""
+    if x.dtype not in LOWP:
+        raise TypeError(f"linear_int8: 16-bit activations only (bf16, f16), got {x.dtype}")
+    _req(torch.int8, wq)
+    _req_f32(ws, bias)
+    N, K = wq.shape
+    if x.dim() < 1 or x.shape[-1] != K:
+        raise ValueError(f"linear_int8: x {tuple(x.shape)} against a weight {tuple(wq.shape)}")
+    if tuple(ws.shape) != (N,) or (bias is not None and tuple(bias.shape) != (N,)):
+        raise ValueError("linear_int8: one scale and one bias per output channel")
+    out_dtype = out_dtype or x.dtype
+    if out_dtype not in (x.dtype, torch.float32):
+        raise TypeError(f"linear_int8: output {out_dtype} from {x.dtype} activations")
+    shape = (*x.shape[:-1], N)
+    if residual is not None:
+        if tuple(residual.shape) != shape:
+            raise ValueError(f"linear_int8: residual {tuple(residual.shape)} for an output {shape}")
+        _req(residual.dtype if residual.dtype in (x.dtype, torch.float32) else out_dtype, residual)
+    x2 = x.reshape(-1, K)
+    ld = _rows2d("linear_int8: x", x2)
+    M = x2.shape[0]
+    with _same_device(x, wq, ws, bias, residual):
+        if x2.data_ptr() % 16 or ld % 8:
+            x2, ld = x2.clone(memory_format=torch.contiguous_format), K
+        y = torch.empty(shape, dtype=out_dtype, device=x.device)
+        g = torch.empty(shape, dtype=x.dtype, device=x.device) if want_actgrad else None
+        if M:
+            lo, rdt = dtype_code(x.dtype), dtype_code(residual.dtype if residual is not None else out_dtype)
+            lib = _lib.load()
+            if lib.ffvc_linear_int8_few_ok(M, K):
+                _call("ffvc_linear_int8_few", x2.data_ptr(), lo, ld, wq.data_ptr(), K, ws.data_ptr(), _ptr(bias), act, _ptr(residual), rdt, N,
+                      y.data_ptr(), dtype_code(out_dtype), N, _ptr(g), M, N, K, stream_ptr())
+            else:
+                xq = torch.empty(M, K, dtype=torch.int8, device=x.device)
+                xs = torch.empty(M, dtype=torch.float32, device=x.device)
+                _call("ffvc_int8_quant", x2.data_ptr(), lo, ld, xq.data_ptr(), K, xs.data_ptr(), M, K, stream_ptr())
+                _call("ffvc_gemm_int8", xq.data_ptr(), K, xs.data_ptr(), wq.data_ptr(), K, ws.data_ptr(), _ptr(bias), act, _ptr(residual), rdt, N,
+                      y.data_ptr(), dtype_code(out_dtype), N, _ptr(g), lo, M, N, K, stream_ptr())
+    return (y, g) if want_actgrad else y

@@ -247,9 +247,11 @@ def clip_arch(model_type):
     return arch, quick
 
 
-def load_clip_model(model_type, path=None, cdt=torch.float16, fp8=False):
+def load_clip_model(model_type, path=None, cdt=torch.float16, fp8=False, int8=False, text_packed=False):
     """main.py:1308-1333 for the OpenAI / OpenCLIP ViT families (state_dict in clip.model.CLIP layout).
-    fp8: image-tower linears on the fp8 MFMA path (config key `clip_fp8`)."""
+    fp8: image-tower linears on the fp8 MFMA path (config key `clip_fp8`).
+    int8: the same linears in 8-bit integers, scales per token and channel (config key `clip_int8`); text_packed: the text tower over packed
+    prompts in the compute dtype (the `encode_text` command's --packed)."""
     arch, quick = clip_arch(model_type)
     if path is None or str(path).startswith("random:"):
         seed = int(str(path).split(":", 1)[1]) if path else 1234
@@ -257,7 +259,7 @@ def load_clip_model(model_type, path=None, cdt=torch.float16, fp8=False):
     else:
         obj = torch.load(path, map_location="cpu", weights_only=False)
         sd = obj.state_dict() if hasattr(obj, "state_dict") else obj.get("state_dict", obj)
-    return _clip.CLIP(sd, cdt, quick_gelu=quick, fp8=fp8)
+    return _clip.CLIP(sd, cdt, quick_gelu=quick, fp8=fp8, int8=int8, text_packed=text_packed)
 
 
 def synthetic_tokens(n, seed=0, context_length=77):
@@ -317,16 +319,20 @@ def clip_dim_size(config):
     return dim, size
 
 
-def encode_text(data_path, out="text_features.pkl", clip_model="ViT-B/32", clip_path=None, batch_size=256, bpe_path=None):
+def encode_text(data_path, out="text_features.pkl", clip_model="ViT-B/32", clip_path=None, batch_size=256, bpe_path=None, packed=False, int8=False):
     """Text-feature cache: run the frozen text tower ONCE over a prompt dataset and save the fp32
     features; `train` on the resulting `.pkl` takes the pre-computed-feature branch of main.py:733,737 (anything that is
-    not torch.long is used as features), so the text tower leaves the training step altogether."""
+    not torch.long is used as features), so the text tower leaves the training step altogether.
+    packed: run the prompts' own tokens packed behind one another instead of 77 padded ones each, in 16-bit arithmetic (int8: with the Linear
+    layers in 8-bit integers); the default is the fp32-grade padded tower."""
+    if int8 and not packed:
+        raise ValueError("encode_text: int8 needs packed (the padded tower stays at fp32 grade)")
     toks = load_dataset(data_path, bpe_path=bpe_path)
     toks = toks[0] if isinstance(toks, tuple) else toks
     if toks.dtype != torch.long:
         raise TypeError("encode_text: the dataset already holds features")
-    perceptor = load_clip_model(clip_model, path=clip_path)
-    feats = torch.cat([perceptor.encode_text(toks[i:i + batch_size].cuda()).float().cpu()
+    perceptor = load_clip_model(clip_model, path=clip_path, int8=int8, text_packed=packed)
+    feats = torch.cat([perceptor.encode_text(toks[i:i + batch_size] if packed else toks[i:i + batch_size].cuda()).float().cpu()
                        for i in range(0, len(toks), batch_size)])
     torch.save(feats, out)
     return feats
@@ -738,7 +744,8 @@ def train(config_file):
         os.environ["FFVC_SK_FIXUP"] = "0"
     toks = load_dataset(config.path)
     vq = load_vqgan_model(config.vqgan_config, config.vqgan_checkpoint, cdt, fp8=bool(config.get("decoder_fp8", False)))
-    perceptor = load_clip_model(config.clip_model, path=config.get("clip_model_path"), cdt=cdt, fp8=bool(config.get("clip_fp8", False)))
+    perceptor = load_clip_model(config.clip_model, path=config.get("clip_model_path"), cdt=cdt, fp8=bool(config.get("clip_fp8", False)),
+                                int8=bool(config.get("clip_int8", False)))
     vq_channels = vq.codebook.shape[1]
     checkpoint_path = os.path.join(config.folder, "checkpoint.th")
     checkpoint_ema_path = os.path.join(config.folder, "checkpoint_ema.th")
@@ -906,7 +913,8 @@ def test(model_path, text_or_path, *, nb_repeats=1, out_path="gen.png", images_p
         torch.manual_seed(seed)
     net = load_model(model_path, cdt)
     config = net.config
-    perceptor = load_clip_model(config.clip_model, path=config.get("clip_model_path"), cdt=cdt, fp8=bool(config.get("clip_fp8", False)))
+    perceptor = load_clip_model(config.clip_model, path=config.get("clip_model_path"), cdt=cdt, fp8=bool(config.get("clip_fp8", False)),
+                                int8=bool(config.get("clip_int8", False)))
     vq = load_vqgan_model(config.vqgan_config, config.vqgan_checkpoint, cdt)
     if text_or_path.startswith("synthetic:") or text_or_path.endswith(".pkl"):
         toks = load_dataset(text_or_path)
@@ -957,13 +965,16 @@ def _cli(argv):
         tokenize(argv[1], *(argv[2:3] or ["tokenized.pkl"]))
         return 0
     if len(argv) >= 2 and argv[0] == "encode_text":
-        encode_text(argv[1], *(argv[2:3] or ["text_features.pkl"]))
-        return 0
+        flags = [a for a in argv[1:] if a.startswith("--")]
+        rest = [a for a in argv[1:] if not a.startswith("--")]
+        if rest and not set(flags) - {"--packed", "--int8"}:
+            encode_text(rest[0], *(rest[1:2] or ["text_features.pkl"]), packed="--packed" in flags, int8="--int8" in flags)
+            return 0
     if len(argv) >= 2 and argv[0] == "encode_text_and_images":
         encode_text_and_images(argv[1], out=(argv[2:3] or ["features.pkl"])[0])
         return 0
     print("usage: python -m feed_forward_vqgan_clip_amd.main train <config.yaml> | test <model.th> <prompts> [...] | "
-          "tokenize <prompts> [out.pkl] | encode_text <dataset> [out.pkl] | encode_text_and_images <folder> [out.pkl]",
+          "tokenize <prompts> [out.pkl] | encode_text <dataset> [out.pkl] [--packed [--int8]] | encode_text_and_images <folder> [out.pkl]",
           file=sys.stderr)
     return 2
 

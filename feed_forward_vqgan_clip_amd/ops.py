@@ -36,26 +36,34 @@ from .kernels import ACT_GELU, ACT_NONE, ACT_QUICKGELU  # noqa: F401
 class Weights:
     """fp32 master weight [N, K] (+ bias [N]) with compute-dtype shadows."""
 
-    __slots__ = ("weight", "bias", "sh", "sht", "N", "K", "on_grad", "fp8", "group")
+    __slots__ = ("weight", "bias", "sh", "sht", "N", "K", "on_grad", "fp8", "int8", "group")
 
     def __init__(self, weight, bias, sh, sht, on_grad=None):
         self.weight, self.bias, self.sh, self.sht = weight, bias, sh, sht
         self.N, self.K = sh.shape[0], sh.shape[1]
         self.on_grad = on_grad
         self.fp8 = None
+        self.int8 = None            # (int8 weight, fp32 scale per output channel) of a frozen layer
         self.group = None           # (WgradGroup, index): weight gradient deferred into a grouped launch (group_weights)
 
     @staticmethod
-    def frozen(weight, bias, cdt, need_dgrad=True, fp8=False):
+    def frozen(weight, bias, cdt, need_dgrad=True, fp8=False, int8=False):
         """Build shadows once for a frozen layer; weight: fp32 [N, K] (any device -> cuda).
         fp8: also keep OCP e4m3 copies of W and W^T (one per-tensor scale, quantised from the fp32 master) plus the delayed
         scaling state of the layer's activation (e4m3) and gradient (e5m2) streams: Linear fwd / dgrad then run on the
-        fp8 MFMA path (ffvc_gemm_fp8).  Needs 16-element aligned N and K."""
+        fp8 MFMA path (ffvc_gemm_fp8).  Needs 16-element aligned N and K.
+        int8: also keep the weight in 8-bit integers with one scale per output channel: Linear forward quantises its input row by row and
+        runs on kernels.linear_int8; the dgrad passes the quantisation straight through and reads the 16-bit W^T.  Needs K % 16 == 0."""
+        if int8 and (fp8 or cdt not in K.LOWP or weight[0].numel() % 16):
+            raise ValueError("int8 weights need a 16-bit compute dtype, K a multiple of 16 and exclude fp8 "
+                             f"(K={weight[0].numel()}, {cdt}, fp8={bool(fp8)})")
         w = weight.detach().reshape(weight.shape[0], -1).float().cuda().contiguous()
         b = None if bias is None else bias.detach().float().cuda().contiguous()
         sh = K.cast(w, cdt) if cdt != torch.float32 else w
         sht = K.transpose(w, cdt) if need_dgrad else None
         W = Weights(None, b, sh, sht)
+        if int8:
+            W.int8 = K.int8_quant(w)
         if fp8:
             if cdt not in K.LOWP or W.N % 16 or W.K % 16:
                 raise ValueError(f"fp8 weights need a 16-bit compute dtype and N, K multiples of 16 (N={W.N}, K={W.K})")
@@ -409,6 +417,9 @@ class _LinearFn(Function):
             if residual is not None and (residual.dtype != torch.float32 or y.dtype != torch.float32):
                 raise TypeError("linear(drop>0) with a residual needs the fp32 residual stream")
             K.dropout(y, ctx.drop[0], ctx.drop[1], residual=residual, out=y)
+        elif W.int8 is not None and not gn_hw and x.dtype in K.LOWP:
+            _f8_twin(x, None)
+            y = K.linear_int8(x, *W.int8, bias=W.bias, residual=residual, out_dtype=y.dtype)
         elif W.fp8 is not None and not gn_hw and x.dtype in K.LOWP:
             f = W.fp8                  # fp8 MFMA path of a frozen layer: quantise the activation, per-tensor delayed scale
             x8 = _f8_twin(x, f["x"])
@@ -473,6 +484,19 @@ class _MLPFn(Function):
         cdt = W1.sh.dtype
         x = _contig(x)
         rows = x.numel() // W1.K
+        ctx.fp8 = False
+        if W1.int8 is not None and W2.int8 is not None and not drop and x.dtype in K.LOWP:
+            # frozen 8-bit MLP: the first product's epilogue also stores act'(pre), the only thing the backward pass needs
+            _f8_twin(x, None)
+            ctx.ag, ctx.drop, h_pre = K.F_AUX_ACTGRAD, None, None
+            if ctx.needs_input_grad[0]:
+                h, h_pre = K.linear_int8(x, *W1.int8, bias=W1.bias, act=act, want_actgrad=True)
+            else:
+                h = K.linear_int8(x, *W1.int8, bias=W1.bias, act=act)
+            ctx.W1, ctx.W2, ctx.rows, ctx.act, ctx.train, ctx.has_res = W1, W2, rows, act, False, residual is not None
+            ctx.save_for_backward(None, h_pre, None)
+            ctx.xshape = x.shape
+            return K.linear_int8(h, *W2.int8, bias=W2.bias, residual=residual, out_dtype=out_dtype or cdt)
         h_pre = torch.empty(*x.shape[:-1], W1.N, dtype=cdt, device=x.device)
         h = torch.empty_like(h_pre)
         ctx.fp8 = (W1.fp8 is not None and W2.fp8 is not None and not drop and x.dtype in K.LOWP)
@@ -1023,6 +1047,77 @@ class _AttentionFn(Function):
 def attention(qkv, heads, scale, causal=False, f8_for=None):
     """f8_for: the frozen fp8 `Weights` pack of the projection that consumes the result (see layernorm_fork)."""
     return _AttentionFn.apply(qkv, heads, scale, causal, f8_for)
+
+
+class _AttentionPackedFn(Function):
+    """Causal attention over packed sequences; keeps qkv, the output and the row statistics (no score matrix)."""
+
+    @staticmethod
+    def forward(ctx, qkv, cu, heads, kv_heads, scale):
+        q, k, v = _split_heads(qkv, heads, kv_heads)
+        o, lse = K.attn_packed_fwd(q, k, v, cu, scale, want_lse=ctx.needs_input_grad[0])
+        ctx.save_for_backward(qkv, cu, o, lse)
+        ctx.cfg = (heads, kv_heads, scale)
+        return o.view(qkv.shape[0], -1)
+
+    @staticmethod
+    def backward(ctx, do):
+        qkv, cu, o, lse = ctx.saved_tensors
+        heads, kv_heads, scale = ctx.cfg
+        do = _as(_contig(do), qkv.dtype).view(o.shape)
+        dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+        K.attn_packed_bwd(*_split_heads(qkv, heads, kv_heads), o, do, lse, cu, scale, *_split_heads(dqkv, heads, kv_heads))
+        return dqkv, None, None, None, None
+
+
+def _split_heads(qkv, heads, kv_heads):
+    """[rows, (heads + 2 kv_heads) * dh] -> views q (rows, heads, dh), k, v (rows, kv_heads, dh)."""
+    dh = qkv.shape[1] // (heads + 2 * kv_heads)
+    return tuple(qkv[:, a * dh:(a + n) * dh].unflatten(1, (n, dh)) for a, n in ((0, heads), (heads, kv_heads), (heads + kv_heads, kv_heads)))
+
+
+def attention_packed(qkv, cu_seqlens, heads, kv_heads=None, scale=None):
+    """Causal attention over sequences packed behind one another (the text tower without its padding, cloob.py:199-200,510-516).
+
+    qkv: [rows, (heads + 2 * kv_heads) * dh] 16-bit, the packed projection q | k | v (kv_heads None: as many as heads; otherwise consecutive groups
+    of heads / kv_heads query heads share one key / value head); a slice of wider rows is fine.  cu_seqlens: int32 [sequences + 1] on the device,
+    rows cu[b] .. cu[b+1]-1 are sequence b; empty sequences and rows behind the last one are allowed (those come out as zeros, and so do
+    their gradients).  -> [rows, heads * dh]; gradients flow to qkv."""
+    kv_heads = heads if kv_heads is None else kv_heads
+    if qkv.dim() != 2 or heads < 1 or kv_heads < 1 or heads % kv_heads or qkv.shape[1] % (heads + 2 * kv_heads):
+        raise ValueError(f"attention_packed: a [rows, (heads + 2 kv_heads) * dh] projection is expected, got {tuple(qkv.shape)} for {heads} / {kv_heads} heads")
+    dh = qkv.shape[1] // (heads + 2 * kv_heads)
+    if dh % 8 or not 8 <= dh <= 128:
+        raise ValueError(f"attention_packed: head width {dh} unsupported (a multiple of 8, at most 128)")
+    return _AttentionPackedFn.apply(qkv, cu_seqlens, heads, kv_heads, default_scale(dh) if scale is None else scale)
+
+
+class _EmbeddingFn(Function):
+    @staticmethod
+    def forward(ctx, table, pos, ids, pos_ids, scale, out_dtype):
+        ctx.save_for_backward(ids, pos_ids)
+        ctx.cfg = (table.shape[0], table.dtype, None if pos is None else pos.shape[0], scale)
+        return K.embed_fwd(ids, table, scale, pos, pos_ids, out_dtype)
+
+    @staticmethod
+    def backward(ctx, g):
+        ids, pos_ids = ctx.saved_tensors
+        V, dt, P, scale = ctx.cfg
+        g = _contig(g)
+        dtable = K.embed_bwd(g, ids, V, scale, dt) if ctx.needs_input_grad[0] else None
+        dpos = None
+        if P is not None and ctx.needs_input_grad[1]:
+            at = pos_ids if pos_ids is not None else torch.arange(ids.numel(), device=ids.device)
+            dpos = K.embed_bwd(g, at.view(ids.shape), P, 1.0, dt)
+        return dtable, dpos, None, None, None, None
+
+
+def embedding(ids, table, scale=1.0, pos=None, pos_ids=None, out_dtype=None):
+    """scale * table[ids] + pos[pos_ids]: token (+ position) embedding (cloob.py:526-528), differentiable in both tables.
+
+    ids (and pos_ids): int64; an index outside its table (e.g. -1 for the unused rows of a buffer) reads a zero row and gets no gradient.
+    pos without pos_ids: row t for the t-th token.  The gradients are sums over the sorted tokens: no atomics, the same bits every time."""
+    return _EmbeddingFn.apply(table, pos, ids, pos_ids, float(scale), out_dtype)
 
 
 class _AttentionTinyFn(Function):

@@ -552,6 +552,66 @@ int ffvc_tokmix_fwd_save(const void* xn, const void* w1, const float* b1, const 
 int ffvc_tokmix_bwd_hidden(const void* xn, const void* dy, const void* w1, const float* b1, const void* w2t, void* h,
                            void* dh, float* db1, int dtype, int B, int T, int D, int O, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Packed prompts: the text tower (cloob.py:525-538) over the prompts' own tokens instead of 77 padded ones, forward and backward
+ * (the causal mask of cloob.py:510-516 makes a prompt's features independent of what stands behind its last token).
+ * ------------------------------------------------------------------------- */
+
+/* out[t] = scale * table[ids[t]] + pos[place[t]], t < n (cloob.py:526-528 with a scale).  table: [vocab] rows of dim, `ld` elements apart;
+ * pos (may be NULL): npos rows of table's dtype; place (may be NULL: t itself) int64.  An id / place outside its table reads a zero row. */
+int ffvc_embed_fwd(const void* table, int table_dtype, int64_t ld, int64_t vocab, const int64_t* ids, float scale, const void* pos, int64_t pos_ld,
+                   int64_t npos, const int64_t* place, void* out, int out_dtype, int64_t ldo, int64_t n, int dim, void* stream);
+/* dtable[v] = scale * sum_{t: ids[t] = v} dout[t] for every row v of the contiguous [vocab, dim] gradient (rows without a token are written as
+ * zeros; ids outside the table add nothing).  Summed in fp32 in the order of t: the same bits on every call.  ws: ffvc_embed_bwd_ws_bytes(n,
+ * dim) bytes, 16-byte aligned, contents irrelevant before and after. */
+int64_t ffvc_embed_bwd_ws_bytes(int64_t n, int dim);
+int ffvc_embed_bwd(const void* dout, int dout_dtype, int64_t ld, const int64_t* ids, int64_t n, int64_t vocab, int dim, float scale, void* dtable,
+                   int table_dtype, void* ws, int64_t ws_bytes, void* stream);
+
+/* Causal attention over packed sequences with grouped heads (cloob.py:199-200 under :510-516, one launch for prompts of any lengths).
+ * Rows cu[b] .. cu[b+1]-1 are sequence b (cu: int32 [seqs + 1] on the device, ascending from 0; offsets outside [0, rows] are clamped); query i of a
+ * sequence sees its keys 0 .. i; query heads h share key / value head h / (heads / kv_heads).  Element (row, head, feature) of a tensor sits
+ * at row * ?_rs + head * ?_hs + feature: any of them may be a slice of a packed projection.  Rows behind cu[seqs]: left as they were, or
+ * zeroed with zero_tail (out; dq, dk, dv).  head_dim: a multiple of 8 up to 128; strides multiples of 8, 16-byte aligned pointers; dtype
+ * FFVC_BF16 | FFVC_F16, statistics and accumulators fp32.
+ * Forward: q, k, v, out, cu; lse (may be NULL) fp32 [heads][rows] <- base-2 log-sum-exp.  Backward: also dout, dq, dk, dv, the forward's out
+ * and lse, and delta: fp32 [heads][rows] scratch.  No atomics: the same bits on every call. */
+typedef struct ffvc_attn_packed_desc {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  float* lse;
+  const int32_t* cu;
+  const void* dout;
+  void* dq;
+  void* dk;
+  void* dv;
+  float* delta;
+  int64_t rows;
+  int64_t q_rs, q_hs, k_rs, k_hs, v_rs, v_hs, o_rs, o_hs;
+  int64_t do_rs, do_hs, dq_rs, dq_hs, dk_rs, dk_hs, dv_rs, dv_hs;
+  int32_t seqs, heads, kv_heads, head_dim, dtype, zero_tail;
+  float scale;
+} ffvc_attn_packed_desc;
+int ffvc_attn_packed_fwd(const ffvc_attn_packed_desc* d, void* stream);
+int ffvc_attn_packed_bwd(const ffvc_attn_packed_desc* d, void* stream);
+
+/* Linear in 8-bit integers with one scale per token and one per channel (the Linear layers of cloob.py:188-200 for frozen weights):
+ *   scale[r] = max_k |x[r, k]| / 127,  q = round-half-even(x / scale)     (ffvc_int8_quant: activations and weight rows alike)
+ *   y[m, n]  = act(xs[m] * ws[n] * sum_k x[m, k] w[n, k] + bias[n]) + residual[m, n]
+ * The integer sum is exact.  A row with an inf or NaN gets a NaN scale.  act: NONE | GELU | QUICKGELU; actgrad (may be NULL): contiguous
+ * [M, N] of lo_dtype <- act'(pre-activation); y / residual fp32 or lo_dtype; K a multiple of 16 up to 131072, any M and N.
+ * ffvc_linear_int8_few: the same for up to 16 rows straight from 16-bit x, quantised inside the launch (ffvc_linear_int8_few_ok). */
+int ffvc_int8_quant(const void* x, int x_dtype, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t rows, int K, void* stream);
+int ffvc_gemm_int8(const int8_t* x, int64_t ldx, const float* xs, const int8_t* w, int64_t ldw, const float* ws, const float* bias, int act,
+                   const void* residual, int res_dtype, int64_t ldr, void* y, int y_dtype, int64_t ldy, void* actgrad, int lo_dtype, int M, int N, int K,
+                   void* stream);
+int ffvc_linear_int8_few_ok(int M, int K);
+int ffvc_linear_int8_few(const void* x, int lo_dtype, int64_t ldx, const int8_t* w, int64_t ldw, const float* ws, const float* bias, int act,
+                         const void* residual, int res_dtype, int64_t ldr, void* y, int y_dtype, int64_t ldy, void* actgrad, int M, int N, int K,
+                         void* stream);
+
 /* Kernel-selection overrides for tests / A-B measurements (defaults come from FFVC_GEMM2_BM / FFVC_CONV_ROW):
  *   "gemm2_tile": 0 = register-staged kernel only, 1 = heuristic, 128 | 256 | 512 = force the LDS-DMA tile
  *                 (128x128 | 256x128 | 256x256);   "conv_row": 0 off, 1 heuristic, 2 force the haloed row-tile conv;
