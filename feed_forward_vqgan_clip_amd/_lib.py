@@ -239,7 +239,7 @@ _SIGNATURES = {
     "ffvc_tokmix_fwd_save": (c_int, [c_void_p] * 9 + [c_int, c_int, c_int, c_int, c_int, c_void_p]),
     "ffvc_embed_fwd": (c_int, [c_void_p, c_int, c_int64, c_int64, c_void_p, c_float, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int, c_int64,
                                c_int64, c_int, c_void_p]),
-    "ffvc_embed_bwd_ws_bytes": (c_int64, [c_int64, c_int]),
+    "ffvc_embed_bwd_ws_bytes": (c_int64, [c_int64, c_int64, c_int]),
     "ffvc_embed_bwd": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int64, c_int64, c_int, c_float, c_void_p, c_int, c_void_p, c_int64, c_void_p]),
     "ffvc_attn_packed_fwd": (c_int, [POINTER(AttnPackedDesc), c_void_p]),
     "ffvc_attn_packed_bwd": (c_int, [POINTER(AttnPackedDesc), c_void_p]),

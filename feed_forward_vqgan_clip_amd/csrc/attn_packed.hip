@@ -408,7 +408,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_dq_kernel(const ffvc_a
 // ---- backward: dk, dv --------------------------------------------------------------------------------------------------------------
 // NW waves x 32 keys of one key / value head; walks the query tiles that see them, for every query head of the group.
 template <typename L, int DP, int NW>
-__global__ __launch_bounds__(64 * NW, 1) void attn_packed_dkv_kernel(const ffvc_attn_packed_desc p, int64_t slots) {
+__global__ __launch_bounds__(64 * NW, 2) void attn_packed_dkv_kernel(const ffvc_attn_packed_desc p, int64_t slots) {
   constexpr int BM = 32 * NW, NS = DP / 16, ND = DP / 32, TB = KB * DP * 2;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;

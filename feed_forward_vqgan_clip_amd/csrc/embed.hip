@@ -6,8 +6,8 @@
 // Gradient.  fp32 atomics would need a zero pass over the table and would sum in an order that changes from run to run (and one opening
 // token per prompt makes thousands of adds collide on one row).  Here the token positions are sorted by id first — stable, so the sum of a
 // row runs over its tokens in their order — and then every table row is produced by one owner: no zero pass, no atomics, the same bits
-// every time.  Runs of equal ids are cut into chunks of CHUNK sorted positions whose sums a first kernel leaves in a workspace, so a row
-// with thousands of tokens costs its owner a few dozen reads.
+// every time.  The work is cut by sorted positions, not by rows (ids come ordered by frequency, so a few neighbouring rows hold most tokens): a
+// wave sums CHUNK of them and writes the rows whose tokens it has all seen, a second kernel joins the parts of longer runs and writes the zeros.
 // Sorting: up to RANK_MAX tokens one launch ranks every key against all others out of LDS (n^2 compares spread over the chip); above, a
 // least-significant-digit radix sort, 8 bits per pass, three launches each.
 #include "common.h"
@@ -15,8 +15,8 @@
 namespace {
 
 constexpr int RANK_MAX = 8192;      // tokens
-constexpr int CHUNK = 32;
-constexpr int RT = 4096;            // keys per workgroup of a radix pass
+constexpr int CHUNK = 64;
+constexpr int RT = 1024;            // keys per workgroup of a radix pass
 
 template <typename T, int VEC>
 struct Vec {
@@ -72,17 +72,23 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const TT* __restrict__ t
   }
 }
 
+// first[v] = -1 (no token) for every row, by the first kernel of the chain
+__device__ __forceinline__ void clear_first(int* __restrict__ first, int64_t vocab) {
+  for (int64_t v = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; v < vocab; v += (int64_t)gridDim.x * blockDim.x) first[v] = -1;
+}
+
 // ids outside the table sort behind every row
 __device__ __forceinline__ uint32_t key_of(int64_t id, int64_t vocab) { return id >= 0 && id < vocab ? (uint32_t)id : (uint32_t)vocab; }
 
 // ---- sort, small: position of token t = #{keys below its own} + #{equal keys before it}.  A workgroup ranks 32 tokens; its 32 half-waves
 // split the keys (all of a half-wave's lanes read the same key: an LDS broadcast).
 __global__ __launch_bounds__(1024) void embed_rank_kernel(const int64_t* __restrict__ ids, int64_t vocab, int n, uint32_t* __restrict__ keys,
-                                                          uint32_t* __restrict__ vals) {
-  __shared__ __attribute__((aligned(16))) uint32_t k[RANK_MAX];
-  __shared__ int cnt[32];
+                                                          uint32_t* __restrict__ vals, int* __restrict__ first) {
+  clear_first(first, vocab);
+  extern __shared__ __attribute__((aligned(16))) uint32_t k[];
   const int tid = threadIdx.x;
   const int np = (n + 127) / 128 * 128;                       // whole groups of 4 keys per part
+  int* cnt = (int*)(k + np);                                  // [32]
   for (int i = tid; i < np; i += 1024) k[i] = i < n ? key_of(ids[i], vocab) : 0xFFFFFFFFu;
   if (tid < 32) cnt[tid] = 0;
   __syncthreads();
@@ -112,7 +118,8 @@ __global__ __launch_bounds__(1024) void embed_rank_kernel(const int64_t* __restr
 // ---- sort, large ----------------------------------------------------------------------------------------------------------------------
 // hist[digit][tile] of the 8 bits at `shift`
 __global__ __launch_bounds__(256) void embed_hist_kernel(const int64_t* __restrict__ ids, const uint32_t* __restrict__ keys, int64_t vocab, int64_t n,
-                                                         int shift, uint32_t* __restrict__ hist, int tiles) {
+                                                         int shift, uint32_t* __restrict__ hist, int tiles, int* __restrict__ first) {
+  if (first) clear_first(first, vocab);
   __shared__ uint32_t h[256];
   const int tid = threadIdx.x;
   h[tid] = 0;
@@ -151,7 +158,7 @@ __global__ __launch_bounds__(256) void embed_scan_kernel(uint32_t* __restrict__ 
   if (tid == 0) total[blockIdx.x] = run;
 }
 
-// Stable scatter: wave w of a tile owns its keys 1024 w .. + 1023 and walks them 64 at a time; lanes of one digit find each other by ballots.
+// Stable scatter: wave w of a tile owns a quarter of its keys and walks them 64 at a time; lanes of one digit find each other by ballots.
 __global__ __launch_bounds__(256) void embed_scatter_kernel(const int64_t* __restrict__ ids, const uint32_t* __restrict__ keys,
                                                             const uint32_t* __restrict__ vals, int64_t vocab, int64_t n, int shift,
                                                             const uint32_t* __restrict__ hist, const uint32_t* __restrict__ total, int tiles,
@@ -159,7 +166,7 @@ __global__ __launch_bounds__(256) void embed_scatter_kernel(const int64_t* __res
   __shared__ uint32_t at[4][256];                            // next position of each digit, per wave
   __shared__ uint32_t part[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  constexpr int PW = RT / 4;
+  constexpr int PW = RT / 4;                                  // keys of a wave
 #pragma unroll
   for (int w = 0; w < 4; ++w) at[w][tid] = 0;
   uint32_t base;                                              // keys of smaller digits, and of this digit in earlier tiles
@@ -218,148 +225,154 @@ __global__ __launch_bounds__(256) void embed_scatter_kernel(const int64_t* __res
 }
 
 // ---- sums ------------------------------------------------------------------------------------------------------------------------------
-// part[c] = sum of dout over sorted positions CHUNK c .. + CHUNK - 1, where they all hold one id (others are not needed).  One wave each.
-template <typename DT, int VEC>
-__global__ __launch_bounds__(256) void embed_part_kernel(const uint32_t* __restrict__ keys, const uint32_t* __restrict__ vals, int64_t n,
-                                                         uint32_t vocab, const DT* __restrict__ dout, int64_t ld, int dim, float* __restrict__ part) {
-  const int lane = threadIdx.x & 63;
-  const int64_t c = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int64_t p0 = c * CHUNK;
-  if (p0 + CHUNK > n) return;
-  const uint32_t key = keys[p0];
-  if (key >= vocab || keys[p0 + CHUNK - 1] != key) return;
-  for (int d = lane * VEC; d < dim; d += 64 * VEC) {
-    float acc[VEC];
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) acc[j] = 0.0f;
-#pragma unroll 8
-    for (int i = 0; i < CHUNK; ++i) {
-      const Vec<DT, VEC> a = load_vec<DT, VEC>(dout + (int64_t)vals[p0 + i] * ld + d);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) acc[j] += a.v[j];
-    }
-    store_vec<float, VEC>(part + c * dim + d, acc);
-  }
-}
-
-// first sorted position whose key is >= v, 64 probes at a time (one wave)
-__device__ __forceinline__ int64_t lower_bound64(const uint32_t* __restrict__ keys, int64_t n, uint32_t v, int lane) {
-  int64_t lo = 0, hi = n;                                     // the answer is in lo .. hi
-  while (hi > lo) {
-    const int64_t step = (hi - lo + 63) / 64;
-    const int64_t p = lo + lane * step;
-    const uint64_t below = __ballot(p < hi && keys[p] < v);
-    const int k = __popcll(below);                            // probes 0 .. k - 1 are below v
-    if (k == 0) return lo;
-    hi = min(hi, lo + k * step);
-    lo += (k - 1) * step + 1;
-  }
-  return lo;
-}
-
-// R table rows per workgroup.  A row's tokens: single ones up to a chunk border, whole chunks, single ones behind; the four waves take
-// them in four consecutive shares whose sums meet in LDS in order (short rows: one wave takes the row alone).
+// One wave per chunk of CHUNK sorted positions and block of 64 * VEC columns.  Runs of one id that begin and end inside the chunk go straight
+// to their table row; one that came in from the chunk before leaves its sum in part[2 c], one that goes on into the next in part[2 c + 1].
+// first / end: the sorted positions of each row's tokens (the rows kernel's map).
 template <typename DT, typename TT, int VEC>
-__global__ __launch_bounds__(256) void embed_reduce_kernel(const uint32_t* __restrict__ keys, const uint32_t* __restrict__ vals, int64_t n, int64_t vocab,
-                                                           const DT* __restrict__ dout, int64_t ld, int dim, float scale,
-                                                           const float* __restrict__ part, TT* __restrict__ dtable, int R) {
-  constexpr int SHORT = 16;
-  __shared__ int64_t edge[17];                                // R <= 16
-  __shared__ float sums[4][64 * VEC];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t v0 = (int64_t)blockIdx.x * R;
-  const int nr = (int)(vocab - v0 < R ? vocab - v0 : R);
-  for (int r = wave; r <= nr; r += 4) {
-    const int64_t e = lower_bound64(keys, n, (uint32_t)(v0 + r), lane);
-    if (lane == 0) edge[r] = e;
+__global__ __launch_bounds__(256) void embed_runs_kernel(const uint32_t* __restrict__ keys, const uint32_t* __restrict__ vals, int n, uint32_t vocab,
+                                                         const DT* __restrict__ dout, int64_t ld, int dim, float scale, float* __restrict__ part,
+                                                         int* __restrict__ first, int* __restrict__ end, TT* __restrict__ dtable) {
+  const int lane = threadIdx.x & 63;
+  const int64_t c = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t p0 = c * CHUNK;
+  if (p0 >= n) return;
+  const int m = __builtin_amdgcn_readfirstlane((int)(n - p0 < CHUNK ? n - p0 : CHUNK));
+  const uint32_t key = lane < m ? keys[p0 + lane] : 0xFFFFFFFFu;
+  const uint32_t val = lane < m ? vals[p0 + lane] : 0u;
+  const uint32_t left = p0 + lane > 0 && lane <= m ? keys[p0 + lane - 1] : 0xFFFFFFFFu;      // (lane m: the chunk's last key)
+  const uint32_t next = p0 + m < n ? keys[p0 + m] : 0xFFFFFFFFu;                              // first key of the next chunk
+  const uint64_t starts = __ballot(lane < m && key != left);
+  if (blockIdx.y == 0 && lane < m && key < vocab) {
+    if (key != left) first[key] = (int)(p0 + lane);
+    const uint32_t right = lane + 1 < m ? keys[p0 + lane + 1] : next;
+    if (key != right) end[key] = (int)(p0 + lane + 1);
   }
-  __syncthreads();
-  // items of a row: head tokens a .. h, chunks h / CHUNK .. t / CHUNK, tail tokens t .. b
-  auto add_items = [&](float (&acc)[VEC], int64_t a, int64_t h, int64_t t, int64_t i0, int64_t i1, int d) {
-    const int64_t nh = h - a, nc = (t - h) / CHUNK;
-    int64_t i = i0;
-#pragma unroll 4
-    for (; i < i1 && i < nh; ++i) {
-      const Vec<DT, VEC> x = load_vec<DT, VEC>(dout + (int64_t)vals[a + i] * ld + d);
+  const bool in = !(starts & 1ull);                            // the chunk's first run came in from the chunk before
+  const bool out = m == CHUNK && __builtin_amdgcn_readlane(key, CHUNK - 1) == __builtin_amdgcn_readfirstlane(next);
+  const int d = (blockIdx.y * 64 + lane) * VEC;
+  const bool live = d < dim;
+  float acc[VEC];
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) acc[j] += x.v[j];
-    }
-#pragma unroll 4
-    for (; i < i1 && i < nh + nc; ++i) {
-      const Vec<float, VEC> x = load_vec<float, VEC>(part + (h / CHUNK + i - nh) * dim + d);
+  for (int e = 0; e < VEC; ++e) acc[e] = 0.0f;
+  auto flush = [&](int j) {                                    // the run that ends before token j
+    const uint32_t k = __builtin_amdgcn_readlane(key, j - 1);
+    const bool came = in && (starts & ((2ull << (j - 1)) - 1ull)) == 0;
+    if (k < vocab && live) {
+      if (came) {
+        store_vec<float, VEC>(part + 2 * c * dim + d, acc);
+      } else if (j == m && out) {
+        store_vec<float, VEC>(part + (2 * c + 1) * dim + d, acc);
+      } else {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) acc[j] += x.v[j];
-    }
-#pragma unroll 4
-    for (; i < i1; ++i) {
-      const Vec<DT, VEC> x = load_vec<DT, VEC>(dout + (int64_t)vals[t + i - nh - nc] * ld + d);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) acc[j] += x.v[j];
-    }
-  };
-  for (int r = 0; r < nr; ++r) {
-    const int64_t a = edge[r], b = edge[r + 1];
-    const int64_t up = (a + CHUNK - 1) / CHUNK * CHUNK, dn = b / CHUNK * CHUNK;
-    const int64_t h = up < dn ? up : b, t = up < dn ? dn : b;    // no whole chunk: every token is a head token
-    const int64_t items = (h - a) + (t - h) / CHUNK + (b - t);
-    TT* row = dtable + (v0 + r) * dim;
-    if (items <= SHORT) {
-      if ((r & 3) == wave)
-        for (int d = lane * VEC; d < dim; d += 64 * VEC) {
-          float acc[VEC];
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) acc[j] = 0.0f;
-          add_items(acc, a, h, t, 0, items, d);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) acc[j] *= scale;
-          store_vec<TT, VEC>(row + d, acc);
-        }
-    } else {
-      for (int d0 = 0; d0 < dim; d0 += 64 * VEC) {
-        const int d = d0 + lane * VEC;
-        float acc[VEC];
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) acc[j] = 0.0f;
-        if (d < dim) add_items(acc, a, h, t, items * wave / 4, items * (wave + 1) / 4, d);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) sums[wave][lane * VEC + j] = acc[j];
-        __syncthreads();
-        if (wave == 0 && d < dim) {
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const int x = lane * VEC + j;
-            acc[j] = (((sums[0][x] + sums[1][x]) + sums[2][x]) + sums[3][x]) * scale;
-          }
-          store_vec<TT, VEC>(row + d, acc);
-        }
-        __syncthreads();
+        for (int e = 0; e < VEC; ++e) acc[e] *= scale;
+        store_vec<TT, VEC>(dtable + (int64_t)k * dim + d, acc);
       }
     }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) acc[e] = 0.0f;
+  };
+  constexpr int U = 8;                                         // rows under way
+  for (int j0 = 0; j0 < m; j0 += U) {
+    Vec<DT, VEC> x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (j0 + u < m && live) x[u] = load_vec<DT, VEC>(dout + (int64_t)__builtin_amdgcn_readlane(val, j0 + u) * ld + d);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (j0 + u < m) {
+        if (j0 + u > 0 && ((starts >> (j0 + u)) & 1)) flush(j0 + u);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[e] += x[u].v[e];
+      }
+  }
+  flush(m);
+}
+
+// The rows the runs kernel has not written: zeros where no token asked for the row, the sum of the parts where its run crosses chunks.  R rows per
+// workgroup; up to SHORT parts one wave sums them, more are taken by the four waves in consecutive shares that meet in LDS in order.
+constexpr int ROWS = 4, SHORT = 8;
+template <typename TT, int VEC>
+__global__ __launch_bounds__(256) void embed_rows_kernel(const int* __restrict__ first, const int* __restrict__ end, int64_t vocab, int dim, float scale,
+                                                         const float* __restrict__ part, TT* __restrict__ dtable) {
+  __shared__ float sums[4][64 * VEC];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t v0 = (int64_t)blockIdx.x * ROWS;
+  const int nr = (int)(vocab - v0 < ROWS ? vocab - v0 : ROWS);
+  const int d = (blockIdx.y * 64 + lane) * VEC;
+  const bool live = d < dim;
+  // parts of a row: part[2 ca + 1], then part[2 c] of the chunks ca + 1 .. cb
+  auto add = [&](float (&acc)[VEC], int ca, int i0, int i1) {
+#pragma unroll 8
+    for (int i = i0; i < i1; ++i)
+      if (live) {
+        const Vec<float, VEC> x = load_vec<float, VEC>(part + (i ? 2 * (int64_t)(ca + i) : 2 * (int64_t)ca + 1) * dim + d);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[e] += x.v[e];
+      }
+  };
+  int a[ROWS], np[ROWS];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    a[r] = r < nr ? __builtin_amdgcn_readfirstlane(first[v0 + r]) : 0;
+    const int b = r < nr && a[r] >= 0 ? __builtin_amdgcn_readfirstlane(end[v0 + r]) : 0;
+    np[r] = r < nr && a[r] >= 0 ? (b - 1) / CHUNK - a[r] / CHUNK + 1 : 0;         // 0: no token; 1: written already
+  }
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    float acc[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) acc[e] = 0.0f;
+    TT* row = dtable + (v0 + r) * dim + d;
+    if (np[r] <= SHORT) {
+      if (r < nr && r % 4 == wave && np[r] != 1) {
+        add(acc, a[r] / CHUNK, 0, np[r]);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[e] *= scale;
+        if (live) store_vec<TT, VEC>(row, acc);
+      }
+    } else {
+      add(acc, a[r] / CHUNK, (int)((int64_t)np[r] * wave / 4), (int)((int64_t)np[r] * (wave + 1) / 4));
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) sums[wave][lane * VEC + e] = acc[e];
+      __syncthreads();
+      if (wave == 0 && live) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const int y = lane * VEC + e;
+          acc[e] = (((sums[0][y] + sums[1][y]) + sums[2][y]) + sums[3][y]) * scale;
+        }
+        store_vec<TT, VEC>(row, acc);
+      }
+      __syncthreads();
+    }
   }
 }
 
-struct Layout {      // the workspace: two (keys, vals) pairs, the radix counters, the chunk sums
-  int64_t pair, tiles, hist, part, bytes;
-  Layout(int64_t n, int dim) {
-    pair = (n * 4 + 15) / 16 * 16;
+struct Layout {      // the workspace: two (keys, vals) pairs, first / end of every row, the radix counters, the parts
+  int64_t pair, tiles, rows, hist, part, bytes;
+  bool rank;
+  Layout(int64_t n, int64_t vocab, int dim) {
+    auto up = [](int64_t b) { return (b + 15) / 16 * 16; };
+    // One ranking launch against one or more radix passes of three: the ranking grows with n^2 (measured 17 us at 8192 tokens, 46 at 13600),
+    // a pass takes about 12 us up to 100000 tokens.
+    rank = n <= (vocab < 256 ? RANK_MAX / 2 : RANK_MAX);
+    pair = up(n * 4);
+    rows = 4 * pair;
+    hist = rows + 2 * up(vocab * 4);
     tiles = (n + RT - 1) / RT;
-    hist = 4 * pair;
-    part = hist + (n > RANK_MAX ? (256 * tiles + 256) * 4 : 0);
-    bytes = part + n / CHUNK * dim * 4;
+    part = hist + (rank ? 0 : up((256 * tiles + 256) * 4));
+    bytes = part + 2 * ((n + CHUNK - 1) / CHUNK) * dim * 4;
   }
 };
 
 template <typename DT, typename TT, int VEC>
 int run_sums(const uint32_t* keys, const uint32_t* vals, int64_t n, int64_t vocab, const void* dout, int64_t ld, int dim, float scale, float* part,
-             void* dtable, hipStream_t st) {
-  const int64_t chunks = n / CHUNK;
-  if (chunks)
-    hipLaunchKernelGGL((embed_part_kernel<DT, VEC>), dim3((unsigned)((chunks + 3) / 4)), dim3(256), 0, st, keys, vals, n, (uint32_t)vocab, (const DT*)dout,
-                       ld, dim, part);
-  // rows per workgroup: enough workgroups to fill the chip first, then fewer searches per row
-  const int R = (int)(vocab / 1024 < 1 ? 1 : (vocab / 1024 > 16 ? 16 : vocab / 1024));
-  hipLaunchKernelGGL((embed_reduce_kernel<DT, TT, VEC>), dim3((unsigned)((vocab + R - 1) / R)), dim3(256), 0, st, keys, vals, n, vocab, (const DT*)dout, ld,
-                     dim, scale, part, (TT*)dtable, R);
+             int* first, int* end, void* dtable, hipStream_t st) {
+  const int ncb = (dim + 64 * VEC - 1) / (64 * VEC);
+  hipLaunchKernelGGL((embed_runs_kernel<DT, TT, VEC>), dim3((unsigned)((n + 4 * CHUNK - 1) / (4 * CHUNK)), ncb), dim3(256), 0, st, keys, vals, (int)n,
+                     (uint32_t)vocab, (const DT*)dout, ld, dim, scale, part, first, end, (TT*)dtable);
+  hipLaunchKernelGGL((embed_rows_kernel<TT, VEC>), dim3((unsigned)((vocab + ROWS - 1) / ROWS), ncb), dim3(256), 0, st, first, end, vocab, dim, scale, part,
+                     (TT*)dtable);
   FFVC_LAUNCH_CHECK();
   return 0;
 }
@@ -388,7 +401,9 @@ extern "C" int ffvc_embed_fwd(const void* table, int table_dtype, int64_t ld, in
   return 0;
 }
 
-extern "C" int64_t ffvc_embed_bwd_ws_bytes(int64_t n, int dim) { return n > 0 && dim > 0 ? Layout(n, dim).bytes : 0; }
+extern "C" int64_t ffvc_embed_bwd_ws_bytes(int64_t n, int64_t vocab, int dim) {
+  return n > 0 && vocab > 0 && dim > 0 ? Layout(n, vocab, dim).bytes : 0;
+}
 
 extern "C" int ffvc_embed_bwd(const void* dout, int dout_dtype, int64_t ld, const int64_t* ids, int64_t n, int64_t vocab, int dim, float scale,
                               void* dtable, int table_dtype, void* ws, int64_t ws_bytes, void* stream) {
@@ -396,16 +411,22 @@ extern "C" int ffvc_embed_bwd(const void* dout, int dout_dtype, int64_t ld, cons
   FFVC_CHECK_ARG(ffvc_dtype_ok(dout_dtype) && ffvc_dtype_ok(table_dtype), "ffvc_embed_bwd: bad dtype");
   FFVC_CHECK_ARG(ld >= dim, "ffvc_embed_bwd: rows shorter than dim");
   FFVC_CHECK_ARG(n < (1ll << 31) && vocab < (1ll << 31), "ffvc_embed_bwd: token count and vocabulary must stay below 2^31");
-  const Layout lay(n, dim);
+  const Layout lay(n, vocab, dim);
   FFVC_CHECK_ARG((uintptr_t)ws % 16 == 0 && ws_bytes >= lay.bytes, "ffvc_embed_bwd: workspace of %lld bytes needed, got %lld", (long long)lay.bytes,
                  (long long)ws_bytes);
   hipStream_t st = (hipStream_t)stream;
   char* w = (char*)ws;
   uint32_t* keys[2] = {(uint32_t*)w, (uint32_t*)(w + 2 * lay.pair)};
   uint32_t* vals[2] = {(uint32_t*)(w + lay.pair), (uint32_t*)(w + 3 * lay.pair)};
+  int* row_first = (int*)(w + lay.rows);
+  int* row_end = (int*)(w + lay.rows + (lay.hist - lay.rows) / 2);
   int cur = 0;
-  if (n <= RANK_MAX) {
-    hipLaunchKernelGGL(embed_rank_kernel, dim3((unsigned)((n + 31) / 32)), dim3(1024), 0, st, ids, vocab, (int)n, keys[0], vals[0]);
+  if (lay.rank) {
+    const int lds = (int)((n + 127) / 128 * 128 * 4 + 32 * 4);
+    static ffvc_lds_once once;
+    const int rc = once.set((const void*)embed_rank_kernel, RANK_MAX * 4 + 32 * 4);
+    if (rc) return rc;
+    hipLaunchKernelGGL(embed_rank_kernel, dim3((unsigned)((n + 31) / 32)), dim3(1024), lds, st, ids, vocab, (int)n, keys[0], vals[0], row_first);
   } else {
     uint32_t* hist = (uint32_t*)(w + lay.hist);
     uint32_t* total = hist + 256 * lay.tiles;
@@ -414,7 +435,7 @@ extern "C" int ffvc_embed_bwd(const void* dout, int dout_dtype, int64_t ld, cons
     for (int shift = 0; shift == 0 || (shift < 32 && (vocab >> shift) != 0); shift += 8) {
       const int64_t* src = first ? ids : nullptr;
       const int nx = first ? 0 : cur ^ 1;
-      hipLaunchKernelGGL(embed_hist_kernel, dim3(tiles), dim3(256), 0, st, src, keys[cur], vocab, n, shift, hist, tiles);
+      hipLaunchKernelGGL(embed_hist_kernel, dim3(tiles), dim3(256), 0, st, src, keys[cur], vocab, n, shift, hist, tiles, first ? row_first : nullptr);
       hipLaunchKernelGGL(embed_scan_kernel, dim3(256), dim3(256), 0, st, hist, total, tiles);
       hipLaunchKernelGGL(embed_scatter_kernel, dim3(tiles), dim3(256), 0, st, src, keys[cur], first ? nullptr : vals[cur], vocab, n, shift, hist, total,
                          tiles, keys[nx], vals[nx]);
@@ -426,8 +447,8 @@ extern "C" int ffvc_embed_bwd(const void* dout, int dout_dtype, int64_t ld, cons
   const bool vec = dim % 8 == 0 && al(dout, dout_dtype, ld) && al(dtable, table_dtype, dim);
   float* part = (float*)(w + lay.part);
   DISPATCH_DT(dout_dtype, DT, DISPATCH_DT(table_dtype, TT, {
-    return vec ? run_sums<DT, TT, 8>(keys[cur], vals[cur], n, vocab, dout, ld, dim, scale, part, dtable, st)
-               : run_sums<DT, TT, 1>(keys[cur], vals[cur], n, vocab, dout, ld, dim, scale, part, dtable, st);
+    return vec ? run_sums<DT, TT, 8>(keys[cur], vals[cur], n, vocab, dout, ld, dim, scale, part, row_first, row_end, dtable, st)
+               : run_sums<DT, TT, 1>(keys[cur], vals[cur], n, vocab, dout, ld, dim, scale, part, row_first, row_end, dtable, st);
   }));
   return 0;
 }

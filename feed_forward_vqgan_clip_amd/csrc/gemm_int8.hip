@@ -7,7 +7,11 @@
 // and the result does not depend on how K is cut.  Rounding to 8 bits follows the definition exactly: the quotient is formed with a
 // reciprocal, then corrected with one fused residual (x - q xs is exact in fp32 once q is within one step of x / xs).
 // A row of zeros has scale 0 and stays 0; a row that holds an inf or a NaN gets scale NaN, so its outputs are NaN and nothing is hidden.
+#include <type_traits>
+
 #include "common.h"
+
+#pragma clang fp contract(off)      // a product and a sum fuse only where fmaf says so: the kernels below agree bit for bit on a row's outputs
 
 namespace {
 
@@ -29,19 +33,8 @@ __device__ __forceinline__ float amax_with_nan(float m, float v) {  // fmaxf dro
   const float a = fabsf(v);
   return a > m || a != a ? a : m;
 }
-// round-half-even(x / s); inv = 1 / s.  (Only where s itself is subnormal, and so a coarse amax / 127, can the quotient pass 127.)
-__device__ __forceinline__ int quant1(float x, float s, float inv) {
-  float q = rintf(x * inv);
-  const float r = fmaf(-q, s, x);                                   // exact: what is left after q steps
-  const float half = 0.5f * s;
-  const bool odd = ((int)q & 1) != 0;
-  if (fabsf(r) > half || (odd && fabsf(r) == half)) q += r > 0.0f ? 1.0f : -1.0f;
-  return (int)fminf(fmaxf(q, -127.0f), 127.0f);
-}
-__device__ __forceinline__ uint32_t pack_i8(int a, int b, int c, int d) {
-  return (uint32_t)(a & 255) | ((uint32_t)(b & 255) << 8) | ((uint32_t)(c & 255) << 16) | ((uint32_t)d << 24);
-}
-// One row's scale, ready to divide by: rows whose 1 / s would overflow are lifted by a power of two first (exact)
+// One row's scale, ready to divide by: rows whose 1 / s would overflow are lifted by a power of two first (exact).  Such a scale may itself be
+// subnormal, and so a coarse amax / 127: only there can a quotient pass 127.
 struct RowQuant {
   float s, inv, up;
   __device__ __forceinline__ RowQuant(float scale) {
@@ -50,13 +43,42 @@ struct RowQuant {
     inv = s > 0.0f ? 1.0f / s : 0.0f;                               // 0: a row of zeros or one with a NaN / inf, stored as zeros
   }
 };
+__device__ __forceinline__ uint32_t pack_i8(int a, int b, int c, int d) {
+  const uint32_t lo = __builtin_amdgcn_perm((uint32_t)b, (uint32_t)a, 0x0c0c0400u), hi = __builtin_amdgcn_perm((uint32_t)d, (uint32_t)c, 0x04000c0cu);
+  return lo | hi;
+}
+// round-half-even(x / s) of eight values.  x * inv is within 127 * 2^-23 of the quotient (two roundings of at most half a unit each), so its
+// rounding is right unless it lies within 2^-15 of a border; then (3 % of the waves) the remainder x - q s, which one fma gives exactly,
+// decides, a remainder of exactly half a step going to the even neighbour.
 __device__ __forceinline__ u32x2_t quant8(const f32x8& v, const RowQuant& r) {
-  int q[8];
+  float x[8], q[8];
+  float far = 0.0f;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) q[j] = r.inv > 0.0f ? quant1(v.v[j] * r.up, r.s, r.inv) : 0;
+  for (int j = 0; j < 8; ++j) {
+    x[j] = r.inv > 0.0f ? v.v[j] * r.up : 0.0f;
+    const float f = x[j] * r.inv;
+    q[j] = rintf(f);
+    far = fmaxf(far, fabsf(f - q[j]));
+  }
+  if (__any(far > 0.5f - 0x1p-15f)) {
+    const float half = 0.5f * r.s;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float d = fmaf(-q[j], r.s, x[j]);
+      const bool odd = ((int)q[j] & 1) != 0;
+      if (fabsf(d) > half || (odd && fabsf(d) == half)) q[j] += d > 0.0f ? 1.0f : -1.0f;
+    }
+  }
+  int i[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) i[j] = (int)q[j];
+  if (r.up != 1.0f) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) i[j] = min(max(i[j], -127), 127);
+  }
   u32x2_t o;
-  o[0] = pack_i8(q[0], q[1], q[2], q[3]);
-  o[1] = pack_i8(q[4], q[5], q[6], q[7]);
+  o[0] = pack_i8(i[0], i[1], i[2], i[3]);
+  o[1] = pack_i8(i[4], i[5], i[6], i[7]);
   return o;
 }
 
@@ -104,27 +126,40 @@ __global__ __launch_bounds__(256) void int8_quant_kernel(const T* __restrict__ x
 }
 
 // ---- epilogue ----------------------------------------------------------------------------------------------------------------------
-// The activation and its derivative; 16-bit outputs take the hardware exp / rcp forms (errors ~2^-22), fp32 outputs the accurate ones.
-template <bool FAST>
-__device__ __forceinline__ void act_and_grad(int act, float z, float& y, float& g) {
-  if (act == FFVC_ACT_GELU) {
+// The activation (and its derivative); 16-bit outputs take the hardware exp / rcp forms (errors ~2^-22; erf after Abramowitz & Stegun 7.1.26,
+// 1.5e-7), fp32 outputs the accurate ones.
+template <bool FAST, int ACT, bool GRAD>
+__device__ __forceinline__ void activate(float z, float& y, float& g) {
+  if constexpr (ACT == FFVC_ACT_GELU) {
     if constexpr (FAST) {
-      float cdf, e;
-      gelu_parts_fast(z, cdf, e);
+      const float u = fabsf(z) * 0.70710678118654752440f;
+      const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, u, 1.0f));
+      const float e = __builtin_amdgcn_exp2f(-1.44269504088896341f * (u * u));
+      const float q = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+      const float cdf = fmaf(copysignf(0.5f, z), fmaf(-q, e, 1.0f), 0.5f);
       y = z * cdf;
-      g = cdf + z * 0.39894228040143267794f * e;
+      if constexpr (GRAD) g = fmaf(z * 0.39894228040143267794f, e, cdf);
     } else {
       y = act_gelu(z);
-      g = act_gelu_grad(z);
+      if constexpr (GRAD) g = act_gelu_grad(z);
     }
-  } else if (act == FFVC_ACT_QUICKGELU) {
-    const float s = FAST ? sigmoid_fast_(1.702f * z) : 1.0f / (1.0f + expf(-1.702f * z));
+  } else if constexpr (ACT == FFVC_ACT_QUICKGELU) {
+    const float s = FAST ? __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-2.45546696f * z)) : 1.0f / (1.0f + expf(-1.702f * z));
     y = z * s;
-    g = s * (1.0f + 1.702f * z * (1.0f - s));
+    if constexpr (GRAD) g = s * (1.0f + 1.702f * z * (1.0f - s));
   } else {
     y = z;
     g = 1.0f;
   }
+}
+template <bool FAST, bool GRAD>
+__device__ __forceinline__ void activate_by(int act, float z, float& y, float& g) {
+  if (act == FFVC_ACT_GELU)
+    activate<FAST, FFVC_ACT_GELU, GRAD>(z, y, g);
+  else if (act == FFVC_ACT_QUICKGELU)
+    activate<FAST, FFVC_ACT_QUICKGELU, GRAD>(z, y, g);
+  else
+    activate<FAST, FFVC_ACT_NONE, GRAD>(z, y, g);
 }
 
 struct I8Args {
@@ -139,104 +174,79 @@ struct I8Args {
   int64_t ldx, ldw, ldy, ldr;
   int M, N, K;
   int act;
+  int res_f32;
   int vec;                // rows of y / res / aux take 16-byte accesses and N % 8 == 0
 };
 
-// eight neighbouring outputs of row m.  YT: float or the 16-bit storage type; RT: the residual's type
-template <typename L, typename YT, typename RT>
-__device__ __forceinline__ void store_oct(const I8Args& p, const float (&acc)[8], int m, int n) {
-  constexpr bool FAST = sizeof(YT) == 2;
-  const float xs = p.xs[m];
-  float v[8], g[8];
-  YT* yr = (YT*)p.y + m * p.ldy + n;
-  const RT* rr = (const RT*)p.res + m * p.ldr + n;
-  L* ar = (L*)p.aux + (int64_t)m * p.N + n;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int nn = n + j < p.N ? n + j : p.N - 1;
-    const float z = fmaf(acc[j], xs * p.ws[nn], p.bias ? p.bias[nn] : 0.0f);
-    act_and_grad<FAST>(p.act, z, v[j], g[j]);
-  }
-  if (p.vec) {
-    f32x8 o;
-    if (p.res) {
-      const f32x8 r = load8(rr);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] += r.v[j];
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) o.v[j] = v[j];
-    store8(yr, o);
-    if (p.aux) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) o.v[j] = g[j];
-      store8(ar, o);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (n + j < p.N) {
-        ElemTraits<YT>::store(yr + j, v[j] + (p.res ? ElemTraits<RT>::load(rr + j) : 0.0f));
-        if (p.aux) ElemTraits<L>::store(ar + j, g[j]);
-      }
-  }
+// one output from its row-scaled sum (v = sum * xs[m]); every kernel of this file takes the same steps, so they agree bit for bit
+template <typename L, typename YT>
+__device__ __forceinline__ void store_one(const I8Args& p, float v, int64_t m, int n) {
+  const float z = fmaf(v, p.ws[n], p.bias ? p.bias[n] : 0.0f);
+  float y, g;
+  activate_by<sizeof(YT) == 2, true>(p.act, z, y, g);
+  if (p.res) y += p.res_f32 ? ((const float*)p.res)[m * p.ldr + n] : ElemTraits<L>::load((const L*)p.res + m * p.ldr + n);
+  ElemTraits<YT>::store((YT*)p.y + m * p.ldy + n, y);
+  if (p.aux) ElemTraits<L>::store((L*)p.aux + m * p.N + n, g);
 }
 
 // ---- the tiled product -----------------------------------------------------------------------------------------------------------------
-// BM x BN outputs per workgroup, waves of (32 MT) x 64; K steps of 128 bytes, two LDS stages filled by LDS-DMA.  A staged row is 128 bytes,
-// two rows to a 256-byte line, 16-byte chunks XOR-swizzled by the line: the 16-byte fragment reads of 32 rows hit every bank evenly.
-__device__ __forceinline__ u32x4_t frag_i8(const unsigned char* tile, int row, int sub, int h) {
-  const int line = row >> 1;
-  return *(const u32x4_t*)(tile + line * 256 + (((((row & 1) << 3) | (2 * sub + h)) ^ (line & 15)) << 4));
+// BM x 128 outputs per workgroup of four waves ((BM / 2) x 64 each), K steps of 64 bytes in a ring of three LDS stages filled by LDS-DMA two
+// steps ahead (one barrier per step, the youngest stage may still be in flight).  Two (BM = 256: 72 KiB) or three (BM = 128: 48 KiB) workgroups
+// share a CU, so the epilogue of one, as long as its K loop where K is 1024 and an activation is due, runs under the products of another.
+// A staged row is 64 bytes, four rows to a 256-byte line, its 16-byte chunks XOR-swizzled by the line: the fragment reads hit every bank evenly.
+constexpr int BN = 128, BK = 64;
+
+__device__ __forceinline__ u32x4_t frag_i8(const unsigned char* tile, int row, int chunk) {
+  return *(const u32x4_t*)(tile + row * 64 + ((chunk ^ ((row >> 2) & 3)) << 4));
 }
 
+// the staging of `ROWS` rows by NW waves: a piece is 16 rows; the lane's row and source chunk inside a piece are the same for every piece
 template <int ROWS, int NW>
 struct RowsDma {
-  static constexpr int NP = ROWS / (8 * NW);
+  static constexpr int NP = ROWS / (16 * NW);
   rsrc_t rs;
   uint32_t off[NP];
+  int chunk;
   // rows row0 .. of a matrix with `rows` rows of K bytes; the descriptor ends with the last staged row, rows past it read as zeros
   __device__ __forceinline__ void init(const int8_t* base, int64_t ld, int row0, int rows, int K, int wave, int lane) {
     const int live = rows - row0 < ROWS ? rows - row0 : ROWS;
     rs = __builtin_amdgcn_make_buffer_rsrc((void*)(base + row0 * ld), 0, (int)((live - 1) * ld + K), 0x00020000);
+    chunk = ((lane & 3) ^ ((lane >> 4) & 3)) * 16;
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      const int pos = (wave * NP + i) * 64 + lane, line = pos >> 4;
-      const int cp = (pos & 15) ^ (line & 15);
-      const int row = 2 * line + (cp >> 3);
-      off[i] = row < live ? (uint32_t)(row * ld + (cp & 7) * 16) : OOB;
+      const int row = (wave * NP + i) * 16 + (lane >> 2);
+      off[i] = row < live ? (uint32_t)(row * ld + chunk) : OOB;
     }
   }
+  // K step k0 (wave-uniform): interior steps cost no address arithmetic, the last one drops the chunks past K, steps past the end fetch zeros
   __device__ __forceinline__ void issue(unsigned char* tile, int k0, int K, int wave) {
+    const bool whole = k0 + BK <= K;
+    const bool in = k0 + chunk < K;
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      uint32_t o = off[i];
-      if (k0 + 128 > K) {                    // K tail: chunks past K read as zeros
-        const int pos = (wave * NP + i) * 64 + (threadIdx.x & 63), line = pos >> 4;
-        if (k0 + ((((pos & 15) ^ (line & 15)) & 7) * 16) >= K) o = OOB;
-      }
-      dma16(rs, o, k0, tile + (wave * NP + i) * 1024);
-    }
+    for (int i = 0; i < NP; ++i) dma16(rs, whole || in ? off[i] : OOB, k0 < K ? k0 : 0, tile + (wave * NP + i) * 1024);
   }
 };
 
-template <typename L, typename YT, typename RT, int BM, int BN>
-__global__ __launch_bounds__(2 * BN, (BM == 256 ? 2 : 1)) void gemm_int8_kernel(const I8Args p, int tiles_n, int n_tiles) {
-  constexpr int MT = BM / 64, NW = 2 * (BN / 64);
-  constexpr int XT = BM * 128, WT = BN * 128, STAGE = XT + WT;
+template <typename L, typename YT, int ACT, int BM>
+__global__ __launch_bounds__(256, 2) void gemm_int8_kernel(const I8Args p, int tiles_n) {
+  constexpr int MT = BM / 64, XT = BM * BK, STAGE = (BM + BN) * BK;
+  constexpr int PIECES = (BM + BN) / 64;                  // LDS-DMA instructions per wave and stage
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave & 1, wn = wave >> 1;
-  int tile;
-  {   // consecutive workgroups go to the 8 XCDs in turn: give each XCD a contiguous run of tiles
-    const int bid = blockIdx.x, q = n_tiles >> 3, r = n_tiles & 7, xcd = bid & 7;
-    tile = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (bid >> 3);
+  // Consecutive workgroups go to the 8 XCDs in turn: give each XCD a contiguous run of the whole tiles.  The tiles of a last, partly filled row
+  // block come after all others, spread over the XCDs: their dead 32-row blocks are skipped, so they are short.
+  int tile = blockIdx.x;
+  const int whole = (p.M / BM) * tiles_n;
+  if (tile < whole) {
+    const int q = whole >> 3, r = whole & 7, xcd = tile & 7;
+    tile = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (tile >> 3);
   }
   const int tm = tile / tiles_n, tn = tile - tm * tiles_n;
   const int m0 = tm * BM, n0 = tn * BN;
-  RowsDma<BM, NW> dx;
-  RowsDma<BN, NW> dw;
+  RowsDma<BM, 4> dx;
+  RowsDma<BN, 4> dw;
   dx.init(p.x, p.ldx, m0, p.M, p.K, wave, lane);
   dw.init(p.w, p.ldw, n0, p.N, p.K, wave, lane);
   i32x16_t acc[2][MT];
@@ -246,88 +256,217 @@ __global__ __launch_bounds__(2 * BN, (BM == 256 ? 2 : 1)) void gemm_int8_kernel(
     for (int b = 0; b < MT; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[a][b][i] = 0;
-  const int nk = (p.K + 127) / 128;
-  dx.issue(smem, 0, p.K, wave);
-  dw.issue(smem + XT, 0, p.K, wave);
+  const int nk = (p.K + BK - 1) / BK;
+  const int live = min(MT, (p.M - m0 - wm * (32 * MT) + 31) / 32);   // 32-row blocks of this wave that hold a row (may be < 1)
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    dx.issue(smem + t * STAGE, t * BK, p.K, wave);
+    dw.issue(smem + t * STAGE + XT, t * BK, p.K, wave);
+  }
+  auto steps = [&](auto partial) {
+    constexpr bool PARTIAL = decltype(partial)::value;
+    int cur = 0, nxt = 2;
 #pragma unroll 1
-  for (int kt = 0; kt < nk; ++kt) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    const unsigned char* sx = smem + (kt & 1) * STAGE;
-    const unsigned char* sw = sx + XT;
-    if (kt + 1 < nk) {
-      unsigned char* nx = smem + ((kt + 1) & 1) * STAGE;
-      dx.issue(nx, (kt + 1) * 128, p.K, wave);
-      dw.issue(nx + XT, (kt + 1) * 128, p.K, wave);
-    }
+    for (int kt = 0; kt < nk; ++kt) {
+      // my pieces of this step have landed (those of the next may be under way), then everyone's; and nobody reads the slot filled next
+      // (the bare barrier: __syncthreads would wait for the pieces under way as well)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PIECES) : "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      dx.issue(smem + nxt * STAGE, (kt + 2) * BK, p.K, wave);
+      dw.issue(smem + nxt * STAGE + XT, (kt + 2) * BK, p.K, wave);
+      const unsigned char* sx = smem + cur * STAGE;
+      const unsigned char* sw = sx + XT;
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      u32x4_t fa[2], fb[MT];
+      for (int s = 0; s < 2; ++s) {
+        u32x4_t fa[2], fb[MT];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) fa[t] = frag_i8(sw, wn * 64 + t * 32 + l31, s, h);
+        for (int t = 0; t < 2; ++t) fa[t] = frag_i8(sw, wn * 64 + t * 32 + l31, 2 * s + h);
 #pragma unroll
-      for (int t = 0; t < MT; ++t) fb[t] = frag_i8(sx, wm * (32 * MT) + t * 32 + l31, s, h);
-#pragma unroll
-      for (int a = 0; a < 2; ++a)
+        for (int t = 0; t < MT; ++t) fb[t] = frag_i8(sx, wm * (32 * MT) + t * 32 + l31, 2 * s + h);
 #pragma unroll
         for (int b = 0; b < MT; ++b)
-          acc[a][b] = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4_t, fa[a]), __builtin_bit_cast(i32x4_t, fb[b]), acc[a][b], 0, 0, 0);
+          if (!PARTIAL || b < live) {
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+              acc[a][b] = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4_t, fa[a]), __builtin_bit_cast(i32x4_t, fb[b]), acc[a][b], 0, 0, 0);
+          }
+      }
+      cur = cur == 2 ? 0 : cur + 1;
+      nxt = nxt == 2 ? 0 : nxt + 1;
     }
-  }
-  // A lane holds 4 neighbouring n of one m; through a 4 KiB pad of its wave (in the stage memory nobody reads any more) a block of
-  // 32 x 32 leaves as rows of 8 outputs per lane.
+  };
+  if (live == MT)
+    steps(std::false_type{});
+  else
+    steps(std::true_type{});
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");         // the zero pieces of the steps past the end
   __syncthreads();
-  unsigned char* pad = smem + wave * 4096;
+  // A lane holds 4 neighbouring n of one m: it scales them by its row's xs.  Through an 8 KiB pad of its wave (in the stage memory nobody reads
+  // any more) 32 rows x 64 columns at a time leave as 8 outputs per lane, 8 lanes to a row; the lane's columns, and so their scales and
+  // biases, stay the same throughout.  Row scales and residuals are requested before they are needed.
+  unsigned char* pad = smem + wave * 8192;
+  const int c8 = lane & 7, r8 = lane >> 3;
+  const int n = n0 + wn * 64 + 8 * c8;
+  const int mw = m0 + wm * (32 * MT);
+  float xs[MT], ws[8], bias[8];
 #pragma unroll
-  for (int b = 0; b < MT; ++b)
+  for (int b = 0; b < MT; ++b) {
+    const int m = mw + 32 * b + l31;
+    xs[b] = p.xs[m < p.M ? m : p.M - 1];
+  }
 #pragma unroll
-    for (int a = 0; a < 2; ++a) {
+  for (int j = 0; j < 8; ++j) {
+    const int nn = n + j < p.N ? n + j : p.N - 1;
+    ws[j] = p.ws[nn];
+    bias[j] = p.bias ? p.bias[nn] : 0.0f;
+  }
+#pragma unroll
+  for (int b = 0; b < MT; ++b) {
+    if (b >= live) break;
+    const int mb = mw + 32 * b;
+    f32x8 res[4];
+    if (p.vec && p.res) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int m = mb + r8 + 8 * i;
+        if (m < p.M && n < p.N) res[i] = p.res_f32 ? load8((const float*)p.res + m * p.ldr + n) : load8((const L*)p.res + m * p.ldr + n);
+      }
+    }
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         f32x4_t v;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = (float)acc[a][b][4 * q + j];
-        *(f32x4_t*)(pad + l31 * 128 + (((2 * q + h) ^ (l31 & 7)) << 4)) = v;
+        for (int j = 0; j < 4; ++j) v[j] = (float)acc[a][b][4 * q + j] * xs[b];
+        *(f32x4_t*)(pad + l31 * 256 + (((8 * a + 2 * q + h) ^ (l31 & 15)) << 4)) = v;
       }
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-      const int cc = lane & 3;
-      const int n = n0 + wn * 64 + a * 32 + 8 * cc;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (p.vec) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int row = (lane >> 2) + 16 * i;
-        const int m = m0 + wm * (32 * MT) + b * 32 + row;
-        const f32x4_t lo = *(const f32x4_t*)(pad + row * 128 + (((2 * cc) ^ (row & 7)) << 4));
-        const f32x4_t hi = *(const f32x4_t*)(pad + row * 128 + (((2 * cc + 1) ^ (row & 7)) << 4));
-        const float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-        if (m < p.M && n < p.N) store_oct<L, YT, RT>(p, v, m, n);
+      for (int i = 0; i < 4; ++i) {
+        const int row = r8 + 8 * i, m = mb + row;
+        const f32x4_t lo = *(const f32x4_t*)(pad + row * 256 + (((2 * c8) ^ (row & 15)) << 4));
+        const f32x4_t hi = *(const f32x4_t*)(pad + row * 256 + (((2 * c8 + 1) ^ (row & 15)) << 4));
+        if (m < p.M && n < p.N) {
+          constexpr bool FAST = sizeof(YT) == 2;
+          f32x8 o, g;
+          if (p.aux) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) activate<FAST, ACT, true>(fmaf(j < 4 ? lo[j & 3] : hi[j & 3], ws[j], bias[j]), o.v[j], g.v[j]);
+            store8((L*)p.aux + (int64_t)m * p.N + n, g);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) activate<FAST, ACT, false>(fmaf(j < 4 ? lo[j & 3] : hi[j & 3], ws[j], bias[j]), o.v[j], g.v[j]);
+          }
+          if (p.res) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o.v[j] += res[i].v[j];
+          }
+          store8((YT*)p.y + m * p.ldy + n, o);
+        }
       }
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    } else {
+#pragma unroll 1
+      for (int x = lane; x < 32 * 64; x += 64) {             // odd widths or unaligned rows: one output at a time
+        const int row = x >> 6, col = x & 63;
+        const int m = mb + row, nn = n0 + wn * 64 + col;
+        const float v = *(const float*)(pad + row * 256 + (((col >> 2) ^ (row & 15)) << 4) + (col & 3) * 4);
+        if (m < p.M && nn < p.N) store_one<L, YT>(p, v, m, nn);
+      }
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
 }
 
-template <typename L, typename YT, typename RT, int BM, int BN>
-int launch_tile(const I8Args& p, hipStream_t st) {
-  constexpr int lds = 2 * (BM * 128 + BN * 128);
-  const int tiles_n = ceil_div(p.N, BN);
-  const int64_t n_tiles = (int64_t)ceil_div(p.M, BM) * tiles_n;
-  FFVC_CHECK_ARG(n_tiles < (1ll << 31), "ffvc_gemm_int8: too many tiles for one launch");
-  static ffvc_lds_once once;
-  const int rc = once.set((const void*)gemm_int8_kernel<L, YT, RT, BM, BN>, lds);
-  if (rc) return rc;
-  hipLaunchKernelGGL((gemm_int8_kernel<L, YT, RT, BM, BN>), dim3((unsigned)n_tiles), dim3(2 * BN), lds, st, p, tiles_n, (int)n_tiles);
+// ---- up to 64 rows of quantised x ----------------------------------------------------------------------------------------------------------
+// A workgroup owns 32 output columns, its eight waves take the 32-byte K steps in turn, operands straight from global memory (a lane reads the
+// 16 bytes of its row that its MFMA needs); the partial sums meet in LDS, exactly.  For small calls, and for the last up to 64 rows of large ones:
+// as a row of nearly empty tiles those walk the whole K loop alone once everything else is done.
+constexpr int SKINNY_M = 64;
+template <typename L, typename YT>
+__global__ __launch_bounds__(512) void gemm_int8_skinny_kernel(const I8Args p) {
+  __shared__ int part[8][32][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, h = lane >> 5;
+  const int n0 = blockIdx.x * 32;
+  const int8_t* wr = p.w + (int64_t)(n0 + l31 < p.N ? n0 + l31 : p.N - 1) * p.ldw;
+  const int8_t* x0 = p.x + (int64_t)(l31 < p.M ? l31 : 0) * p.ldx;
+  const int8_t* x1 = p.x + (int64_t)(32 + l31 < p.M ? 32 + l31 : 0) * p.ldx;
+  const bool two = p.M > 32;
+  i32x16_t acc[2];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) acc[0][i] = acc[1][i] = 0;
+  const u32x4_t z = {0u, 0u, 0u, 0u};
+#pragma unroll 4
+  for (int k = wave * 32; k < p.K; k += 256) {
+    const int kk = k + 16 * h;                               // K % 16 == 0: a 16-byte chunk is inside or outside
+    const bool in = kk < p.K;
+    const u32x4_t a = in ? *(const u32x4_t*)(wr + kk) : z;
+    const u32x4_t b0 = in && l31 < p.M ? *(const u32x4_t*)(x0 + kk) : z;
+    acc[0] = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4_t, a), __builtin_bit_cast(i32x4_t, b0), acc[0], 0, 0, 0);
+    if (two) {
+      const u32x4_t b1 = in && 32 + l31 < p.M ? *(const u32x4_t*)(x1 + kk) : z;
+      acc[1] = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4_t, a), __builtin_bit_cast(i32x4_t, b1), acc[1], 0, 0, 0);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    part[wave][i][lane] = acc[0][i];
+    part[wave][16 + i][lane] = acc[1][i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int x = tid + 512 * j, col = x & 31, m = x >> 5;   // consecutive lanes -> consecutive columns
+    // where the product's (column, row) sits: register 8 q + 4 h + e of the column's block, lane 32 h + row
+    const int reg = 16 * (m >> 5) + 4 * (col >> 3) + (col & 3), ln = 32 * ((col >> 2) & 1) + (m & 31);
+    int sum = 0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) sum += part[w][reg][ln];
+    if (m < p.M && n0 + col < p.N) store_one<L, YT>(p, (float)sum * p.xs[m], m, n0 + col);
+  }
+}
+
+template <typename L, typename YT>
+int launch_skinny(const I8Args& p, hipStream_t st) {
+  hipLaunchKernelGGL((gemm_int8_skinny_kernel<L, YT>), dim3(ceil_div(p.N, 32)), dim3(512), 0, st, p);
   FFVC_LAUNCH_CHECK();
   return 0;
 }
 
-template <typename L, typename YT, typename RT>
+template <typename L, typename YT, int ACT, int BM>
+int launch_tile(const I8Args& p, hipStream_t st) {
+  constexpr int lds = 3 * (BM + BN) * BK;
+  const int tiles_n = ceil_div(p.N, BN);
+  const int64_t n_tiles = (int64_t)ceil_div(p.M, BM) * tiles_n;
+  FFVC_CHECK_ARG(n_tiles < (1ll << 31), "ffvc_gemm_int8: too many tiles for one launch");
+  static ffvc_lds_once once;
+  const int rc = once.set((const void*)gemm_int8_kernel<L, YT, ACT, BM>, lds);
+  if (rc) return rc;
+  hipLaunchKernelGGL((gemm_int8_kernel<L, YT, ACT, BM>), dim3((unsigned)n_tiles), dim3(256), lds, st, p, tiles_n);
+  FFVC_LAUNCH_CHECK();
+  return 0;
+}
+
+template <typename L, typename YT, int ACT>
 int launch_gemm(const I8Args& p, hipStream_t st) {
-  const int64_t big = (int64_t)ceil_div(p.M, 256) * ceil_div(p.N, 256);
-  if (big >= 192) return launch_tile<L, YT, RT, 256, 256>(p, st);
-  return launch_tile<L, YT, RT, 128, 128>(p, st);
+  if (p.M <= SKINNY_M) return launch_skinny<L, YT>(p, st);
+  const int64_t big = (int64_t)(p.M / 256) * ceil_div(p.N, BN);
+  if (big < 512) return launch_tile<L, YT, ACT, 128>(p, st);
+  const int rest = p.M % 256;
+  if (rest == 0 || rest > SKINNY_M) return launch_tile<L, YT, ACT, 256>(p, st);
+  I8Args head = p, tail = p;
+  head.M = p.M - rest;
+  const int64_t m = head.M;
+  tail.M = rest;
+  tail.x += m * p.ldx;
+  tail.xs += m;
+  tail.y = (YT*)p.y + m * p.ldy;
+  if (p.res) tail.res = p.res_f32 ? (const void*)((const float*)p.res + m * p.ldr) : (const void*)((const L*)p.res + m * p.ldr);
+  if (p.aux) tail.aux = (L*)p.aux + m * p.N;
+  const int rc = launch_skinny<L, YT>(tail, st);             // (first: it runs beside the first tiles)
+  return rc ? rc : launch_tile<L, YT, ACT, 256>(head, st);
 }
 
 // ---- a handful of rows ---------------------------------------------------------------------------------------------------------------------
@@ -335,7 +474,7 @@ int launch_gemm(const I8Args& p, hipStream_t st) {
 // split K.  v_mfma_i32_16x16x64_i8: A = 16 weight rows straight from global memory, B = the quantised rows from LDS.
 constexpr int FEW_M = 16;
 
-template <typename L, typename YT, typename RT>
+template <typename L, typename YT>
 __global__ __launch_bounds__(256) void linear_int8_few_kernel(const L* __restrict__ x, const I8Args p) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -372,42 +511,33 @@ __global__ __launch_bounds__(256) void linear_int8_few_kernel(const L* __restric
   for (int r = 0; r < 4; ++r) part[(wave * 4 + r) * 64 + lane] = acc[r];
   __syncthreads();
   if (wave || l15 >= p.M) return;                           // column l15 of the product = row m, rows 4 g4 + r = output n0 + ...
-#pragma unroll
+#pragma unroll 1
   for (int r = 0; r < 4; ++r) {
     const int n = n0 + 4 * g4 + r;
     if (n >= p.N) break;
     int sum = 0;
 #pragma unroll
     for (int w = 0; w < 4; ++w) sum += part[(w * 4 + r) * 64 + lane];
-    const float zz = fmaf((float)sum, xs[l15] * p.ws[n], p.bias ? p.bias[n] : 0.0f);
-    float y, g;
-    act_and_grad<sizeof(YT) == 2>(p.act, zz, y, g);
-    if (p.res) y += ElemTraits<RT>::load((const RT*)p.res + l15 * p.ldr + n);
-    ElemTraits<YT>::store((YT*)p.y + l15 * p.ldy + n, y);
-    if (p.aux) ElemTraits<L>::store((L*)p.aux + (int64_t)l15 * p.N + n, g);
+    store_one<L, YT>(p, (float)sum * xs[l15], l15, n);
   }
 }
 
-template <typename L, typename YT, typename RT>
+template <typename L, typename YT>
 int launch_few(const void* x, const I8Args& p, hipStream_t st) {
   const int lds = p.M * (p.K + 16) + FEW_M * 4 + 4 * 4 * 64 * 4;
   static ffvc_lds_once once;
-  const int rc = once.set((const void*)linear_int8_few_kernel<L, YT, RT>, 160 * 1024);
+  const int rc = once.set((const void*)linear_int8_few_kernel<L, YT>, 160 * 1024);
   if (rc) return rc;
-  hipLaunchKernelGGL((linear_int8_few_kernel<L, YT, RT>), dim3(ceil_div(p.N, 16)), dim3(256), lds, st, (const L*)x, p);
+  hipLaunchKernelGGL((linear_int8_few_kernel<L, YT>), dim3(ceil_div(p.N, 16)), dim3(256), lds, st, (const L*)x, p);
   FFVC_LAUNCH_CHECK();
   return 0;
 }
 
-// the storage types of one call: 16-bit lo (x of the one-launch form, aux), y fp32 or lo, residual fp32 or lo
+// the storage types of one call: 16-bit lo (x of the one-launch form, aux, a 16-bit residual), y fp32 or lo
 template <typename F>
-int by_types(int lo, int y_dtype, int r_dtype, F&& f) {
-  auto with = [&](auto l) {
-    using L = decltype(l);
-    if (y_dtype == FFVC_F32) return r_dtype == FFVC_F32 ? f(L{}, float{}, float{}) : f(L{}, float{}, L{});
-    return r_dtype == FFVC_F32 ? f(L{}, L{}, float{}) : f(L{}, L{}, L{});
-  };
-  return lo == FFVC_F16 ? with(f16_t{}) : with(uint16_t{});
+int by_types(int lo, int y_dtype, F&& f) {
+  if (lo == FFVC_F16) return y_dtype == FFVC_F32 ? f(f16_t{}, float{}) : f(f16_t{}, f16_t{});
+  return y_dtype == FFVC_F32 ? f(uint16_t{}, float{}) : f(uint16_t{}, uint16_t{});
 }
 
 int check_out(const char* who, int lo, int M, int N, int K, const int8_t* w, int64_t ldw, const float* ws, const float* bias, int act, const void* res,
@@ -452,10 +582,15 @@ extern "C" int ffvc_gemm_int8(const int8_t* x, int64_t ldx, const float* xs, con
   const int rc = check_out("ffvc_gemm_int8", lo_dtype, M, N, K, w, ldw, ws, bias, act, residual, res_dtype, ldr, y, y_dtype, ldy);
   if (rc) return rc;
   FFVC_CHECK_ARG(x && xs && (uintptr_t)x % 16 == 0 && ldx % 16 == 0 && ldx >= K && ldx < (1 << 22), "ffvc_gemm_int8: x rows must be 16-byte aligned");
-  I8Args p{x, w, xs, ws, bias, residual, y, actgrad, ldx, ldw, ldy, ldr, M, N, K, act, 0};
+  I8Args p{x, w, xs, ws, bias, residual, y, actgrad, ldx, ldw, ldy, ldr, M, N, K, act, res_dtype == FFVC_F32, 0};
   p.vec = N % 8 == 0 && rows_vec(y, y_dtype, ldy) && (!residual || rows_vec(residual, res_dtype, ldr)) && (!actgrad || rows_vec(actgrad, lo_dtype, N));
-  return by_types(lo_dtype, y_dtype, residual ? res_dtype : y_dtype, [&](auto l, auto yt, auto rt) {
-    return launch_gemm<decltype(l), decltype(yt), decltype(rt)>(p, (hipStream_t)stream);
+  hipStream_t st = (hipStream_t)stream;
+  return by_types(lo_dtype, y_dtype, [&](auto l, auto yt) {
+    using L = decltype(l);
+    using YT = decltype(yt);
+    if (act == FFVC_ACT_GELU) return launch_gemm<L, YT, FFVC_ACT_GELU>(p, st);
+    if (act == FFVC_ACT_QUICKGELU) return launch_gemm<L, YT, FFVC_ACT_QUICKGELU>(p, st);
+    return launch_gemm<L, YT, FFVC_ACT_NONE>(p, st);
   });
 }
 
@@ -470,8 +605,6 @@ extern "C" int ffvc_linear_int8_few(const void* x, int lo_dtype, int64_t ldx, co
   if (rc) return rc;
   FFVC_CHECK_ARG(ffvc_linear_int8_few_ok(M, K), "ffvc_linear_int8_few: M=%d K=%d unsupported", M, K);
   FFVC_CHECK_ARG(x && (uintptr_t)x % 16 == 0 && ldx % 8 == 0 && ldx >= K, "ffvc_linear_int8_few: x rows must be 16-byte aligned");
-  const I8Args p{nullptr, w, nullptr, ws, bias, residual, y, actgrad, ldx, ldw, ldy, ldr, M, N, K, act, 0};
-  return by_types(lo_dtype, y_dtype, residual ? res_dtype : y_dtype, [&](auto l, auto yt, auto rt) {
-    return launch_few<decltype(l), decltype(yt), decltype(rt)>(x, p, (hipStream_t)stream);
-  });
+  const I8Args p{nullptr, w, nullptr, ws, bias, residual, y, actgrad, ldx, ldw, ldy, ldr, M, N, K, act, res_dtype == FFVC_F32, 0};
+  return by_types(lo_dtype, y_dtype, [&](auto l, auto yt) { return launch_few<decltype(l), decltype(yt)>(x, p, (hipStream_t)stream); });
 }

@@ -1563,18 +1563,29 @@ def avgpool_patches_bwd(gout, N, S, out_size, patch, std):
 # ---------------------------------------------------------------------------
 # packed prompts: embedding, causal attention over sequences of different lengths, 8-bit integer Linear
 # ---------------------------------------------------------------------------
+class _Nothing:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_NOTHING = _Nothing()
+
+
 def _same_device(*ts):
     """Context in which these tensors' device is the current one (the launch goes to ITS current stream); they must share it."""
-    dev = None
+    dev = -1
     for t in ts:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise _lib.FFVCError("ffvc kernels need CUDA(HIP) tensors; there is no CPU fallback")
-        if dev is not None and t.device != dev:
-            raise ValueError(f"ffvc launcher: tensors on {dev} and {t.device}")
-        dev = t.device
-    return torch.cuda.device(dev)
+        if t is not None:
+            i = t.get_device()
+            if i < 0:
+                raise _lib.FFVCError("ffvc kernels need CUDA(HIP) tensors; there is no CPU fallback")
+            if dev >= 0 and i != dev:
+                raise ValueError(f"ffvc launcher: tensors on cuda:{dev} and cuda:{i}")
+            dev = i
+    return _NOTHING if dev == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
 def _rows2d(name, t):
@@ -1630,7 +1641,7 @@ def embed_bwd(dout, ids, rows, scale=1.0, out_dtype=None):
         if n == 0 or rows == 0 or dim == 0:
             return torch.zeros(rows, dim, dtype=dt, device=dout.device)
         grad = torch.empty(rows, dim, dtype=dt, device=dout.device)
-        nb = int(_lib.load().ffvc_embed_bwd_ws_bytes(n, dim))
+        nb = int(_lib.load().ffvc_embed_bwd_ws_bytes(n, rows, dim))
         ws = torch.empty(nb, dtype=torch.uint8, device=dout.device)
         _call("ffvc_embed_bwd", d2.data_ptr(), dtype_code(d2.dtype), ld, ids.data_ptr(), n, rows, dim, float(scale), grad.data_ptr(), dtype_code(dt),
               ws.data_ptr(), nb, stream_ptr())

@@ -563,8 +563,8 @@ int ffvc_embed_fwd(const void* table, int table_dtype, int64_t ld, int64_t vocab
                    int64_t npos, const int64_t* place, void* out, int out_dtype, int64_t ldo, int64_t n, int dim, void* stream);
 /* dtable[v] = scale * sum_{t: ids[t] = v} dout[t] for every row v of the contiguous [vocab, dim] gradient (rows without a token are written as
  * zeros; ids outside the table add nothing).  Summed in fp32 in the order of t: the same bits on every call.  ws: ffvc_embed_bwd_ws_bytes(n,
- * dim) bytes, 16-byte aligned, contents irrelevant before and after. */
-int64_t ffvc_embed_bwd_ws_bytes(int64_t n, int dim);
+ * vocab, dim) bytes, 16-byte aligned, contents irrelevant before and after. */
+int64_t ffvc_embed_bwd_ws_bytes(int64_t n, int64_t vocab, int dim);
 int ffvc_embed_bwd(const void* dout, int dout_dtype, int64_t ld, const int64_t* ids, int64_t n, int64_t vocab, int dim, float scale, void* dtable,
                    int table_dtype, void* ws, int64_t ws_bytes, void* stream);
 

@@ -128,8 +128,8 @@ def test_c_entry_points_refuse_bad_arguments():
         return lib.ffvc_embed_fwd(table, dt, ld, V, ids, 1.0, pos, pld, npos, 0, out, odt, ldo, n, dim, None)
     for kw in (dict(table=0), dict(dt=7), dict(ld=7), dict(V=0), dict(ids=0), dict(pos=A), dict(out=0), dict(odt=-1), dict(ldo=4), dict(n=0), dict(dim=0)):
         assert embed_fwd(**kw) != 0, kw
-    need = lib.ffvc_embed_bwd_ws_bytes(100, 8)
-    assert need > 0 and lib.ffvc_embed_bwd_ws_bytes(0, 8) == 0
+    need = lib.ffvc_embed_bwd_ws_bytes(100, 5, 8)
+    assert need > 0 and lib.ffvc_embed_bwd_ws_bytes(0, 5, 8) == 0
 
     def embed_bwd(dout=A, dt=1, ld=8, ids=A, n=100, V=5, dim=8, grad=A, gdt=1, ws=A, nb=need):
         return lib.ffvc_embed_bwd(dout, dt, ld, ids, n, V, dim, 1.0, grad, gdt, ws, nb, None)
