@@ -244,7 +244,7 @@ _SIGNATURES = {
     "ffvc_attn_packed_fwd": (c_int, [POINTER(AttnPackedDesc), c_void_p]),
     "ffvc_attn_packed_bwd": (c_int, [POINTER(AttnPackedDesc), c_void_p]),
     "ffvc_int8_quant": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p]),
-    "ffvc_gemm_int8": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int64, c_void_p, c_int,
+    "ffvc_gemm_int8": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int64, c_void_p, c_int,
                                c_int64, c_void_p, c_int, c_int, c_int, c_int, c_void_p]),
     "ffvc_linear_int8_few_ok": (c_int, [c_int, c_int]),
     "ffvc_linear_int8_few": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int64, c_void_p, c_int,

@@ -89,6 +89,12 @@ __device__ __forceinline__ float wave_amax(float m) {
   return m;
 }
 
+// Where the quantised value (row, k) goes: rows of ldq bytes, or (ldq 0) panels of 64 consecutive k, [ceil(K / 64)][rows][64], the last one
+// filled up with zeros.  In panels the 64-byte pieces of neighbouring rows share a cache line, so a K step of the product reads whole lines.
+__device__ __forceinline__ int8_t* q_at(int8_t* q, int64_t ldq, int64_t rows, int64_t row, int k) {
+  return ldq ? q + row * ldq + k : q + ((int64_t)(k >> 6) * rows + row) * 64 + (k & 63);
+}
+
 // One wave per row; a row of up to 64 * 8 * CH values stays in registers between the two passes, longer ones are read again (from L2).
 template <typename T, int CH>
 __global__ __launch_bounds__(256) void int8_quant_kernel(const T* __restrict__ x, int64_t ldx, int8_t* __restrict__ q, int64_t ldq,
@@ -97,17 +103,17 @@ __global__ __launch_bounds__(256) void int8_quant_kernel(const T* __restrict__ x
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= rows) return;
   const T* xr = x + row * ldx;
-  int8_t* qr = q + row * ldq;
+  const int Kq = ldq ? K : (K + 63) & ~63;
   f32x8 v[CH];
   float m = 0.0f;
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
     const int k = (i * 64 + lane) * 8;
-    if (k < K) {
-      v[i] = load8(xr + k);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) m = amax_with_nan(m, v[i].v[j]);
-    }
+    for (int j = 0; j < 8; ++j) v[i].v[j] = 0.0f;
+    if (k < K) v[i] = load8(xr + k);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = amax_with_nan(m, v[i].v[j]);
   }
   for (int k = (CH * 64 + lane) * 8; k < K; k += 512) {
     const f32x8 t = load8(xr + k);
@@ -120,9 +126,13 @@ __global__ __launch_bounds__(256) void int8_quant_kernel(const T* __restrict__ x
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
     const int k = (i * 64 + lane) * 8;
-    if (k < K) *(u32x2_t*)(qr + k) = quant8(v[i], rq);
+    if (k < Kq) *(u32x2_t*)q_at(q, ldq, rows, row, k) = quant8(v[i], rq);
   }
-  for (int k = (CH * 64 + lane) * 8; k < K; k += 512) *(u32x2_t*)(qr + k) = quant8(load8(xr + k), rq);
+  for (int k = (CH * 64 + lane) * 8; k < Kq; k += 512) {
+    u32x2_t o = {0u, 0u};
+    if (k < K) o = quant8(load8(xr + k), rq);
+    *(u32x2_t*)q_at(q, ldq, rows, row, k) = o;
+  }
 }
 
 // ---- epilogue ----------------------------------------------------------------------------------------------------------------------
@@ -171,7 +181,8 @@ struct I8Args {
   const void* res;
   void* y;
   void* aux;              // act'(pre-activation), may be null
-  int64_t ldx, ldw, ldy, ldr;
+  int64_t xrows;          // rows of a panel of x (quantised), or the row stride of 16-bit x (linear_int8_few)
+  int64_t ldw, ldy, ldr;
   int M, N, K;
   int act;
   int res_f32;
@@ -190,48 +201,74 @@ __device__ __forceinline__ void store_one(const I8Args& p, float v, int64_t m, i
 }
 
 // ---- the tiled product -----------------------------------------------------------------------------------------------------------------
-// BM x 128 outputs per workgroup of four waves ((BM / 2) x 64 each), K steps of 64 bytes in a ring of three LDS stages filled by LDS-DMA two
-// steps ahead (one barrier per step, the youngest stage may still be in flight).  Two (BM = 256: 72 KiB) or three (BM = 128: 48 KiB) workgroups
-// share a CU, so the epilogue of one, as long as its K loop where K is 1024 and an activation is due, runs under the products of another.
-// A staged row is 64 bytes, four rows to a 256-byte line, its 16-byte chunks XOR-swizzled by the line: the fragment reads hit every bank evenly.
+// BM x 128 outputs per workgroup of four waves ((BM / 2) x 64 each), K steps of 64 bytes.  x comes in panels (see q_at), a step of a tile is one
+// contiguous block, three LDS slots; w keeps its rows, two steps (128 bytes, a whole cache line of each row) at a time, two slots.  LDS-DMA
+// runs two steps ahead with one barrier per step, the youngest pieces may still be under way.  Two workgroups share a CU (BM = 256: 80 KiB
+// each), so the epilogue of one, as long as its K loop where K is 1024 and an activation is due, runs under the products of the other.
+// (With 64-byte steps of plain rows every step fetched each line twice: 104 us at 16448 x 4096 x 1024.)
+// 16-byte chunks are XOR-swizzled inside 256-byte lines (4 rows of x, 2 of w): the fragment reads hit every bank evenly.
 constexpr int BN = 128, BK = 64;
 
-__device__ __forceinline__ u32x4_t frag_i8(const unsigned char* tile, int row, int chunk) {
+__device__ __forceinline__ u32x4_t frag_x(const unsigned char* tile, int row, int chunk) {        // chunk 0..3
   return *(const u32x4_t*)(tile + row * 64 + ((chunk ^ ((row >> 2) & 3)) << 4));
 }
+__device__ __forceinline__ u32x4_t frag_w(const unsigned char* tile, int row, int chunk) {        // chunk 0..7
+  const int line = row >> 1;
+  return *(const u32x4_t*)(tile + line * 256 + (((((row & 1) << 3) | chunk) ^ (line & 15)) << 4));
+}
 
-// the staging of `ROWS` rows by NW waves: a piece is 16 rows; the lane's row and source chunk inside a piece are the same for every piece
-template <int ROWS, int NW>
-struct RowsDma {
-  static constexpr int NP = ROWS / (16 * NW);
+// staging of BM panel rows by four waves: a piece is 16 rows of 64 bytes
+template <int ROWS>
+struct PanelDma {
+  static constexpr int NP = ROWS / 64;
+  const int8_t* base;
+  int64_t panel;
+  uint32_t off[NP];
+  int bytes;
+  __device__ __forceinline__ void init(const int8_t* x, int64_t xrows, int row0, int rows, int wave, int lane) {
+    const int live = rows - row0 < ROWS ? rows - row0 : ROWS;
+    base = x + (int64_t)row0 * 64;
+    panel = xrows * 64;
+    bytes = live * 64;                                       // rows past the end read as zeros
+    const int chunk = (lane & 3) ^ ((lane >> 4) & 3);
+#pragma unroll
+    for (int i = 0; i < NP; ++i) off[i] = ((wave * NP + i) * 16 + (lane >> 2)) * 64 + chunk * 16;
+  }
+  __device__ __forceinline__ void issue(unsigned char* tile, int kt, int nk, int wave) {      // steps past the last one fetch zeros
+    const rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(base + (kt < nk ? kt : 0) * panel), 0, kt < nk ? bytes : 0, 0x00020000);
+#pragma unroll
+    for (int i = 0; i < NP; ++i) dma16(rs, off[i], 0, tile + (wave * NP + i) * 1024);
+  }
+};
+// staging of 128 rows of w, 128 bytes wide, by four waves: a piece is 8 rows
+struct WideDma {
+  static constexpr int NP = 4;
   rsrc_t rs;
   uint32_t off[NP];
-  int chunk;
-  // rows row0 .. of a matrix with `rows` rows of K bytes; the descriptor ends with the last staged row, rows past it read as zeros
-  __device__ __forceinline__ void init(const int8_t* base, int64_t ld, int row0, int rows, int K, int wave, int lane) {
-    const int live = rows - row0 < ROWS ? rows - row0 : ROWS;
-    rs = __builtin_amdgcn_make_buffer_rsrc((void*)(base + row0 * ld), 0, (int)((live - 1) * ld + K), 0x00020000);
-    chunk = ((lane & 3) ^ ((lane >> 4) & 3)) * 16;
+  int chunk[NP];
+  __device__ __forceinline__ void init(const int8_t* w, int64_t ld, int row0, int rows, int K, int wave, int lane) {
+    const int live = rows - row0 < BN ? rows - row0 : BN;
+    rs = __builtin_amdgcn_make_buffer_rsrc((void*)(w + row0 * ld), 0, (int)((live - 1) * ld + K), 0x00020000);
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      const int row = (wave * NP + i) * 16 + (lane >> 2);
-      off[i] = row < live ? (uint32_t)(row * ld + chunk) : OOB;
+      const int line = (wave * NP + i) * 4 + (lane >> 4), cp = (lane & 15) ^ (line & 15);
+      const int row = 2 * line + (cp >> 3);
+      chunk[i] = (cp & 7) * 16;
+      off[i] = row < live ? (uint32_t)(row * ld + chunk[i]) : OOB;
     }
   }
-  // K step k0 (wave-uniform): interior steps cost no address arithmetic, the last one drops the chunks past K, steps past the end fetch zeros
-  __device__ __forceinline__ void issue(unsigned char* tile, int k0, int K, int wave) {
-    const bool whole = k0 + BK <= K;
-    const bool in = k0 + chunk < K;
+  __device__ __forceinline__ void issue(unsigned char* tile, int k0, int K, int wave) {       // (chunks past K read as zeros)
 #pragma unroll
-    for (int i = 0; i < NP; ++i) dma16(rs, whole || in ? off[i] : OOB, k0 < K ? k0 : 0, tile + (wave * NP + i) * 1024);
+    for (int i = 0; i < NP; ++i) dma16(rs, k0 + chunk[i] < K ? off[i] : OOB, k0 < K ? k0 : 0, tile + (wave * NP + i) * 1024);
   }
 };
 
 template <typename L, typename YT, int ACT, int BM>
 __global__ __launch_bounds__(256, 2) void gemm_int8_kernel(const I8Args p, int tiles_n) {
-  constexpr int MT = BM / 64, XT = BM * BK, STAGE = (BM + BN) * BK;
-  constexpr int PIECES = (BM + BN) / 64;                  // LDS-DMA instructions per wave and stage
+  constexpr int MT = BM / 64, XS = BM * BK, WS = BN * 128;
+  constexpr int XP = PanelDma<BM>::NP, WP = WideDma::NP;  // LDS-DMA instructions per wave and slot
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  unsigned char* wmem = smem + 3 * XS;
   const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave & 1, wn = wave >> 1;
@@ -245,9 +282,9 @@ __global__ __launch_bounds__(256, 2) void gemm_int8_kernel(const I8Args p, int t
   }
   const int tm = tile / tiles_n, tn = tile - tm * tiles_n;
   const int m0 = tm * BM, n0 = tn * BN;
-  RowsDma<BM, 4> dx;
-  RowsDma<BN, 4> dw;
-  dx.init(p.x, p.ldx, m0, p.M, p.K, wave, lane);
+  PanelDma<BM> dx;
+  WideDma dw;
+  dx.init(p.x, p.xrows, m0, p.M, wave, lane);
   dw.init(p.w, p.ldw, n0, p.N, p.K, wave, lane);
   i32x16_t acc[2][MT];
 #pragma unroll
@@ -258,42 +295,51 @@ __global__ __launch_bounds__(256, 2) void gemm_int8_kernel(const I8Args p, int t
       for (int i = 0; i < 16; ++i) acc[a][b][i] = 0;
   const int nk = (p.K + BK - 1) / BK;
   const int live = min(MT, (p.M - m0 - wm * (32 * MT) + 31) / 32);   // 32-row blocks of this wave that hold a row (may be < 1)
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    dx.issue(smem + t * STAGE, t * BK, p.K, wave);
-    dw.issue(smem + t * STAGE + XT, t * BK, p.K, wave);
-  }
+  dx.issue(smem, 0, nk, wave);
+  dw.issue(wmem, 0, p.K, wave);
+  dx.issue(smem + XS, 1, nk, wave);
   auto steps = [&](auto partial) {
     constexpr bool PARTIAL = decltype(partial)::value;
     int cur = 0, nxt = 2;
-#pragma unroll 1
-    for (int kt = 0; kt < nk; ++kt) {
-      // my pieces of this step have landed (those of the next may be under way), then everyone's; and nobody reads the slot filled next
-      // (the bare barrier: __syncthreads would wait for the pieces under way as well)
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PIECES) : "memory");
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      dx.issue(smem + nxt * STAGE, (kt + 2) * BK, p.K, wave);
-      dw.issue(smem + nxt * STAGE + XT, (kt + 2) * BK, p.K, wave);
-      const unsigned char* sx = smem + cur * STAGE;
-      const unsigned char* sw = sx + XT;
+    auto step = [&](int kt, const unsigned char* sw, int half) {
+      const unsigned char* sx = smem + cur * XS;
+      u32x4_t fa[2][2], fb[2][MT];                          // the whole step's fragments are requested before its first product
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        u32x4_t fa[2], fb[MT];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) fa[t] = frag_i8(sw, wn * 64 + t * 32 + l31, 2 * s + h);
+        for (int t = 0; t < 2; ++t) fa[s][t] = frag_w(sw, wn * 64 + t * 32 + l31, 4 * half + 2 * s + h);
 #pragma unroll
-        for (int t = 0; t < MT; ++t) fb[t] = frag_i8(sx, wm * (32 * MT) + t * 32 + l31, 2 * s + h);
+        for (int t = 0; t < MT; ++t) fb[s][t] = frag_x(sx, wm * (32 * MT) + t * 32 + l31, 2 * s + h);
+      }
+      if constexpr (!PARTIAL) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int b = 0; b < MT; ++b)
           if (!PARTIAL || b < live) {
 #pragma unroll
             for (int a = 0; a < 2; ++a)
-              acc[a][b] = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4_t, fa[a]), __builtin_bit_cast(i32x4_t, fb[b]), acc[a][b], 0, 0, 0);
+              acc[a][b] = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4_t, fa[s][a]), __builtin_bit_cast(i32x4_t, fb[s][b]), acc[a][b], 0, 0, 0);
           }
-      }
       cur = cur == 2 ? 0 : cur + 1;
       nxt = nxt == 2 ? 0 : nxt + 1;
+    };
+#pragma unroll 1
+    for (int kt = 0; kt < nk; kt += 2) {
+      const unsigned char* sw = wmem + ((kt >> 1) & 1) * WS;
+      // my pieces of this step have landed (x of the next may be under way), then everyone's; and nobody reads the slots filled next
+      // (the bare barrier: __syncthreads would wait for the pieces under way as well)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(XP) : "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      dx.issue(smem + nxt * XS, kt + 2, nk, wave);
+      dw.issue(wmem + (((kt >> 1) & 1) ^ 1) * WS, (kt + 2) * BK, p.K, wave);
+      step(kt, sw, 0);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(XP + WP) : "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      dx.issue(smem + nxt * XS, kt + 3, nk, wave);
+      step(kt + 1, sw, 1);                                  // (an odd last step multiplies zeros)
     }
   };
   if (live == MT)
@@ -381,9 +427,9 @@ __global__ __launch_bounds__(256, 2) void gemm_int8_kernel(const I8Args p, int t
 }
 
 // ---- up to 64 rows of quantised x ----------------------------------------------------------------------------------------------------------
-// A workgroup owns 32 output columns, its eight waves take the 32-byte K steps in turn, operands straight from global memory (a lane reads the
-// 16 bytes of its row that its MFMA needs); the partial sums meet in LDS, exactly.  For small calls, and for the last up to 64 rows of large ones:
-// as a row of nearly empty tiles those walk the whole K loop alone once everything else is done.
+// A workgroup owns 32 output columns, its eight waves take pairs of K panels (a 128-byte line of every weight row) in turn, operands straight
+// from global memory (a lane reads the 16 bytes of its row that its MFMA needs); the partial sums meet in LDS, exactly.  For small calls, and
+// for the last up to 64 rows of large ones: as a row of nearly empty tiles those walk the whole K loop alone once everything else is done.
 constexpr int SKINNY_M = 64;
 template <typename L, typename YT>
 __global__ __launch_bounds__(512) void gemm_int8_skinny_kernel(const I8Args p) {
@@ -391,23 +437,29 @@ __global__ __launch_bounds__(512) void gemm_int8_skinny_kernel(const I8Args p) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, h = lane >> 5;
   const int n0 = blockIdx.x * 32;
   const int8_t* wr = p.w + (int64_t)(n0 + l31 < p.N ? n0 + l31 : p.N - 1) * p.ldw;
-  const int8_t* x0 = p.x + (int64_t)(l31 < p.M ? l31 : 0) * p.ldx;
-  const int8_t* x1 = p.x + (int64_t)(32 + l31 < p.M ? 32 + l31 : 0) * p.ldx;
-  const bool two = p.M > 32;
+  const bool in0 = l31 < p.M, in1 = 32 + l31 < p.M, two = p.M > 32;
+  const int8_t* x0 = p.x + (in0 ? l31 : 0) * 64 + 16 * h;
+  const int8_t* x1 = p.x + (in1 ? 32 + l31 : 0) * 64 + 16 * h;
+  const int64_t panel = p.xrows * 64;
   i32x16_t acc[2];
 #pragma unroll
   for (int i = 0; i < 16; ++i) acc[0][i] = acc[1][i] = 0;
   const u32x4_t z = {0u, 0u, 0u, 0u};
-#pragma unroll 4
-  for (int k = wave * 32; k < p.K; k += 256) {
-    const int kk = k + 16 * h;                               // K % 16 == 0: a 16-byte chunk is inside or outside
-    const bool in = kk < p.K;
-    const u32x4_t a = in ? *(const u32x4_t*)(wr + kk) : z;
-    const u32x4_t b0 = in && l31 < p.M ? *(const u32x4_t*)(x0 + kk) : z;
-    acc[0] = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4_t, a), __builtin_bit_cast(i32x4_t, b0), acc[0], 0, 0, 0);
-    if (two) {
-      const u32x4_t b1 = in && 32 + l31 < p.M ? *(const u32x4_t*)(x1 + kk) : z;
-      acc[1] = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4_t, a), __builtin_bit_cast(i32x4_t, b1), acc[1], 0, 0, 0);
+  for (int k0 = wave * 128; k0 < p.K; k0 += 1024) {
+    u32x4_t a[4], b0[4], b1[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int kk = k0 + 32 * s + 16 * h;                   // K % 16 == 0: a 16-byte chunk is inside or outside
+      const bool in = kk < p.K;
+      const int64_t at = (k0 / 64 + s / 2) * panel + 32 * (s & 1);
+      a[s] = in ? *(const u32x4_t*)(wr + kk) : z;
+      b0[s] = in && in0 ? *(const u32x4_t*)(x0 + at) : z;
+      b1[s] = in && in1 ? *(const u32x4_t*)(x1 + at) : z;
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      acc[0] = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4_t, a[s]), __builtin_bit_cast(i32x4_t, b0[s]), acc[0], 0, 0, 0);
+      if (two) acc[1] = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4_t, a[s]), __builtin_bit_cast(i32x4_t, b1[s]), acc[1], 0, 0, 0);
     }
   }
 #pragma unroll
@@ -437,7 +489,7 @@ int launch_skinny(const I8Args& p, hipStream_t st) {
 
 template <typename L, typename YT, int ACT, int BM>
 int launch_tile(const I8Args& p, hipStream_t st) {
-  constexpr int lds = 3 * (BM + BN) * BK;
+  constexpr int lds = 3 * BM * BK + 2 * BN * 128;
   const int tiles_n = ceil_div(p.N, BN);
   const int64_t n_tiles = (int64_t)ceil_div(p.M, BM) * tiles_n;
   FFVC_CHECK_ARG(n_tiles < (1ll << 31), "ffvc_gemm_int8: too many tiles for one launch");
@@ -460,7 +512,7 @@ int launch_gemm(const I8Args& p, hipStream_t st) {
   head.M = p.M - rest;
   const int64_t m = head.M;
   tail.M = rest;
-  tail.x += m * p.ldx;
+  tail.x += m * 64;
   tail.xs += m;
   tail.y = (YT*)p.y + m * p.ldy;
   if (p.res) tail.res = p.res_f32 ? (const void*)((const float*)p.res + m * p.ldr) : (const void*)((const L*)p.res + m * p.ldr);
@@ -482,7 +534,7 @@ __global__ __launch_bounds__(256) void linear_int8_few_kernel(const L* __restric
   float* xs = (float*)(smem + p.M * ldk);                   // [16]
   int* part = (int*)(xs + FEW_M);                           // [4 waves][4][64]
   for (int r = wave; r < p.M; r += 4) {
-    const L* xr = x + r * p.ldx;
+    const L* xr = x + r * p.xrows;
     float m = 0.0f;
     for (int k = lane * 8; k < p.K; k += 512) {
       const f32x8 v = load8(xr + k);
@@ -559,7 +611,7 @@ bool rows_vec(const void* p, int dtype, int64_t ld) { return (uintptr_t)p % 16 =
 extern "C" int ffvc_int8_quant(const void* x, int x_dtype, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t rows, int K, void* stream) {
   FFVC_CHECK_ARG(x && q && scale && rows > 0 && K > 0 && K % 16 == 0, "ffvc_int8_quant: bad args (K must be a multiple of 16)");
   FFVC_CHECK_ARG(ffvc_dtype_ok(x_dtype), "ffvc_int8_quant: bad dtype %d", x_dtype);
-  FFVC_CHECK_ARG((uintptr_t)x % 16 == 0 && ldx % (16 / ffvc_dtype_size(x_dtype)) == 0 && ldx >= K && (uintptr_t)q % 16 == 0 && ldq % 16 == 0 && ldq >= K,
+  FFVC_CHECK_ARG((uintptr_t)x % 16 == 0 && ldx % (16 / ffvc_dtype_size(x_dtype)) == 0 && ldx >= K && (uintptr_t)q % 16 == 0 && ldq % 16 == 0 && (ldq == 0 || ldq >= K),
                  "ffvc_int8_quant: rows must be 16-byte aligned");
   FFVC_CHECK_ARG((rows + 3) / 4 < (1ll << 31), "ffvc_int8_quant: too many rows");
   const dim3 grid((unsigned)((rows + 3) / 4)), block(256);
@@ -576,13 +628,13 @@ extern "C" int ffvc_int8_quant(const void* x, int x_dtype, int64_t ldx, int8_t* 
   return 0;
 }
 
-extern "C" int ffvc_gemm_int8(const int8_t* x, int64_t ldx, const float* xs, const int8_t* w, int64_t ldw, const float* ws, const float* bias, int act,
+extern "C" int ffvc_gemm_int8(const int8_t* x, const float* xs, const int8_t* w, int64_t ldw, const float* ws, const float* bias, int act,
                               const void* residual, int res_dtype, int64_t ldr, void* y, int y_dtype, int64_t ldy, void* actgrad, int lo_dtype, int M,
                               int N, int K, void* stream) {
   const int rc = check_out("ffvc_gemm_int8", lo_dtype, M, N, K, w, ldw, ws, bias, act, residual, res_dtype, ldr, y, y_dtype, ldy);
   if (rc) return rc;
-  FFVC_CHECK_ARG(x && xs && (uintptr_t)x % 16 == 0 && ldx % 16 == 0 && ldx >= K && ldx < (1 << 22), "ffvc_gemm_int8: x rows must be 16-byte aligned");
-  I8Args p{x, w, xs, ws, bias, residual, y, actgrad, ldx, ldw, ldy, ldr, M, N, K, act, res_dtype == FFVC_F32, 0};
+  FFVC_CHECK_ARG(x && xs && (uintptr_t)x % 16 == 0, "ffvc_gemm_int8: x must be non-null and 16-byte aligned");
+  I8Args p{x, w, xs, ws, bias, residual, y, actgrad, M, ldw, ldy, ldr, M, N, K, act, res_dtype == FFVC_F32, 0};
   p.vec = N % 8 == 0 && rows_vec(y, y_dtype, ldy) && (!residual || rows_vec(residual, res_dtype, ldr)) && (!actgrad || rows_vec(actgrad, lo_dtype, N));
   hipStream_t st = (hipStream_t)stream;
   return by_types(lo_dtype, y_dtype, [&](auto l, auto yt) {

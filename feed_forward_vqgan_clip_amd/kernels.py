@@ -1771,9 +1771,9 @@ def linear_int8(x, wq, ws, bias=None, act=ACT_NONE, residual=None, out_dtype=Non
                 _call("ffvc_linear_int8_few", x2.data_ptr(), lo, ld, wq.data_ptr(), K, ws.data_ptr(), _ptr(bias), act, _ptr(residual), rdt, N,
                       y.data_ptr(), dtype_code(out_dtype), N, _ptr(g), M, N, K, stream_ptr())
             else:
-                xq = torch.empty(M, K, dtype=torch.int8, device=x.device)
+                xq = torch.empty((K + 63) // 64, M, 64, dtype=torch.int8, device=x.device)      # K panels
                 xs = torch.empty(M, dtype=torch.float32, device=x.device)
-                _call("ffvc_int8_quant", x2.data_ptr(), lo, ld, xq.data_ptr(), K, xs.data_ptr(), M, K, stream_ptr())
-                _call("ffvc_gemm_int8", xq.data_ptr(), K, xs.data_ptr(), wq.data_ptr(), K, ws.data_ptr(), _ptr(bias), act, _ptr(residual), rdt, N,
+                _call("ffvc_int8_quant", x2.data_ptr(), lo, ld, xq.data_ptr(), 0, xs.data_ptr(), M, K, stream_ptr())
+                _call("ffvc_gemm_int8", xq.data_ptr(), xs.data_ptr(), wq.data_ptr(), K, ws.data_ptr(), _ptr(bias), act, _ptr(residual), rdt, N,
                       y.data_ptr(), dtype_code(out_dtype), N, _ptr(g), lo, M, N, K, stream_ptr())
     return (y, g) if want_actgrad else y

@@ -142,10 +142,10 @@ def test_c_entry_points_refuse_bad_arguments():
     for kw in (dict(x=0), dict(x=A + 2), dict(dt=5), dict(ldx=16), dict(ldx=33), dict(q=A + 8), dict(ldq=40), dict(s=0), dict(rows=0), dict(k=24)):
         assert quant(**kw) != 0, kw
 
-    def gemm(x=A, ldx=32, xs=A, w=A, ldw=32, ws=A, act=0, res=0, rdt=1, ldr=8, y=A, ydt=0, ldy=8, lo=0, M=4, N=8, k=32):
-        return lib.ffvc_gemm_int8(x, ldx, xs, w, ldw, ws, 0, act, res, rdt, ldr, y, ydt, ldy, 0, lo, M, N, k, None)
-    for kw in (dict(x=0), dict(x=A + 1), dict(ldx=24), dict(xs=0), dict(w=0), dict(ldw=16), dict(ws=0), dict(act=3), dict(res=A, rdt=2), dict(res=A, ldr=7),
-               dict(y=0), dict(ydt=2), dict(ldy=7), dict(lo=1), dict(M=0), dict(N=0), dict(k=0), dict(k=40), dict(k=131088, ldx=131088, ldw=131088)):
+    def gemm(x=A, xs=A, w=A, ldw=32, ws=A, act=0, res=0, rdt=1, ldr=8, y=A, ydt=0, ldy=8, lo=0, M=4, N=8, k=32):
+        return lib.ffvc_gemm_int8(x, xs, w, ldw, ws, 0, act, res, rdt, ldr, y, ydt, ldy, 0, lo, M, N, k, None)
+    for kw in (dict(x=0), dict(x=A + 1), dict(xs=0), dict(w=0), dict(ldw=16), dict(ws=0), dict(act=3), dict(res=A, rdt=2), dict(res=A, ldr=7),
+               dict(y=0), dict(ydt=2), dict(ldy=7), dict(lo=1), dict(M=0), dict(N=0), dict(k=0), dict(k=40), dict(k=131088, ldw=131088)):
         assert gemm(**kw) != 0, kw
     assert lib.ffvc_linear_int8_few_ok(16, 512) == 1 and lib.ffvc_linear_int8_few_ok(17, 512) == 0 and lib.ffvc_linear_int8_few_ok(16, 8192) == 0
     assert lib.ffvc_linear_int8_few(A, 0, 512, A, 512, A, 0, 0, 0, 1, 8, A, 0, 8, 0, 17, 8, 512, None) != 0
