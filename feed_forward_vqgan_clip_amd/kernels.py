@@ -1588,13 +1588,19 @@ def _same_device(*ts):
     return _NOTHING if dev == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
+def _stream_of(t):
+    """The current stream of t's device as an integer (no Stream object: these launchers serve calls of a few microseconds)."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
 def _rows2d(name, t):
     """A 2-d tensor whose rows are contiguous; returns its row stride."""
     if t.dim() != 2:
         raise ValueError(f"{name}: expected a 2-d tensor, got {tuple(t.shape)}")
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    rows, cols = t.shape
+    if cols > 1 and t.stride(1) != 1:
         raise ValueError(f"{name}: the elements of a row must be contiguous (strides {t.stride()})")
-    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], t.stride(0))
+    return t.stride(0) if rows > 1 else max(cols, t.stride(0))
 
 
 def _ids(name, t, n=None):
@@ -1607,8 +1613,9 @@ def _ids(name, t, n=None):
 def embed_fwd(ids, table, scale=1.0, pos=None, pos_ids=None, out_dtype=None):
     """scale * table[ids] (+ pos[pos_ids]; pos_ids None: row t for token t) -> [*ids.shape, dim].  Indices outside their table read zero rows."""
     _ids("embed_fwd", ids)
+    n = ids.numel()
     if pos_ids is not None:
-        _ids("embed_fwd: pos_ids", pos_ids, ids.numel())
+        _ids("embed_fwd: pos_ids", pos_ids, n)
     ld = _rows2d("embed_fwd: table", table)
     V, dim = table.shape
     pld = npos = 0
@@ -1619,11 +1626,11 @@ def embed_fwd(ids, table, scale=1.0, pos=None, pos_ids=None, out_dtype=None):
     code = dtype_code(table.dtype)
     with _same_device(ids, table, pos, pos_ids):
         out = torch.empty(*ids.shape, dim, dtype=out_dtype or table.dtype, device=table.device)
-        if out.numel():
+        if n and dim:
             if V < 1 or (pos is not None and npos < 1):
                 raise ValueError("embed_fwd: empty table")
-            _call("ffvc_embed_fwd", table.data_ptr(), code, ld, V, ids.data_ptr(), float(scale), _ptr(pos), pld, npos, _ptr(pos_ids), out.data_ptr(),
-                  dtype_code(out.dtype), dim, ids.numel(), dim, stream_ptr())
+            _call("ffvc_embed_fwd", table.data_ptr(), code, ld, V, ids.data_ptr(), scale, _ptr(pos), pld, npos, _ptr(pos_ids), out.data_ptr(),
+                  dtype_code(out.dtype), dim, n, dim, _stream_of(table))
     return out
 
 
@@ -1643,8 +1650,8 @@ def embed_bwd(dout, ids, rows, scale=1.0, out_dtype=None):
         grad = torch.empty(rows, dim, dtype=dt, device=dout.device)
         nb = int(_lib.load().ffvc_embed_bwd_ws_bytes(n, rows, dim))
         ws = torch.empty(nb, dtype=torch.uint8, device=dout.device)
-        _call("ffvc_embed_bwd", d2.data_ptr(), dtype_code(d2.dtype), ld, ids.data_ptr(), n, rows, dim, float(scale), grad.data_ptr(), dtype_code(dt),
-              ws.data_ptr(), nb, stream_ptr())
+        _call("ffvc_embed_bwd", d2.data_ptr(), dtype_code(d2.dtype), ld, ids.data_ptr(), n, rows, dim, scale, grad.data_ptr(), dtype_code(dt),
+              ws.data_ptr(), nb, _stream_of(dout))
     return grad
 
 
@@ -1658,17 +1665,21 @@ def _heads3d(name, t, like=None):
     return (t.stride(0) if T > 1 else max(H * D, t.stride(0))), (t.stride(1) if H > 1 else D)
 
 
+def _packed_cu(cu):
+    if cu.dtype != torch.int32 or cu.dim() != 1 or cu.numel() < 2 or not cu.is_contiguous():
+        raise TypeError("attn_packed: cu_seqlens must be a contiguous int32 vector of at least two offsets")
+    return cu.numel() - 1
+
+
 def _attn_packed_desc(q, k, v, cu, scale):
     if q.dtype not in LOWP:
         raise TypeError(f"attn_packed: 16-bit tensors only (bf16, f16), got {q.dtype}")
     for n, t in (("k", k), ("v", v)):
         if t.dtype != q.dtype:
             raise TypeError(f"attn_packed: {n} is {t.dtype}, q is {q.dtype}")
-    if cu.dtype != torch.int32 or cu.dim() != 1 or cu.numel() < 2 or not cu.is_contiguous():
-        raise TypeError("attn_packed: cu_seqlens must be a contiguous int32 vector of at least two offsets")
     T, H, D = q.shape
     d = _lib.AttnPackedDesc()
-    d.rows, d.seqs, d.heads, d.kv_heads, d.head_dim = T, cu.numel() - 1, H, k.shape[1], D
+    d.rows, d.seqs, d.heads, d.kv_heads, d.head_dim = T, _packed_cu(cu), H, k.shape[1], D
     d.dtype, d.scale, d.cu = dtype_code(q.dtype), float(scale), cu.data_ptr()
     d.q, (d.q_rs, d.q_hs) = q.data_ptr(), _heads3d("attn_packed: q", q)
     d.k, (d.k_rs, d.k_hs) = k.data_ptr(), _heads3d("attn_packed: k", k, (T, k.shape[1], D))
@@ -1692,7 +1703,7 @@ def attn_packed_fwd(q, k, v, cu_seqlens, scale, out=None, want_lse=False):
         lse = torch.empty(H, T, dtype=torch.float32, device=q.device) if want_lse else None
         d.lse = _ptr(lse)
         if T:
-            _call("ffvc_attn_packed_fwd", byref(d), stream_ptr())
+            _call("ffvc_attn_packed_fwd", byref(d), _stream_of(q))
     return out, lse
 
 
@@ -1715,7 +1726,50 @@ def attn_packed_bwd(q, k, v, out, dout, lse, cu_seqlens, scale, dq, dk, dv):
         delta = torch.empty_like(lse)
         d.lse, d.delta, d.zero_tail = lse.data_ptr(), delta.data_ptr(), 1
         if T:
-            _call("ffvc_attn_packed_bwd", byref(d), stream_ptr())
+            _call("ffvc_attn_packed_bwd", byref(d), _stream_of(q))
+
+
+def attn_packed_qkv_fwd(qkv, cu_seqlens, heads, kv_heads, scale, want_lse=False):
+    """attn_packed_fwd of a packed projection [rows, (heads + 2 kv_heads) * dh] -> (out [rows, heads * dh], lse or None)."""
+    if qkv.dtype not in LOWP:
+        raise TypeError(f"attn_packed: 16-bit tensors only (bf16, f16), got {qkv.dtype}")
+    ld = _rows2d("attn_packed: qkv", qkv)
+    T, W = qkv.shape
+    D = W // (heads + 2 * kv_heads)
+    seqs = _packed_cu(cu_seqlens)
+    with _same_device(qkv, cu_seqlens):
+        out = torch.empty(T, heads * D, dtype=qkv.dtype, device=qkv.device)
+        lse = torch.empty(heads, T, dtype=torch.float32, device=qkv.device) if want_lse else None
+        if T:
+            p = qkv.data_ptr()
+            pk = p + 2 * heads * D
+            d = _lib.AttnPackedDesc(p, pk, pk + 2 * kv_heads * D, out.data_ptr(), _ptr(lse), cu_seqlens.data_ptr(), 0, 0, 0, 0, 0, T, ld, D, ld, D, ld, D,
+                                    heads * D, D, 0, 0, 0, 0, 0, 0, 0, 0, seqs, heads, kv_heads, D, dtype_code(qkv.dtype), 1, scale)
+            _call("ffvc_attn_packed_fwd", byref(d), _stream_of(qkv))
+    return out, lse
+
+
+def attn_packed_qkv_bwd(qkv, out, dout, lse, cu_seqlens, heads, kv_heads, scale):
+    """The gradient [rows, (heads + 2 kv_heads) * dh] of attn_packed_qkv_fwd's projection; dout contiguous like out."""
+    _req(qkv.dtype, out, dout)
+    _req_f32(lse)
+    ld = _rows2d("attn_packed: qkv", qkv)
+    T, W = qkv.shape
+    D = W // (heads + 2 * kv_heads)
+    if tuple(out.shape) != (T, heads * D) or tuple(dout.shape) != (T, heads * D) or tuple(lse.shape) != (heads, T):
+        raise ValueError("attn_packed_qkv_bwd: shape mismatch")
+    seqs = _packed_cu(cu_seqlens)
+    with _same_device(qkv, out, dout, lse, cu_seqlens):
+        dqkv = torch.empty(T, W, dtype=qkv.dtype, device=qkv.device)
+        delta = torch.empty_like(lse)
+        if T:
+            p, g = qkv.data_ptr(), dqkv.data_ptr()
+            pk, gk, o = p + 2 * heads * D, g + 2 * heads * D, heads * D
+            d = _lib.AttnPackedDesc(p, pk, pk + 2 * kv_heads * D, out.data_ptr(), lse.data_ptr(), cu_seqlens.data_ptr(), dout.data_ptr(), g, gk,
+                                    gk + 2 * kv_heads * D, delta.data_ptr(), T, ld, D, ld, D, ld, D, o, D, o, D, W, D, W, D, W, D, seqs, heads, kv_heads, D,
+                                    dtype_code(qkv.dtype), 1, scale)
+            _call("ffvc_attn_packed_bwd", byref(d), _stream_of(qkv))
+    return dqkv
 
 
 def int8_quant(x):
@@ -1732,7 +1786,7 @@ def int8_quant(x):
         q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
         s = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
         if x2.shape[0]:
-            _call("ffvc_int8_quant", x2.data_ptr(), code, ld, q.data_ptr(), K, s.data_ptr(), x2.shape[0], K, stream_ptr())
+            _call("ffvc_int8_quant", x2.data_ptr(), code, ld, q.data_ptr(), K, s.data_ptr(), x2.shape[0], K, _stream_of(x))
     return q, s
 
 
@@ -1741,9 +1795,10 @@ def linear_int8(x, wq, ws, bias=None, act=ACT_NONE, residual=None, out_dtype=Non
     products are summed exactly in 32-bit integers.  out_dtype: x's (default) or fp32.  want_actgrad: -> (y, act'(pre-activation))."""
     if x.dtype not in LOWP:
         raise TypeError(f"linear_int8: 16-bit activations only (bf16, f16), got {x.dtype}")
-    _req(torch.int8, wq)
-    _req_f32(ws, bias)
     N, K = wq.shape
+    for name, t, dt in (("weight", wq, torch.int8), ("scale", ws, torch.float32), ("bias", bias, torch.float32)):
+        if t is not None and (t.dtype != dt or not t.is_contiguous()):
+            raise TypeError(f"linear_int8: {name} must be a contiguous {dt} tensor, got {t.dtype}")
     if x.dim() < 1 or x.shape[-1] != K:
         raise ValueError(f"linear_int8: x {tuple(x.shape)} against a weight {tuple(wq.shape)}")
     if tuple(ws.shape) != (N,) or (bias is not None and tuple(bias.shape) != (N,)):
@@ -1755,8 +1810,9 @@ def linear_int8(x, wq, ws, bias=None, act=ACT_NONE, residual=None, out_dtype=Non
     if residual is not None:
         if tuple(residual.shape) != shape:
             raise ValueError(f"linear_int8: residual {tuple(residual.shape)} for an output {shape}")
-        _req(residual.dtype if residual.dtype in (x.dtype, torch.float32) else out_dtype, residual)
-    x2 = x.reshape(-1, K)
+        if residual.dtype not in (x.dtype, torch.float32) or not residual.is_contiguous():
+            raise TypeError(f"linear_int8: residual must be contiguous, {x.dtype} or fp32, got {residual.dtype}")
+    x2 = x if x.dim() == 2 else x.reshape(-1, K)
     ld = _rows2d("linear_int8: x", x2)
     M = x2.shape[0]
     with _same_device(x, wq, ws, bias, residual):
@@ -1766,14 +1822,14 @@ def linear_int8(x, wq, ws, bias=None, act=ACT_NONE, residual=None, out_dtype=Non
         g = torch.empty(shape, dtype=x.dtype, device=x.device) if want_actgrad else None
         if M:
             lo, rdt = dtype_code(x.dtype), dtype_code(residual.dtype if residual is not None else out_dtype)
-            lib = _lib.load()
+            lib, st = _lib.load(), _stream_of(x)
             if lib.ffvc_linear_int8_few_ok(M, K):
                 _call("ffvc_linear_int8_few", x2.data_ptr(), lo, ld, wq.data_ptr(), K, ws.data_ptr(), _ptr(bias), act, _ptr(residual), rdt, N,
-                      y.data_ptr(), dtype_code(out_dtype), N, _ptr(g), M, N, K, stream_ptr())
+                      y.data_ptr(), dtype_code(out_dtype), N, _ptr(g), M, N, K, st)
             else:
                 xq = torch.empty((K + 63) // 64, M, 64, dtype=torch.int8, device=x.device)      # K panels
                 xs = torch.empty(M, dtype=torch.float32, device=x.device)
-                _call("ffvc_int8_quant", x2.data_ptr(), lo, ld, xq.data_ptr(), 0, xs.data_ptr(), M, K, stream_ptr())
+                _call("ffvc_int8_quant", x2.data_ptr(), lo, ld, xq.data_ptr(), 0, xs.data_ptr(), M, K, st)
                 _call("ffvc_gemm_int8", xq.data_ptr(), xs.data_ptr(), wq.data_ptr(), K, ws.data_ptr(), _ptr(bias), act, _ptr(residual), rdt, N,
-                      y.data_ptr(), dtype_code(out_dtype), N, _ptr(g), lo, M, N, K, stream_ptr())
+                      y.data_ptr(), dtype_code(out_dtype), N, _ptr(g), lo, M, N, K, st)
     return (y, g) if want_actgrad else y

@@ -1054,20 +1054,15 @@ class _AttentionPackedFn(Function):
 
     @staticmethod
     def forward(ctx, qkv, cu, heads, kv_heads, scale):
-        q, k, v = _split_heads(qkv, heads, kv_heads)
-        o, lse = K.attn_packed_fwd(q, k, v, cu, scale, want_lse=ctx.needs_input_grad[0])
+        o, lse = K.attn_packed_qkv_fwd(qkv, cu, heads, kv_heads, scale, want_lse=True)
         ctx.save_for_backward(qkv, cu, o, lse)
         ctx.cfg = (heads, kv_heads, scale)
-        return o.view(qkv.shape[0], -1)
+        return o
 
     @staticmethod
     def backward(ctx, do):
         qkv, cu, o, lse = ctx.saved_tensors
-        heads, kv_heads, scale = ctx.cfg
-        do = _as(_contig(do), qkv.dtype).view(o.shape)
-        dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
-        K.attn_packed_bwd(*_split_heads(qkv, heads, kv_heads), o, do, lse, cu, scale, *_split_heads(dqkv, heads, kv_heads))
-        return dqkv, None, None, None, None
+        return K.attn_packed_qkv_bwd(qkv, o, _as(_contig(do), qkv.dtype), lse, cu, *ctx.cfg), None, None, None, None
 
 
 def _split_heads(qkv, heads, kv_heads):
@@ -1089,7 +1084,10 @@ def attention_packed(qkv, cu_seqlens, heads, kv_heads=None, scale=None):
     dh = qkv.shape[1] // (heads + 2 * kv_heads)
     if dh % 8 or not 8 <= dh <= 128:
         raise ValueError(f"attention_packed: head width {dh} unsupported (a multiple of 8, at most 128)")
-    return _AttentionPackedFn.apply(qkv, cu_seqlens, heads, kv_heads, default_scale(dh) if scale is None else scale)
+    scale = default_scale(dh) if scale is None else float(scale)
+    if not (qkv.requires_grad and torch.is_grad_enabled()):
+        return K.attn_packed_qkv_fwd(qkv, cu_seqlens, heads, kv_heads, scale)[0]
+    return _AttentionPackedFn.apply(qkv, cu_seqlens, heads, kv_heads, scale)
 
 
 class _EmbeddingFn(Function):
@@ -1117,6 +1115,8 @@ def embedding(ids, table, scale=1.0, pos=None, pos_ids=None, out_dtype=None):
 
     ids (and pos_ids): int64; an index outside its table (e.g. -1 for the unused rows of a buffer) reads a zero row and gets no gradient.
     pos without pos_ids: row t for the t-th token.  The gradients are sums over the sorted tokens: no atomics, the same bits every time."""
+    if not (torch.is_grad_enabled() and (table.requires_grad or (pos is not None and pos.requires_grad))):
+        return K.embed_fwd(ids, table, float(scale), pos, pos_ids, out_dtype)
     return _EmbeddingFn.apply(table, pos, ids, pos_ids, float(scale), out_dtype)
 
 
