@@ -55,9 +55,9 @@ __device__ __forceinline__ void tile_src(int pos, int& row, int& chunk) {   // t
 }
 
 // LDS-DMA of one tile by NW waves: piece i of a wave fills 64 consecutive chunk positions; the lane's source offset inside the tile is fixed
-template <int DP, int NW>
+template <int DP, int NW, int ROWS = KB>
 struct TileDma {
-  static constexpr int NP = KB * DP / 8 / 64 / NW;
+  static constexpr int NP = ROWS * DP / 8 / 64 / NW;
   uint32_t off[NP];
   __device__ __forceinline__ void init(int64_t rs, int D, int wave, int lane) {
 #pragma unroll
@@ -69,7 +69,7 @@ struct TileDma {
   }
   // base: element (row0, feature 0) of the tile; live: rows of the sequence from row0 on (> 0)
   __device__ __forceinline__ void issue(const uint16_t* base, int64_t rs, int D, int64_t live, unsigned char* tile, int wave) {
-    const int64_t bytes = ((live < KB ? live : KB) - 1) * rs * 2 + D * 2;
+    const int64_t bytes = ((live < ROWS ? live : ROWS) - 1) * rs * 2 + D * 2;
     const rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)bytes, 0x00020000);
 #pragma unroll
     for (int i = 0; i < NP; ++i)
@@ -406,11 +406,17 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_dq_kernel(const ffvc_a
 }
 
 // ---- backward: dk, dv --------------------------------------------------------------------------------------------------------------
-// NW waves x 32 keys of one key / value head; walks the query tiles that see them, for every query head of the group.
+// NW waves x 32 keys of one key / value head; walks the query tiles (QB rows of q and dout, two LDS stages) that see them, for every query head
+// of the group.  K stays in registers as the B operand of s = q k^T; V, the B operand of dp = do v^T, stays in LDS: with both in registers next
+// to the two accumulators a wave needs more than half the register file, and one wave per SIMD cannot hide its own waits (963 us against
+// ... at 8192 rows, 16 heads of 128).
+constexpr int QB = 32;
 template <typename L, int DP, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void attn_packed_dkv_kernel(const ffvc_attn_packed_desc p, int64_t slots) {
-  constexpr int BM = 32 * NW, NS = DP / 16, ND = DP / 32, TB = KB * DP * 2;
+  constexpr int BM = 32 * NW, NS = DP / 16, ND = DP / 32, TB = QB * DP * 2, VB = BM * DP * 2;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  unsigned char* vmem = smem + 4 * TB;
+  float* stat = (float*)(vmem + VB);                         // [2 stages][lse | delta][QB]
   const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int64_t slot;
@@ -435,24 +441,31 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_dkv_kernel(const ffvc_
   const uint16_t* V = (const uint16_t*)p.v + pl.row0 * p.v_rs + kvh * p.v_hs;
   const int group = p.heads / p.kv_heads;
   const float c = p.scale * LOG2E;
-  TileDma<DP, NW> dq, dd;
+  TileDma<DP, NW, QB> dq, dd;
   dq.init(p.q_rs, D, wave, lane);
   dd.init(p.do_rs, D, wave, lane);
-  const int qb0 = (int)(k0 / KB);                            // first query tile that sees any of these keys
-  const int nqb = (int)((pl.len + KB - 1) / KB);
+  {
+    TileDma<DP, NW, BM> dv;
+    dv.init(p.v_rs, D, wave, lane);
+    dv.issue(V + k0 * p.v_rs, p.v_rs, D, pl.len - k0, vmem, wave);
+  }
+  const int qb0 = (int)(k0 / QB);                            // first query tile that sees any of these keys
+  const int nqb = (int)((pl.len + QB - 1) / QB);
   const int total = (nqb - qb0) * group;
-  float* stat = (float*)(smem + 4 * TB);                     // [2 stages][lse | delta][KB]
   int head_i = kvh * group, qb_i = qb0;                      // the next tile to fetch
   auto issue = [&](int st_i) {
-    const int64_t r0 = (int64_t)qb_i * KB;
+    const int64_t r0 = (int64_t)qb_i * QB;
     unsigned char* st = smem + st_i * 2 * TB;
     dq.issue((const uint16_t*)p.q + (pl.row0 + r0) * p.q_rs + head_i * p.q_hs, p.q_rs, D, pl.len - r0, st, wave);
     dd.issue((const uint16_t*)p.dout + (pl.row0 + r0) * p.do_rs + head_i * p.do_hs, p.do_rs, D, pl.len - r0, st + TB, wave);
-    if (wave < 2) {                                          // their lse and delta, zeros past the end
-      const float* src = (wave ? p.delta : p.lse) + (int64_t)head_i * p.rows + pl.row0 + r0;
-      const int n = (int)(pl.len - r0 < KB ? pl.len - r0 : KB);
-      const rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)src, 0, n * 4, 0x00020000);
-      dma4(r, lane * 4, stat + (st_i * 2 + wave) * KB);
+    if (wave == 0) {                                         // lanes 0..31 their lse, 32..63 their delta; zeros past the end
+      const int64_t at = (int64_t)head_i * p.rows + pl.row0 + r0;
+      const int n = (int)(pl.len - r0 < QB ? pl.len - r0 : QB);
+      // one descriptor over both arrays would need their distance: two half-masked loads instead
+      const rsrc_t rl = __builtin_amdgcn_make_buffer_rsrc((void*)(p.lse + at), 0, n * 4, 0x00020000);
+      const rsrc_t rd = __builtin_amdgcn_make_buffer_rsrc((void*)(p.delta + at), 0, n * 4, 0x00020000);
+      dma4(rl, lane * 4, stat + st_i * 4 * QB);              // [0, 64): lse and zeros
+      dma4(rd, lane * 4, stat + st_i * 4 * QB + 2 * QB);     // [64, 128): delta and zeros
     }
     if (++qb_i == nqb) {
       qb_i = qb0;
@@ -463,12 +476,9 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_dkv_kernel(const ffvc_
   const int64_t kw = k0 + 32 * wave;
   const int64_t ki = kw + l31;
   const bool ok = ki < pl.len;
-  u32x4_t fk[NS], fv[NS];
+  u32x4_t fk[NS];
 #pragma unroll
-  for (int s = 0; s < NS; ++s) {
-    fk[s] = row_frag(Kp, p.k_rs, ki, ok, s, h, D);
-    fv[s] = row_frag(V, p.v_rs, ki, ok, s, h, D);
-  }
+  for (int s = 0; s < NS; ++s) fk[s] = row_frag(Kp, p.k_rs, ki, ok, s, h, D);
   f32x16_t aK[ND], aV[ND];
 #pragma unroll
   for (int t = 0; t < ND; ++t) {
@@ -480,47 +490,44 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_dkv_kernel(const ffvc_
   for (int it = 0; it < total; ++it) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    const int64_t r0 = (int64_t)qb * KB;
+    const int64_t r0 = (int64_t)qb * QB;
     if (++qb == nqb) qb = qb0;
     if (it + 1 < total) issue((it + 1) & 1);
-    if (r0 + KB - 1 < kw || kw >= pl.len) continue;          // every query of the tile is earlier than this wave's keys
+    if (r0 + QB - 1 < kw || kw >= pl.len) continue;          // every query of the tile is earlier than this wave's keys
     const unsigned char* sq = smem + (it & 1) * 2 * TB;
     const unsigned char* sd = sq + TB;
-    const float* st = stat + (it & 1) * 2 * KB;
+    const float* st = stat + (it & 1) * 4 * QB;
+    f32x16_t S, dP;
+    zero16(S);
+    zero16(dP);
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      mma(S, frag_rows<DP>(sq, l31, s, h), fk[s]);
+      mma(dP, frag_rows<DP>(sd, l31, s, h), frag_rows<DP>(vmem, 32 * wave + l31, s, h));
+    }
     const bool diag = r0 < kw + 31;
+    const int lim = (int)(ki - r0);                           // first query of the tile that sees this lane's key
 #pragma unroll
-    for (int qt = 0; qt < 2; ++qt) {
-      f32x16_t S, dP;
-      zero16(S);
-      zero16(dP);
+    for (int g = 0; g < 4; ++g) {
+      const f32x4_t l4 = *(const f32x4_t*)(st + 8 * g + 4 * h);
+      const f32x4_t d4 = *(const f32x4_t*)(st + 2 * QB + 8 * g + 4 * h);
 #pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        mma(S, frag_rows<DP>(sq, 32 * qt + l31, s, h), fk[s]);
-        mma(dP, frag_rows<DP>(sd, 32 * qt + l31, s, h), fv[s]);
+      for (int j = 0; j < 4; ++j) {
+        const int r = 4 * g + j;
+        const bool see = !diag || 8 * g + 4 * h + j >= lim;
+        const float pr = __builtin_amdgcn_exp2f(fmaf(S[r], c, -l4[j]));
+        const float ds = pr * (dP[r] - d4[j]) * p.scale;
+        S[r] = see ? pr : 0.0f;
+        dP[r] = see ? ds : 0.0f;
       }
-      const int lim = (int)(ki - r0);                         // first query of the tile that sees this lane's key
+    }
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4_t l4 = *(const f32x4_t*)(st + 32 * qt + 8 * g + 4 * h);
-        const f32x4_t d4 = *(const f32x4_t*)(st + KB + 32 * qt + 8 * g + 4 * h);
+    for (int sg = 0; sg < 2; ++sg) {
+      const u32x4_t fp = pack8<L>(S, 8 * sg), fs = pack8<L>(dP, 8 * sg);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int r = 4 * g + j;
-          const bool see = !diag || 32 * qt + 8 * g + 4 * h + j >= lim;
-          const float pr = __builtin_amdgcn_exp2f(fmaf(S[r], c, -l4[j]));
-          const float ds = pr * (dP[r] - d4[j]) * p.scale;
-          S[r] = see ? pr : 0.0f;
-          dP[r] = see ? ds : 0.0f;
-        }
-      }
-#pragma unroll
-      for (int sg = 0; sg < 2; ++sg) {
-        const u32x4_t fp = pack8<L>(S, 8 * sg), fs = pack8<L>(dP, 8 * sg);
-#pragma unroll
-        for (int t = 0; t < ND; ++t) {
-          mma(aV[t], frag_cols<DP>(sd, t, 32 * qt + 16 * sg, lane), fp);
-          mma(aK[t], frag_cols<DP>(sq, t, 32 * qt + 16 * sg, lane), fs);
-        }
+      for (int t = 0; t < ND; ++t) {
+        mma(aV[t], frag_cols<DP>(sd, t, 16 * sg, lane), fp);
+        mma(aK[t], frag_cols<DP>(sq, t, 16 * sg, lane), fs);
       }
     }
   }
@@ -568,7 +575,7 @@ int run_bwd(const ffvc_attn_packed_desc& d, hipStream_t st) {
   constexpr int NW = 4;
   const int64_t slots = d.rows / (32 * NW) + d.seqs + 1;
   LAUNCH_PACKED((attn_packed_dq_kernel<L, DP, NW>), 4 * KB * DP * 2, d.heads, 64 * NW);
-  LAUNCH_PACKED((attn_packed_dkv_kernel<L, DP, NW>), 4 * KB * DP * 2 + 4 * KB * 4, d.kv_heads, 64 * NW);
+  LAUNCH_PACKED((attn_packed_dkv_kernel<L, DP, NW>), (4 * QB + 32 * NW) * DP * 2 + 8 * QB * 4, d.kv_heads, 64 * NW);
   return 0;
 }
 
