@@ -26,9 +26,25 @@ constexpr float LOG2E = 1.44269504088896341f;
 constexpr float NEG_BIG = -3.0e38f;
 constexpr int KB = 64;                      // rows of a staged tile
 
-// 64 lanes x 16 (4) bytes from a bounded buffer into consecutive LDS
-__device__ __forceinline__ void dma16(rsrc_t r, uint32_t off, unsigned char* lds) { __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_vp)lds, 16, off, 0, 0, 0); }
-__device__ __forceinline__ void dma4(rsrc_t r, uint32_t off, float* lds) { __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_vp)lds, 4, off, 0, 0, 0); }
+// 64 lanes x 16 (4) bytes from a bounded buffer into consecutive LDS.  Written out, because the compiler would otherwise wait for every load under way
+// before each transposing LDS read, for it cannot tell that they touch other slots; the kernels below do all their waiting themselves
+// (s_waitcnt counts are in order, so a compiler-made wait for one of its own loads only ever waits for more).  The s_nop covers a descriptor word
+// that a vector instruction has just moved to a scalar register.
+__device__ __forceinline__ void dma16(rsrc_t r, uint32_t off, unsigned char* lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+               :: "v"(off), "s"(r), "s"((uint32_t)(uintptr_t)(lds_vp)lds) : "memory", "m0");
+}
+__device__ __forceinline__ void dma4(rsrc_t r, uint32_t off, float* lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tbuffer_load_dword %0, %1, 0 offen lds"
+               :: "v"(off), "s"(r), "s"((uint32_t)(uintptr_t)(lds_vp)lds) : "memory", "m0");
+}
+// everything but the N youngest loads of this wave has landed and its LDS reads are done, then everyone's; nothing moves across
+template <int N>
+__device__ __forceinline__ void arrive() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 
 // ---- a tile of KB rows x DP features in LDS: rows of DP * 2 bytes in lines of 256, 16-byte chunks XOR-swizzled so that both the 16-byte
 // row reads (16 rows of one chunk column) and the transposing 8-byte reads (4 rows x 32 bytes) spread over all banks
@@ -67,9 +83,9 @@ struct TileDma {
       off[i] = chunk * 8 < D ? (uint32_t)((row * rs + chunk * 8) * 2) : OOB;
     }
   }
-  // base: element (row0, feature 0) of the tile; live: rows of the sequence from row0 on (> 0)
+  // base: element (row0, feature 0) of the tile; live: rows of the sequence from row0 on (none: zeros)
   __device__ __forceinline__ void issue(const uint16_t* base, int64_t rs, int D, int64_t live, unsigned char* tile, int wave) {
-    const int64_t bytes = ((live < ROWS ? live : ROWS) - 1) * rs * 2 + D * 2;
+    const int64_t bytes = live > 0 ? ((live < ROWS ? live : ROWS) - 1) * rs * 2 + D * 2 : 0;
     const rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)bytes, 0x00020000);
 #pragma unroll
     for (int i = 0; i < NP; ++i)
@@ -196,8 +212,8 @@ __device__ __forceinline__ u32x4_t row_frag(const uint16_t* base, int64_t rs, in
 }
 
 // ---- forward -------------------------------------------------------------------------------------------------------------------
-// NW waves x 32 queries; key / value tiles of 64 rows, two LDS stages filled by LDS-DMA while the previous tile is multiplied.
-template <typename L, int DP, int NW>
+// NW waves x 32 queries; key / value tiles of 64 rows in a ring of NST LDS slots, filled by LDS-DMA NST - 1 tiles ahead.
+template <typename L, int DP, int NW, int NST>
 __global__ __launch_bounds__(64 * NW, 2) void attn_packed_fwd_kernel(const ffvc_attn_packed_desc p, int64_t slots) {
   constexpr int BM = 32 * NW, NS = DP / 16, ND = DP / 32, TB = KB * DP * 2;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
@@ -225,13 +241,17 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_fwd_kernel(const ffvc_
   dv.init(p.v_rs, D, wave, lane);
   const int64_t qend = q0 + BM < pl.len ? q0 + BM : pl.len;
   const int nkb = (int)((qend + KB - 1) / KB);
-  auto issue = [&](int kb) {
-    const int64_t k0 = (int64_t)kb * KB;
-    unsigned char* st = smem + (kb & 1) * 2 * TB;
-    dk.issue(Kp + k0 * p.k_rs, p.k_rs, D, pl.len - k0, st, wave);
-    dv.issue(V + k0 * p.v_rs, p.v_rs, D, pl.len - k0, st + TB, wave);
+  constexpr int PIECES = 2 * TileDma<DP, NW>::NP;
+  int slot_in = 0, slot_out = 0;                           // LDS slots filled / read next
+  auto issue = [&](int kb) {                               // (tiles past the last one fetch zeros: the counts stay the same)
+    const int64_t k0 = kb < nkb ? (int64_t)kb * KB : 0, live = kb < nkb ? pl.len - k0 : 0;
+    unsigned char* st = smem + slot_in * 2 * TB;
+    dk.issue(Kp + k0 * p.k_rs, p.k_rs, D, live, st, wave);
+    dv.issue(V + k0 * p.v_rs, p.v_rs, D, live, st + TB, wave);
+    slot_in = slot_in + 1 == NST ? 0 : slot_in + 1;
   };
-  issue(0);
+#pragma unroll
+  for (int i = 0; i < NST - 1; ++i) issue(i);
   const int64_t qw = q0 + 32 * wave;                       // this wave's first query
   const int64_t qi = qw + l31;
   const bool ok = qi < pl.len;
@@ -244,13 +264,13 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_fwd_kernel(const ffvc_
   float m = NEG_BIG, l = 0.0f;
 #pragma unroll 1
   for (int kb = 0; kb < nkb; ++kb) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (kb + 1 < nkb) issue(kb + 1);
+    arrive<(NST - 2) * PIECES>();
+    issue(kb + NST - 1);
+    const unsigned char* sk = smem + slot_out * 2 * TB;
+    const unsigned char* sv = sk + TB;
+    slot_out = slot_out + 1 == NST ? 0 : slot_out + 1;
     const int64_t k0 = (int64_t)kb * KB;
     if (k0 > qw + 31 || qw >= pl.len) continue;            // every key of the tile is later than this wave's queries
-    const unsigned char* sk = smem + (kb & 1) * 2 * TB;
-    const unsigned char* sv = sk + TB;
     f32x16_t S[2];
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
@@ -299,6 +319,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_fwd_kernel(const ffvc_
         for (int t = 0; t < ND; ++t) mma(acc[t], frag_cols<DP>(sv, t, 32 * kt + 16 * sg, lane), fp);
       }
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");         // no load may outlive the workgroup's LDS
   l += other_half(l);
   const float inv = 1.0f / l;
 #pragma unroll
@@ -310,7 +331,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_fwd_kernel(const ffvc_
 }
 
 // ---- backward: dq (and delta) ----------------------------------------------------------------------------------------------------
-template <typename L, int DP, int NW>
+template <typename L, int DP, int NW, int NST>
 __global__ __launch_bounds__(64 * NW, 2) void attn_packed_dq_kernel(const ffvc_attn_packed_desc p, int64_t slots) {
   constexpr int BM = 32 * NW, NS = DP / 16, ND = DP / 32, TB = KB * DP * 2;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
@@ -340,13 +361,17 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_dq_kernel(const ffvc_a
   dv.init(p.v_rs, D, wave, lane);
   const int64_t qend = q0 + BM < pl.len ? q0 + BM : pl.len;
   const int nkb = (int)((qend + KB - 1) / KB);
-  auto issue = [&](int kb) {
-    const int64_t k0 = (int64_t)kb * KB;
-    unsigned char* st = smem + (kb & 1) * 2 * TB;
-    dk.issue(Kp + k0 * p.k_rs, p.k_rs, D, pl.len - k0, st, wave);
-    dv.issue(V + k0 * p.v_rs, p.v_rs, D, pl.len - k0, st + TB, wave);
+  constexpr int PIECES = 2 * TileDma<DP, NW>::NP;
+  int slot_in = 0, slot_out = 0;                           // LDS slots filled / read next
+  auto issue = [&](int kb) {                               // (tiles past the last one fetch zeros: the counts stay the same)
+    const int64_t k0 = kb < nkb ? (int64_t)kb * KB : 0, live = kb < nkb ? pl.len - k0 : 0;
+    unsigned char* st = smem + slot_in * 2 * TB;
+    dk.issue(Kp + k0 * p.k_rs, p.k_rs, D, live, st, wave);
+    dv.issue(V + k0 * p.v_rs, p.v_rs, D, live, st + TB, wave);
+    slot_in = slot_in + 1 == NST ? 0 : slot_in + 1;
   };
-  issue(0);
+#pragma unroll
+  for (int i = 0; i < NST - 1; ++i) issue(i);
   const int64_t qw = q0 + 32 * wave;
   const int64_t qi = qw + l31;
   const bool ok = qi < pl.len;
@@ -363,36 +388,37 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_dq_kernel(const ffvc_a
   }
   dl += other_half(dl);
   const float ls = ok ? p.lse[stat] : 0.0f;
-  if (ok && h == 0) p.delta[stat] = dl;
+  if (ok && h == 0) p.delta[stat] = -dl;                   // (negative: the accumulator of dp starts from it)
   f32x16_t acc[ND];
 #pragma unroll
   for (int t = 0; t < ND; ++t) zero16(acc[t]);
 #pragma unroll 1
   for (int kb = 0; kb < nkb; ++kb) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (kb + 1 < nkb) issue(kb + 1);
+    arrive<(NST - 2) * PIECES>();
+    issue(kb + NST - 1);
+    const unsigned char* sk = smem + slot_out * 2 * TB;
+    const unsigned char* sv = sk + TB;
+    slot_out = slot_out + 1 == NST ? 0 : slot_out + 1;
     const int64_t k0 = (int64_t)kb * KB;
     if (k0 > qw + 31 || qw >= pl.len) continue;
-    const unsigned char* sk = smem + (kb & 1) * 2 * TB;
-    const unsigned char* sv = sk + TB;
     const bool diag = k0 + KB - 1 > qw;
     const int lim = (int)(qi - k0);
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
       f32x16_t S, dP;
       zero16(S);
-      zero16(dP);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dP[r] = -dl;
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
         mma(S, frag_rows<DP>(sk, 32 * kt + l31, s, h), fq[s]);
         mma(dP, frag_rows<DP>(sv, 32 * kt + l31, s, h), fo[s]);
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float pr = __builtin_amdgcn_exp2f(fmaf(S[r], c, -ls));
-        const float ds = pr * (dP[r] - dl) * p.scale;
-        dP[r] = diag && 32 * kt + acc_row(r, h) > lim ? 0.0f : ds;
+      for (int r = 0; r < 16; ++r) dP[r] *= __builtin_amdgcn_exp2f(fmaf(S[r], c, -ls));      // ds / scale
+      if (diag) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dP[r] = 32 * kt + acc_row(r, h) > lim ? 0.0f : dP[r];
       }
 #pragma unroll
       for (int sg = 0; sg < 2; ++sg) {
@@ -402,6 +428,11 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_dq_kernel(const ffvc_a
       }
     }
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+  for (int t = 0; t < ND; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[t][r] *= p.scale;
   store_rows<L, DP>(dQ + qw * p.dq_rs, p.dq_rs, D, acc, l31, ok, h);
 }
 
@@ -410,13 +441,12 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_dq_kernel(const ffvc_a
 // of the group.  K stays in registers as the B operand of s = q k^T; V, the B operand of dp = do v^T, stays in LDS: with both in registers next
 // to the two accumulators a wave needs more than half the register file, and one wave per SIMD cannot hide its own waits (963 us against
 // ... at 8192 rows, 16 heads of 128).
-constexpr int QB = 32;
-template <typename L, int DP, int NW>
+template <typename L, int DP, int NW, int NST, int QB, bool VLDS>
 __global__ __launch_bounds__(64 * NW, 2) void attn_packed_dkv_kernel(const ffvc_attn_packed_desc p, int64_t slots) {
-  constexpr int BM = 32 * NW, NS = DP / 16, ND = DP / 32, TB = QB * DP * 2, VB = BM * DP * 2;
+  constexpr int BM = 32 * NW, NS = DP / 16, ND = DP / 32, TB = QB * DP * 2, VB = VLDS ? BM * DP * 2 : 0;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-  unsigned char* vmem = smem + 4 * TB;
-  float* stat = (float*)(vmem + VB);                         // [2 stages][lse | delta][QB]
+  unsigned char* vmem = smem + NST * 2 * TB;
+  float* stat = (float*)(vmem + VB);                         // [slots][lse | delta][64]
   const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int64_t slot;
@@ -444,7 +474,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_dkv_kernel(const ffvc_
   TileDma<DP, NW, QB> dq, dd;
   dq.init(p.q_rs, D, wave, lane);
   dd.init(p.do_rs, D, wave, lane);
-  {
+  if constexpr (VLDS) {
     TileDma<DP, NW, BM> dv;
     dv.init(p.v_rs, D, wave, lane);
     dv.issue(V + k0 * p.v_rs, p.v_rs, D, pl.len - k0, vmem, wave);
@@ -453,32 +483,35 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_dkv_kernel(const ffvc_
   const int nqb = (int)((pl.len + QB - 1) / QB);
   const int total = (nqb - qb0) * group;
   int head_i = kvh * group, qb_i = qb0;                      // the next tile to fetch
-  auto issue = [&](int st_i) {
-    const int64_t r0 = (int64_t)qb_i * QB;
-    unsigned char* st = smem + st_i * 2 * TB;
-    dq.issue((const uint16_t*)p.q + (pl.row0 + r0) * p.q_rs + head_i * p.q_hs, p.q_rs, D, pl.len - r0, st, wave);
-    dd.issue((const uint16_t*)p.dout + (pl.row0 + r0) * p.do_rs + head_i * p.do_hs, p.do_rs, D, pl.len - r0, st + TB, wave);
-    if (wave == 0) {                                         // lanes 0..31 their lse, 32..63 their delta; zeros past the end
-      const int64_t at = (int64_t)head_i * p.rows + pl.row0 + r0;
-      const int n = (int)(pl.len - r0 < QB ? pl.len - r0 : QB);
-      // one descriptor over both arrays would need their distance: two half-masked loads instead
-      const rsrc_t rl = __builtin_amdgcn_make_buffer_rsrc((void*)(p.lse + at), 0, n * 4, 0x00020000);
-      const rsrc_t rd = __builtin_amdgcn_make_buffer_rsrc((void*)(p.delta + at), 0, n * 4, 0x00020000);
-      dma4(rl, lane * 4, stat + st_i * 4 * QB);              // [0, 64): lse and zeros
-      dma4(rd, lane * 4, stat + st_i * 4 * QB + 2 * QB);     // [64, 128): delta and zeros
-    }
+  constexpr int PIECES = 2 * TileDma<DP, NW, QB>::NP + 1;
+  int slot_in = 0, slot_out = 0;
+  auto issue = [&](int it) {                                 // (steps past the last one fetch zeros: the counts stay the same)
+    const int64_t r0 = (int64_t)qb_i * QB, live = it < total ? pl.len - r0 : 0;
+    const int head = it < total ? head_i : kvh * group;
+    unsigned char* st = smem + slot_in * 2 * TB;
+    dq.issue((const uint16_t*)p.q + (pl.row0 + r0) * p.q_rs + head * p.q_hs, p.q_rs, D, live, st, wave);
+    dd.issue((const uint16_t*)p.dout + (pl.row0 + r0) * p.do_rs + head * p.do_hs, p.do_rs, D, live, st + TB, wave);
+    // even waves their lse, odd ones their delta (the same values to the same place: every wave counts the same loads); zeros past the end
+    const float* src = ((wave & 1) ? p.delta : p.lse) + (int64_t)head * p.rows + pl.row0 + r0;
+    const int n = (int)(live < QB ? live : QB);
+    dma4(__builtin_amdgcn_make_buffer_rsrc((void*)src, 0, n * 4, 0x00020000), lane * 4, stat + (slot_in * 2 + (wave & 1)) * 64);
+    slot_in = slot_in + 1 == NST ? 0 : slot_in + 1;
     if (++qb_i == nqb) {
       qb_i = qb0;
       ++head_i;
     }
   };
-  issue(0);
+#pragma unroll
+  for (int i = 0; i < NST - 1; ++i) issue(i);
   const int64_t kw = k0 + 32 * wave;
   const int64_t ki = kw + l31;
   const bool ok = ki < pl.len;
-  u32x4_t fk[NS];
+  u32x4_t fk[NS], fv[VLDS ? 1 : NS];
 #pragma unroll
-  for (int s = 0; s < NS; ++s) fk[s] = row_frag(Kp, p.k_rs, ki, ok, s, h, D);
+  for (int s = 0; s < NS; ++s) {
+    fk[s] = row_frag(Kp, p.k_rs, ki, ok, s, h, D);
+    if constexpr (!VLDS) fv[s] = row_frag(V, p.v_rs, ki, ok, s, h, D);
+  }
   f32x16_t aK[ND], aV[ND];
 #pragma unroll
   for (int t = 0; t < ND; ++t) {
@@ -488,49 +521,69 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_dkv_kernel(const ffvc_
   int qb = qb0;
 #pragma unroll 1
   for (int it = 0; it < total; ++it) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
+    arrive<(NST - 2) * PIECES>();
+    issue(it + NST - 1);
+    const unsigned char* sq = smem + slot_out * 2 * TB;
+    const unsigned char* sd = sq + TB;
+    const float* st = stat + slot_out * 2 * 64;
+    slot_out = slot_out + 1 == NST ? 0 : slot_out + 1;
     const int64_t r0 = (int64_t)qb * QB;
     if (++qb == nqb) qb = qb0;
-    if (it + 1 < total) issue((it + 1) & 1);
     if (r0 + QB - 1 < kw || kw >= pl.len) continue;          // every query of the tile is earlier than this wave's keys
-    const unsigned char* sq = smem + (it & 1) * 2 * TB;
-    const unsigned char* sd = sq + TB;
-    const float* st = stat + (it & 1) * 4 * QB;
-    f32x16_t S, dP;
-    zero16(S);
-    zero16(dP);
-#pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      mma(S, frag_rows<DP>(sq, l31, s, h), fk[s]);
-      mma(dP, frag_rows<DP>(sd, l31, s, h), frag_rows<DP>(vmem, 32 * wave + l31, s, h));
-    }
     const bool diag = r0 < kw + 31;
     const int lim = (int)(ki - r0);                           // first query of the tile that sees this lane's key
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const f32x4_t l4 = *(const f32x4_t*)(st + 8 * g + 4 * h);
-      const f32x4_t d4 = *(const f32x4_t*)(st + 2 * QB + 8 * g + 4 * h);
+    for (int qt = 0; qt < QB / 32; ++qt) {
+      f32x16_t S, dP;
+      zero16(S);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int r = 4 * g + j;
-        const bool see = !diag || 8 * g + 4 * h + j >= lim;
-        const float pr = __builtin_amdgcn_exp2f(fmaf(S[r], c, -l4[j]));
-        const float ds = pr * (dP[r] - d4[j]) * p.scale;
-        S[r] = see ? pr : 0.0f;
-        dP[r] = see ? ds : 0.0f;
+      for (int g = 0; g < 4; ++g) {                          // dp starts from -delta
+        const f32x4_t d4 = *(const f32x4_t*)(st + 64 + 32 * qt + 8 * g + 4 * h);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) dP[4 * g + j] = d4[j];
       }
-    }
 #pragma unroll
-    for (int sg = 0; sg < 2; ++sg) {
-      const u32x4_t fp = pack8<L>(S, 8 * sg), fs = pack8<L>(dP, 8 * sg);
+      for (int s = 0; s < NS; ++s) {
+        mma(S, frag_rows<DP>(sq, 32 * qt + l31, s, h), fk[s]);
+        if constexpr (VLDS)
+          mma(dP, frag_rows<DP>(sd, 32 * qt + l31, s, h), frag_rows<DP>(vmem, 32 * wave + l31, s, h));
+        else
+          mma(dP, frag_rows<DP>(sd, 32 * qt + l31, s, h), fv[s]);
+      }
 #pragma unroll
-      for (int t = 0; t < ND; ++t) {
-        mma(aV[t], frag_cols<DP>(sd, t, 16 * sg, lane), fp);
-        mma(aK[t], frag_cols<DP>(sq, t, 16 * sg, lane), fs);
+      for (int g = 0; g < 4; ++g) {
+        const f32x4_t l4 = *(const f32x4_t*)(st + 32 * qt + 8 * g + 4 * h);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int r = 4 * g + j;
+          S[r] = __builtin_amdgcn_exp2f(fmaf(S[r], c, -l4[j]));
+          dP[r] *= S[r];                                      // ds / scale
+        }
+      }
+      if (diag) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const bool see = 32 * qt + acc_row(r, h) >= lim;
+          S[r] = see ? S[r] : 0.0f;
+          dP[r] = see ? dP[r] : 0.0f;
+        }
+      }
+#pragma unroll
+      for (int sg = 0; sg < 2; ++sg) {
+        const u32x4_t fp = pack8<L>(S, 8 * sg), fs = pack8<L>(dP, 8 * sg);
+#pragma unroll
+        for (int t = 0; t < ND; ++t) {
+          mma(aV[t], frag_cols<DP>(sd, t, 32 * qt + 16 * sg, lane), fp);
+          mma(aK[t], frag_cols<DP>(sq, t, 32 * qt + 16 * sg, lane), fs);
+        }
       }
     }
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+  for (int t = 0; t < ND; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) aK[t][r] *= p.scale;
   store_rows<L, DP>(dK + kw * p.dk_rs, p.dk_rs, D, aK, l31, ok, h);
   store_rows<L, DP>(dV + kw * p.dv_rs, p.dv_rs, D, aV, l31, ok, h);
 }
@@ -565,17 +618,19 @@ int check_tensor(const void* ptr, int64_t rs, int64_t hs, int D, const char* who
 
 template <typename L, int DP>
 int run_fwd(const ffvc_attn_packed_desc& d, hipStream_t st) {
-  constexpr int NW = 4;
+  constexpr int NW = 4, NST = DP == 64 ? 3 : 2;
   const int64_t slots = d.rows / (32 * NW) + d.seqs + 1;
-  LAUNCH_PACKED((attn_packed_fwd_kernel<L, DP, NW>), 4 * KB * DP * 2, d.heads, 64 * NW);
+  LAUNCH_PACKED((attn_packed_fwd_kernel<L, DP, NW, NST>), NST * 2 * KB * DP * 2, d.heads, 64 * NW);
   return 0;
 }
 template <typename L, int DP>
 int run_bwd(const ffvc_attn_packed_desc& d, hipStream_t st) {
-  constexpr int NW = 4;
+  constexpr int NW = 4, NST = DP == 64 ? 3 : 2;
+  constexpr int QB = DP == 64 ? 64 : 32;
+  constexpr bool VLDS = DP == 128;
   const int64_t slots = d.rows / (32 * NW) + d.seqs + 1;
-  LAUNCH_PACKED((attn_packed_dq_kernel<L, DP, NW>), 4 * KB * DP * 2, d.heads, 64 * NW);
-  LAUNCH_PACKED((attn_packed_dkv_kernel<L, DP, NW>), (4 * QB + 32 * NW) * DP * 2 + 8 * QB * 4, d.kv_heads, 64 * NW);
+  LAUNCH_PACKED((attn_packed_dq_kernel<L, DP, NW, NST>), NST * 2 * KB * DP * 2, d.heads, 64 * NW);
+  LAUNCH_PACKED((attn_packed_dkv_kernel<L, DP, NW, NST, QB, VLDS>), (NST * 2 * QB + (VLDS ? 32 * NW : 0)) * DP * 2 + NST * 2 * 64 * 4, d.kv_heads, 64 * NW);
   return 0;
 }
 

@@ -329,13 +329,13 @@ __global__ __launch_bounds__(256, 2) void gemm_int8_kernel(const I8Args p, int t
       const unsigned char* sw = wmem + ((kt >> 1) & 1) * WS;
       // my pieces of this step have landed (x of the next may be under way), then everyone's; and nobody reads the slots filled next
       // (the bare barrier: __syncthreads would wait for the pieces under way as well)
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(XP) : "memory");
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(XP) : "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
       dx.issue(smem + nxt * XS, kt + 2, nk, wave);
       dw.issue(wmem + (((kt >> 1) & 1) ^ 1) * WS, (kt + 2) * BK, p.K, wave);
       step(kt, sw, 0);
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(XP + WP) : "memory");
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(XP + WP) : "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
       dx.issue(smem + nxt * XS, kt + 3, nk, wave);
