@@ -12,6 +12,8 @@
 // nothing to do.  The rows behind the last sequence are a pseudo-sequence of their own (zero-filled on request, otherwise left alone).
 // Offsets into a tensor are 64 bits wide; inside a tile the buffer descriptor's 32-bit offsets are enough, its record count ends with the
 // sequence, so rows past the end (and features past head_dim) read as zeros without a branch.
+#include <type_traits>
+
 #include "common.h"
 
 namespace {
@@ -24,20 +26,9 @@ typedef __attribute__((address_space(3))) s16x4_t* lds_tr;
 constexpr uint32_t OOB = 0xFFFFFFF0u;
 constexpr float LOG2E = 1.44269504088896341f;
 constexpr float NEG_BIG = -3.0e38f;
-constexpr int KB = 64;                      // rows of a staged tile
-
-// 64 lanes x 16 (4) bytes from a bounded buffer into consecutive LDS.  Written out, because the compiler would otherwise wait for every load under way
-// before each transposing LDS read, for it cannot tell that they touch other slots; the kernels below do all their waiting themselves
-// (s_waitcnt counts are in order, so a compiler-made wait for one of its own loads only ever waits for more).  The s_nop covers a descriptor word
-// that a vector instruction has just moved to a scalar register.
-__device__ __forceinline__ void dma16(rsrc_t r, uint32_t off, unsigned char* lds) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
-               :: "v"(off), "s"(r), "s"((uint32_t)(uintptr_t)(lds_vp)lds) : "memory", "m0");
-}
-__device__ __forceinline__ void dma4(rsrc_t r, uint32_t off, float* lds) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tbuffer_load_dword %0, %1, 0 offen lds"
-               :: "v"(off), "s"(r), "s"((uint32_t)(uintptr_t)(lds_vp)lds) : "memory", "m0");
-}
+// 64 lanes x 16 (4) bytes from a bounded buffer into consecutive LDS
+__device__ __forceinline__ void dma16(rsrc_t r, uint32_t off, unsigned char* lds) { __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_vp)lds, 16, off, 0, 0, 0); }
+__device__ __forceinline__ void dma4(rsrc_t r, uint32_t off, float* lds) { __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_vp)lds, 4, off, 0, 0, 0); }
 // everything but the N youngest loads of this wave has landed and its LDS reads are done, then everyone's; nothing moves across
 template <int N>
 __device__ __forceinline__ void arrive() {
@@ -46,7 +37,7 @@ __device__ __forceinline__ void arrive() {
   asm volatile("" ::: "memory");
 }
 
-// ---- a tile of KB rows x DP features in LDS: rows of DP * 2 bytes in lines of 256, 16-byte chunks XOR-swizzled so that both the 16-byte
+// ---- a tile of rows x DP features in LDS: rows of DP * 2 bytes in lines of 256, 16-byte chunks XOR-swizzled so that both the 16-byte
 // row reads (16 rows of one chunk column) and the transposing 8-byte reads (4 rows x 32 bytes) spread over all banks
 template <int DP>
 __device__ __forceinline__ int tile_off(int row, int chunk) {       // byte offset of 16-byte chunk `chunk` of row `row`
@@ -71,7 +62,7 @@ __device__ __forceinline__ void tile_src(int pos, int& row, int& chunk) {   // t
 }
 
 // LDS-DMA of one tile by NW waves: piece i of a wave fills 64 consecutive chunk positions; the lane's source offset inside the tile is fixed
-template <int DP, int NW, int ROWS = KB>
+template <int DP, int NW, int ROWS>
 struct TileDma {
   static constexpr int NP = ROWS * DP / 8 / 64 / NW;
   uint32_t off[NP];
@@ -212,8 +203,9 @@ __device__ __forceinline__ u32x4_t row_frag(const uint16_t* base, int64_t rs, in
 }
 
 // ---- forward -------------------------------------------------------------------------------------------------------------------
-// NW waves x 32 queries; key / value tiles of 64 rows in a ring of NST LDS slots, filled by LDS-DMA NST - 1 tiles ahead.
-template <typename L, int DP, int NW, int NST>
+// NW waves x 32 queries; key / value tiles of KB = 64 rows in a ring of NST LDS slots, filled by LDS-DMA NST - 1 tiles ahead.  Every variant takes a
+// row's keys 64 at a time in the same steps, so a sequence's output does not depend on what it is packed with.
+template <typename L, int DP, int NW, int NST, int KB>
 __global__ __launch_bounds__(64 * NW, 2) void attn_packed_fwd_kernel(const ffvc_attn_packed_desc p, int64_t slots) {
   constexpr int BM = 32 * NW, NS = DP / 16, ND = DP / 32, TB = KB * DP * 2;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
@@ -236,12 +228,12 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_fwd_kernel(const ffvc_
   const uint16_t* Kp = (const uint16_t*)p.k + pl.row0 * p.k_rs + kvh * p.k_hs;
   const uint16_t* V = (const uint16_t*)p.v + pl.row0 * p.v_rs + kvh * p.v_hs;
   const float c = p.scale * LOG2E;
-  TileDma<DP, NW> dk, dv;
+  TileDma<DP, NW, KB> dk, dv;
   dk.init(p.k_rs, D, wave, lane);
   dv.init(p.v_rs, D, wave, lane);
   const int64_t qend = q0 + BM < pl.len ? q0 + BM : pl.len;
   const int nkb = (int)((qend + KB - 1) / KB);
-  constexpr int PIECES = 2 * TileDma<DP, NW>::NP;
+  constexpr int PIECES = 2 * TileDma<DP, NW, KB>::NP;
   int slot_in = 0, slot_out = 0;                           // LDS slots filled / read next
   auto issue = [&](int kb) {                               // (tiles past the last one fetch zeros: the counts stay the same)
     const int64_t k0 = kb < nkb ? (int64_t)kb * KB : 0, live = kb < nkb ? pl.len - k0 : 0;
@@ -251,7 +243,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_fwd_kernel(const ffvc_
     slot_in = slot_in + 1 == NST ? 0 : slot_in + 1;
   };
 #pragma unroll
-  for (int i = 0; i < NST - 1; ++i) issue(i);
+  for (int i = 0; i < (NST > 1 ? NST - 1 : 1); ++i) issue(i);
   const int64_t qw = q0 + 32 * wave;                       // this wave's first query
   const int64_t qi = qw + l31;
   const bool ok = qi < pl.len;
@@ -262,32 +254,27 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_fwd_kernel(const ffvc_
 #pragma unroll
   for (int t = 0; t < ND; ++t) zero16(acc[t]);
   float m = NEG_BIG, l = 0.0f;
-#pragma unroll 1
-  for (int kb = 0; kb < nkb; ++kb) {
-    arrive<(NST - 2) * PIECES>();
-    issue(kb + NST - 1);
-    const unsigned char* sk = smem + slot_out * 2 * TB;
-    const unsigned char* sv = sk + TB;
-    slot_out = slot_out + 1 == NST ? 0 : slot_out + 1;
-    const int64_t k0 = (int64_t)kb * KB;
-    if (k0 > qw + 31 || qw >= pl.len) continue;            // every key of the tile is later than this wave's queries
-    f32x16_t S[2];
+  // NH: 32-key halves of the tile that any query of the wave sees (the second one is all later keys where the wave starts on the tile's first row:
+  // leaving it out gives the same bits)
+  auto tile = [&](auto halves, const unsigned char* sk, const unsigned char* sv, int64_t k0) {
+    constexpr int NH = decltype(halves)::value;
+    f32x16_t S[NH];
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
+    for (int kt = 0; kt < NH; ++kt) {
       zero16(S[kt]);
 #pragma unroll
       for (int s = 0; s < NS; ++s) mma(S[kt], frag_rows<DP>(sk, 32 * kt + l31, s, h), fq[s]);
     }
-    if (k0 + KB - 1 > qw) {                                // the diagonal crosses this tile
+    if (k0 + 32 * NH - 1 > qw) {                           // the diagonal crosses this tile
       const int lim = (int)(qi - k0);                      // last visible key of this lane's query
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
+      for (int kt = 0; kt < NH; ++kt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) S[kt][r] = 32 * kt + acc_row(r, h) <= lim ? S[kt][r] : -INFINITY;
     }
     float mx = m;
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
+    for (int kt = 0; kt < NH; ++kt)
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, S[kt][r]);
     mx = fmaxf(mx, other_half(mx));
@@ -303,7 +290,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_fwd_kernel(const ffvc_
     const float mc = m * c;
     float sum = 0.0f;
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
+    for (int kt = 0; kt < NH; ++kt)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         S[kt][r] = __builtin_amdgcn_exp2f(fmaf(S[kt][r], c, -mc));
@@ -311,13 +298,33 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_fwd_kernel(const ffvc_
       }
     l += sum;
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
+    for (int kt = 0; kt < NH; ++kt)
 #pragma unroll
       for (int sg = 0; sg < 2; ++sg) {
         const u32x4_t fp = pack8<L>(S[kt], 8 * sg);
 #pragma unroll
         for (int t = 0; t < ND; ++t) mma(acc[t], frag_cols<DP>(sv, t, 32 * kt + 16 * sg, lane), fp);
       }
+  };
+#pragma unroll 1
+  for (int kb = 0; kb < nkb; ++kb) {
+    arrive<(NST > 2 ? NST - 2 : 0) * PIECES>();
+    if constexpr (NST > 1) issue(kb + NST - 1);
+    const unsigned char* sk = smem + slot_out * 2 * TB;
+    const unsigned char* sv = sk + TB;
+    slot_out = slot_out + 1 == NST ? 0 : slot_out + 1;
+    const int64_t k0 = (int64_t)kb * KB;
+    if (k0 <= qw + 31 && qw < pl.len) {                    // (otherwise every key of the tile is later than this wave's queries)
+      // (one wave at 64 features: elsewhere the second body costs the long rows more, 4.6 against 4.1 ms, than it saves)
+      if (NW > 1 || DP > 64 || k0 + 32 <= qw + 31)
+        tile(std::integral_constant<int, 2>{}, sk, sv, k0);
+      else
+        tile(std::integral_constant<int, 1>{}, sk, sv, k0);
+    }
+    if constexpr (NST == 1) {
+      arrive<0>();
+      if (kb + 1 < nkb) issue(kb + 1);
+    }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");         // no load may outlive the workgroup's LDS
   l += other_half(l);
@@ -331,7 +338,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_fwd_kernel(const ffvc_
 }
 
 // ---- backward: dq (and delta) ----------------------------------------------------------------------------------------------------
-template <typename L, int DP, int NW, int NST>
+template <typename L, int DP, int NW, int NST, int KB>
 __global__ __launch_bounds__(64 * NW, 2) void attn_packed_dq_kernel(const ffvc_attn_packed_desc p, int64_t slots) {
   constexpr int BM = 32 * NW, NS = DP / 16, ND = DP / 32, TB = KB * DP * 2;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
@@ -356,12 +363,12 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_dq_kernel(const ffvc_a
   const uint16_t* Oh = (const uint16_t*)p.out + pl.row0 * p.o_rs + head * p.o_hs;
   const uint16_t* dO = (const uint16_t*)p.dout + pl.row0 * p.do_rs + head * p.do_hs;
   const float c = p.scale * LOG2E;
-  TileDma<DP, NW> dk, dv;
+  TileDma<DP, NW, KB> dk, dv;
   dk.init(p.k_rs, D, wave, lane);
   dv.init(p.v_rs, D, wave, lane);
   const int64_t qend = q0 + BM < pl.len ? q0 + BM : pl.len;
   const int nkb = (int)((qend + KB - 1) / KB);
-  constexpr int PIECES = 2 * TileDma<DP, NW>::NP;
+  constexpr int PIECES = 2 * TileDma<DP, NW, KB>::NP;
   int slot_in = 0, slot_out = 0;                           // LDS slots filled / read next
   auto issue = [&](int kb) {                               // (tiles past the last one fetch zeros: the counts stay the same)
     const int64_t k0 = kb < nkb ? (int64_t)kb * KB : 0, live = kb < nkb ? pl.len - k0 : 0;
@@ -404,7 +411,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_dq_kernel(const ffvc_a
     const bool diag = k0 + KB - 1 > qw;
     const int lim = (int)(qi - k0);
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
+    for (int kt = 0; kt < KB / 32; ++kt) {
+      if (kt && k0 + 32 * kt > qw + 31) break;              // a half of later keys only
       f32x16_t S, dP;
       zero16(S);
 #pragma unroll
@@ -441,14 +449,18 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_dq_kernel(const ffvc_a
 // of the group.  K stays in registers as the B operand of s = q k^T; V, the B operand of dp = do v^T, stays in LDS: with both in registers next
 // to the two accumulators a wave needs more than half the register file, and one wave per SIMD cannot hide its own waits (963 us against
 // ... at 8192 rows, 16 heads of 128).
-template <typename L, int DP, int NW, int NST, int QB, bool VLDS>
-__global__ __launch_bounds__(64 * NW, 2) void attn_packed_dkv_kernel(const ffvc_attn_packed_desc p, int64_t slots) {
+//
+// SPLIT = 2: eight waves, the second four take every other (head, query tile) of the same keys and their sums join in LDS at the end.  A key tile's
+// walk is as long as its sequence times the group, so with few tiles the longest one alone decides (see run_bwd).
+template <typename L, int DP, int NW, int NST, int QB, bool VLDS, int SPLIT>
+__global__ __launch_bounds__(64 * NW * SPLIT, 2) void attn_packed_dkv_kernel(const ffvc_attn_packed_desc p, int64_t slots) {
   constexpr int BM = 32 * NW, NS = DP / 16, ND = DP / 32, TB = QB * DP * 2, VB = VLDS ? BM * DP * 2 : 0;
-  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-  unsigned char* vmem = smem + NST * 2 * TB;
-  float* stat = (float*)(vmem + VB);                         // [slots][lse | delta][64]
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem_all[];
   const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave_all = __builtin_amdgcn_readfirstlane(tid >> 6), wave = wave_all % NW, part = wave_all / NW;
+  unsigned char* smem = smem_all + part * (NST * 2 * TB);
+  unsigned char* vmem = smem_all + SPLIT * (NST * 2 * TB);
+  float* stat = (float*)(vmem + VB) + part * (NST * 2 * 64); // [slots][lse | delta][64]
   int64_t slot;
   int kvh;
   block_place(slots, p.kv_heads, slot, kvh);
@@ -462,8 +474,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_dkv_kernel(const ffvc_
   if (pl.tail) {
     if (p.zero_tail) {
       const int64_t n = pl.len - k0 < BM ? pl.len - k0 : BM;
-      zero_rows(dK + k0 * p.dk_rs, p.dk_rs, D, n, tid, 64 * NW);
-      zero_rows(dV + k0 * p.dv_rs, p.dv_rs, D, n, tid, 64 * NW);
+      zero_rows(dK + k0 * p.dk_rs, p.dk_rs, D, n, tid, 64 * NW * SPLIT);
+      zero_rows(dV + k0 * p.dv_rs, p.dv_rs, D, n, tid, 64 * NW * SPLIT);
     }
     return;
   }
@@ -475,31 +487,47 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_dkv_kernel(const ffvc_
   dq.init(p.q_rs, D, wave, lane);
   dd.init(p.do_rs, D, wave, lane);
   if constexpr (VLDS) {
-    TileDma<DP, NW, BM> dv;
-    dv.init(p.v_rs, D, wave, lane);
-    dv.issue(V + k0 * p.v_rs, p.v_rs, D, pl.len - k0, vmem, wave);
+    TileDma<DP, NW * SPLIT, BM> dv;
+    dv.init(p.v_rs, D, wave_all, lane);
+    dv.issue(V + k0 * p.v_rs, p.v_rs, D, pl.len - k0, vmem, wave_all);
   }
   const int qb0 = (int)(k0 / QB);                            // first query tile that sees any of these keys
   const int nqb = (int)((pl.len + QB - 1) / QB);
   const int total = (nqb - qb0) * group;
+  const int steps = (total + SPLIT - 1) / SPLIT;             // (the last step of the second half may be past the end: zeros)
+  auto advance = [&](int& head, int& qb, int by) {
+    qb += by;
+    while (qb >= nqb) {
+      qb -= nqb - qb0;
+      ++head;
+    }
+  };
   int head_i = kvh * group, qb_i = qb0;                      // the next tile to fetch
-  constexpr int PIECES = 2 * TileDma<DP, NW, QB>::NP + 1;
+  if (part) advance(head_i, qb_i, part);
+  int head_o = head_i, qb_o = qb_i;                          // the next tile to multiply
+  constexpr int PIECES = 2 * TileDma<DP, NW, QB>::NP + (NW == 1 ? 2 : 1);
   int slot_in = 0, slot_out = 0;
   auto issue = [&](int it) {                                 // (steps past the last one fetch zeros: the counts stay the same)
-    const int64_t r0 = (int64_t)qb_i * QB, live = it < total ? pl.len - r0 : 0;
-    const int head = it < total ? head_i : kvh * group;
+    const bool in = it * SPLIT + part < total;
+    const int64_t r0 = in ? (int64_t)qb_i * QB : 0, live = in ? pl.len - r0 : 0;
+    const int head = in ? head_i : kvh * group;
     unsigned char* st = smem + slot_in * 2 * TB;
     dq.issue((const uint16_t*)p.q + (pl.row0 + r0) * p.q_rs + head * p.q_hs, p.q_rs, D, live, st, wave);
     dd.issue((const uint16_t*)p.dout + (pl.row0 + r0) * p.do_rs + head * p.do_hs, p.do_rs, D, live, st + TB, wave);
     // even waves their lse, odd ones their delta (the same values to the same place: every wave counts the same loads); zeros past the end
-    const float* src = ((wave & 1) ? p.delta : p.lse) + (int64_t)head * p.rows + pl.row0 + r0;
+    const int64_t at = (int64_t)head * p.rows + pl.row0 + r0;
     const int n = (int)(live < QB ? live : QB);
-    dma4(__builtin_amdgcn_make_buffer_rsrc((void*)src, 0, n * 4, 0x00020000), lane * 4, stat + (slot_in * 2 + (wave & 1)) * 64);
-    slot_in = slot_in + 1 == NST ? 0 : slot_in + 1;
-    if (++qb_i == nqb) {
-      qb_i = qb0;
-      ++head_i;
+    auto fetch = [&](int which) {
+      dma4(__builtin_amdgcn_make_buffer_rsrc((void*)((which ? p.delta : p.lse) + at), 0, n * 4, 0x00020000), lane * 4, stat + (slot_in * 2 + which) * 64);
+    };
+    if constexpr (NW == 1) {
+      fetch(0);
+      fetch(1);
+    } else {
+      fetch(wave & 1);
     }
+    slot_in = slot_in + 1 == NST ? 0 : slot_in + 1;
+    advance(head_i, qb_i, SPLIT);
   };
 #pragma unroll
   for (int i = 0; i < NST - 1; ++i) issue(i);
@@ -518,22 +546,23 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_dkv_kernel(const ffvc_
     zero16(aK[t]);
     zero16(aV[t]);
   }
-  int qb = qb0;
 #pragma unroll 1
-  for (int it = 0; it < total; ++it) {
+  for (int it = 0; it < steps; ++it) {
     arrive<(NST - 2) * PIECES>();
     issue(it + NST - 1);
     const unsigned char* sq = smem + slot_out * 2 * TB;
     const unsigned char* sd = sq + TB;
     const float* st = stat + slot_out * 2 * 64;
     slot_out = slot_out + 1 == NST ? 0 : slot_out + 1;
-    const int64_t r0 = (int64_t)qb * QB;
-    if (++qb == nqb) qb = qb0;
+    const int64_t r0 = (int64_t)qb_o * QB;
+    advance(head_o, qb_o, SPLIT);
+    if (SPLIT > 1 && it * SPLIT + part >= total) continue;
     if (r0 + QB - 1 < kw || kw >= pl.len) continue;          // every query of the tile is earlier than this wave's keys
     const bool diag = r0 < kw + 31;
     const int lim = (int)(ki - r0);                           // first query of the tile that sees this lane's key
 #pragma unroll
     for (int qt = 0; qt < QB / 32; ++qt) {
+      if (r0 + 32 * qt + 31 < kw) continue;                  // a half of earlier queries only
       f32x16_t S, dP;
       zero16(S);
 #pragma unroll
@@ -580,6 +609,26 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_dkv_kernel(const ffvc_
     }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  if constexpr (SPLIT > 1) {
+    float* join = (float*)smem_all + wave * (ND * 16 * 64) + lane;      // [wave][register][lane] over the stages nobody reads any more
+    auto add = [&](f32x16_t (&acc)[ND]) {
+      __syncthreads();
+      if (part)
+#pragma unroll
+        for (int t = 0; t < ND; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) join[(t * 16 + r) * 64] = acc[t][r];
+      __syncthreads();
+      if (!part)
+#pragma unroll
+        for (int t = 0; t < ND; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[t][r] += join[(t * 16 + r) * 64];
+    };
+    add(aK);
+    add(aV);
+    if (part) return;
+  }
 #pragma unroll
   for (int t = 0; t < ND; ++t)
 #pragma unroll
@@ -616,21 +665,44 @@ int check_tensor(const void* ptr, int64_t rs, int64_t hs, int D, const char* who
     FFVC_LAUNCH_CHECK();                                                                                                                        \
   } while (0)
 
+// Short sequences (64 rows or fewer on average): one wave per workgroup, so that a prompt does not pay for rows it has not.
+inline bool short_rows(const ffvc_attn_packed_desc& d) { return d.rows <= 64 * (int64_t)d.seqs; }
+
 template <typename L, int DP>
 int run_fwd(const ffvc_attn_packed_desc& d, hipStream_t st) {
-  constexpr int NW = 4, NST = DP == 64 ? 3 : 2;
-  const int64_t slots = d.rows / (32 * NW) + d.seqs + 1;
-  LAUNCH_PACKED((attn_packed_fwd_kernel<L, DP, NW, NST>), NST * 2 * KB * DP * 2, d.heads, 64 * NW);
+  if (short_rows(d)) {
+    const int64_t slots = d.rows / 32 + d.seqs + 1;
+    LAUNCH_PACKED((attn_packed_fwd_kernel<L, DP, 1, 1, 64>), 2 * 64 * DP * 2, d.heads, 64);
+  } else {
+    constexpr int NW = 4, NST = 2, KB = 64;
+    const int64_t slots = d.rows / (32 * NW) + d.seqs + 1;
+    LAUNCH_PACKED((attn_packed_fwd_kernel<L, DP, NW, NST, KB>), NST * 2 * KB * DP * 2, d.heads, 64 * NW);
+  }
   return 0;
+}
+
+// bytes of LDS of the dk / dv kernel
+constexpr int dkv_lds(int DP, int NW, int NST, int QB, bool VLDS, int SPLIT) {
+  return SPLIT * NST * (2 * QB * DP * 2 + 2 * 64 * 4) + (VLDS ? 32 * NW * DP * 2 : 0);
 }
 template <typename L, int DP>
 int run_bwd(const ffvc_attn_packed_desc& d, hipStream_t st) {
-  constexpr int NW = 4, NST = DP == 64 ? 3 : 2;
-  constexpr int QB = DP == 64 ? 64 : 32;
   constexpr bool VLDS = DP == 128;
-  const int64_t slots = d.rows / (32 * NW) + d.seqs + 1;
-  LAUNCH_PACKED((attn_packed_dq_kernel<L, DP, NW, NST>), NST * 2 * KB * DP * 2, d.heads, 64 * NW);
-  LAUNCH_PACKED((attn_packed_dkv_kernel<L, DP, NW, NST, QB, VLDS>), (NST * 2 * QB + (VLDS ? 32 * NW : 0)) * DP * 2 + NST * 2 * 64 * 4, d.kv_heads, 64 * NW);
+  if (short_rows(d)) {
+    const int64_t slots = d.rows / 32 + d.seqs + 1;
+    LAUNCH_PACKED((attn_packed_dq_kernel<L, DP, 1, 2, 32>), 2 * 2 * 32 * DP * 2, d.heads, 64);
+    LAUNCH_PACKED((attn_packed_dkv_kernel<L, DP, 1, 2, 32, VLDS, 1>), dkv_lds(DP, 1, 2, 32, VLDS, 1), d.kv_heads, 64);
+  } else {
+    constexpr int NW = 4, NST = 2, KB = 64, QB = DP == 64 ? 64 : 32;
+    const int64_t slots = d.rows / (32 * NW) + d.seqs + 1;
+    LAUNCH_PACKED((attn_packed_dq_kernel<L, DP, NW, NST, KB>), NST * 2 * KB * DP * 2, d.heads, 64 * NW);
+    // Two halves per key tile while the tiles do not fill the chip's 512 places one and a half times: 208 -> 143 us on 24 ragged sequences of up to
+    // 2100 rows with 4 key heads (520 tiles), but 594 -> 655 us on one of 8192 rows with 16 (1056 tiles).
+    if (slots * d.kv_heads < 768)
+      LAUNCH_PACKED((attn_packed_dkv_kernel<L, DP, NW, NST, QB, VLDS, 2>), dkv_lds(DP, NW, NST, QB, VLDS, 2), d.kv_heads, 128 * NW);
+    else
+      LAUNCH_PACKED((attn_packed_dkv_kernel<L, DP, NW, NST, QB, VLDS, 1>), dkv_lds(DP, NW, NST, QB, VLDS, 1), d.kv_heads, 64 * NW);
+  }
   return 0;
 }
 
