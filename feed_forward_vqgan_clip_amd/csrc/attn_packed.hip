@@ -202,6 +202,87 @@ __device__ __forceinline__ u32x4_t row_frag(const uint16_t* base, int64_t rs, in
   return ok && d < D ? *(const u32x4_t*)(base + row * rs + d) : z;
 }
 
+// whether the lane's accumulators hold an inf or a NaN
+template <int ND>
+__device__ __forceinline__ bool nonfinite(const f32x16_t (&acc)[ND]) {
+  float z = 0.0f;
+#pragma unroll
+  for (int t = 0; t < ND; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) z = fmaf(acc[t][r], 0.0f, z);        // 0 * inf = NaN
+  return !(z == 0.0f);
+}
+
+// ---- rows next to a non-finite value ---------------------------------------------------------------------------------------------------
+// On the diagonal a tile multiplies masked weights of 0 with rows that their queries (keys) must not see; where such a row holds an inf or a NaN
+// the product is NaN.  A wave whose result is not finite therefore looks at those rows, and only if one of them is not finite either does it
+// sum its rows again without them: a lane per partner for the weights, a lane per feature for the sums.  (Values the row does see, the
+// common way to a NaN, leave the check after at most 95 rows read.)
+
+// any non-finite value in rows r0 .. r1 - 1 (at most 95) of one head
+template <typename L>
+__device__ __forceinline__ bool any_nonfinite(const uint16_t* base, int64_t rs, int D, int64_t r0, int64_t r1, int lane) {
+  bool bad = false;
+  for (int64_t r = r0; r < r1; ++r)
+    for (int d = lane; d < D; d += 64) {
+      const float v = lo_unpack<L>(base[r * rs + d]);
+      bad |= !(fabsf(v) <= 3.4028235e38f);
+    }
+  return __any(bad);
+}
+template <typename L>
+__device__ __forceinline__ float dot_rows(const uint16_t* a, const uint16_t* b, int D) {
+  float s = 0.0f;
+  for (int d = 0; d < D; d += 8) {
+    const f32x8 x = unpack8<L>(*(const u32x4_t*)(a + d)), y = unpack8<L>(*(const u32x4_t*)(b + d));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s = fmaf(x.v[e], y.v[e], s);
+  }
+  return s;
+}
+// o[e] += sum over the 64 lanes' weights of w * row[lane + 64 e]; lane j's row is base + (j0 + j) * rs, n of them
+template <typename L>
+__device__ __forceinline__ void add_weighted(float (&o)[2], float w, const uint16_t* base, int64_t rs, int D, int n, int lane) {
+  for (int j = 0; j < n; ++j) {
+    const float wj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), j));
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (lane + 64 * e < D) o[e] = fmaf(wj, lo_unpack<L>(base[j * rs + lane + 64 * e]), o[e]);
+  }
+}
+// nothing left to learn about a row: a NaN stays one (a tensor full of them costs a wave one chunk per row)
+__device__ __forceinline__ bool all_nan(const float (&o)[2], int D, int lane) {
+  return __all((lane >= D || o[0] != o[0]) && (lane + 64 >= D || o[1] != o[1]));
+}
+template <typename L>
+__device__ __forceinline__ void put_row(uint16_t* row, const float (&o)[2], float mul, int D, int lane) {
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    if (lane + 64 * e < D) row[lane + 64 * e] = (uint16_t)(lo_pack2<L>(o[e] * mul, 0.0f) & 0xffffu);
+}
+
+// outputs of queries i0 .. i1 - 1 from their own keys alone
+template <typename L>
+__device__ __forceinline__ void redo_out(const uint16_t* Q, int64_t q_rs, const uint16_t* K, int64_t k_rs, const uint16_t* V, int64_t v_rs, uint16_t* O,
+                                         int64_t o_rs, int D, float c, int64_t i0, int64_t i1, int lane) {
+  for (int64_t i = i0; i < i1; ++i) {
+    float m = NEG_BIG, l = 0.0f, o[2] = {0.0f, 0.0f};
+    for (int64_t j0 = 0; j0 <= i; j0 += 64) {
+      const int n = (int)(i - j0 < 63 ? i - j0 + 1 : 64);
+      const float s = lane < n ? dot_rows<L>(Q + i * q_rs, K + (j0 + lane) * k_rs, D) : -INFINITY;
+      const float mx = fmaxf(m, wave_max(s)), a = __builtin_amdgcn_exp2f((m - mx) * c);
+      const float w = lane < n ? __builtin_amdgcn_exp2f(fmaf(s, c, -(mx * c))) : 0.0f;
+      m = mx;
+      l = l * a + wave_sum(w);
+      o[0] *= a;
+      o[1] *= a;
+      add_weighted<L>(o, w, V + j0 * v_rs, v_rs, D, n, lane);
+      if (all_nan(o, D, lane)) break;
+    }
+    put_row<L>(O + i * o_rs, o, 1.0f / l, D, lane);
+  }
+}
+
 // ---- forward -------------------------------------------------------------------------------------------------------------------
 // NW waves x 32 queries; key / value tiles of KB = 64 rows in a ring of NST LDS slots, filled by LDS-DMA NST - 1 tiles ahead.  Every variant takes a
 // row's keys 64 at a time in the same steps, so a sequence's output does not depend on what it is packed with.
@@ -335,6 +416,11 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_fwd_kernel(const ffvc_
     for (int r = 0; r < 16; ++r) acc[t][r] *= inv;
   if (p.lse && ok && h == 0) p.lse[(int64_t)head * p.rows + pl.row0 + qi] = m * c + __builtin_amdgcn_logf(l);
   store_rows<L, DP>(O + qw * p.o_rs, p.o_rs, D, acc, l31, ok, h);
+  if (__any(ok && nonfinite<ND>(acc))) {
+    const int64_t far = (qw / KB + 1) * KB, last = far < pl.len ? far : pl.len;       // keys past qw that its last tile holds
+    if (any_nonfinite<L>(V, p.v_rs, D, qw + 1, last, lane))
+      redo_out<L>(Q, p.q_rs, Kp, p.k_rs, V, p.v_rs, O, p.o_rs, D, c, qw, qw + 32 < pl.len ? qw + 32 : pl.len, lane);
+  }
 }
 
 // ---- backward: dq (and delta) ----------------------------------------------------------------------------------------------------
@@ -442,6 +528,26 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_dq_kernel(const ffvc_a
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[t][r] *= p.scale;
   store_rows<L, DP>(dQ + qw * p.dq_rs, p.dq_rs, D, acc, l31, ok, h);
+  if (__any(ok && nonfinite<ND>(acc))) {
+    const int64_t far = (qw / KB + 1) * KB, last = far < pl.len ? far : pl.len;
+    if (any_nonfinite<L>(Kp, p.k_rs, D, qw + 1, last, lane))
+      for (int64_t i = qw; i < qw + 32 && i < pl.len; ++i) {                           // dq of these queries from their own keys alone
+        const float li = p.lse[(int64_t)head * p.rows + pl.row0 + i];
+        const float di = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(dl), (int)(i - qw)));
+        float o[2] = {0.0f, 0.0f};
+        for (int64_t j0 = 0; j0 <= i; j0 += 64) {
+          const int n = (int)(i - j0 < 63 ? i - j0 + 1 : 64);
+          float w = 0.0f;
+          if (lane < n) {
+            const float pr = __builtin_amdgcn_exp2f(fmaf(dot_rows<L>(Q + i * p.q_rs, Kp + (j0 + lane) * p.k_rs, D), c, -li));
+            w = pr * (dot_rows<L>(dO + i * p.do_rs, V + (j0 + lane) * p.v_rs, D) - di);
+          }
+          add_weighted<L>(o, w, Kp + j0 * p.k_rs, p.k_rs, D, n, lane);
+          if (all_nan(o, D, lane)) break;
+        }
+        put_row<L>(dQ + i * p.dq_rs, o, p.scale, D, lane);
+      }
+  }
 }
 
 // ---- backward: dk, dv --------------------------------------------------------------------------------------------------------------
@@ -635,6 +741,39 @@ __global__ __launch_bounds__(64 * NW * SPLIT, 2) void attn_packed_dkv_kernel(con
     for (int r = 0; r < 16; ++r) aK[t][r] *= p.scale;
   store_rows<L, DP>(dK + kw * p.dk_rs, p.dk_rs, D, aK, l31, ok, h);
   store_rows<L, DP>(dV + kw * p.dv_rs, p.dv_rs, D, aV, l31, ok, h);
+  if (!__any(ok && (nonfinite<ND>(aK) || nonfinite<ND>(aV)))) return;
+  // queries before the wave's last key that its first tile holds, in any head of the group
+  bool bad = false;
+  const int64_t f0 = kw / QB * QB, f1 = kw + 31 < pl.len ? kw + 31 : pl.len;
+  for (int gh = 0; gh < group && !bad; ++gh) {
+    const int head = kvh * group + gh;
+    bad = any_nonfinite<L>((const uint16_t*)p.q + pl.row0 * p.q_rs + head * p.q_hs, p.q_rs, D, f0, f1, lane) ||
+          any_nonfinite<L>((const uint16_t*)p.dout + pl.row0 * p.do_rs + head * p.do_hs, p.do_rs, D, f0, f1, lane);
+  }
+  if (!bad) return;
+  for (int64_t j = kw; j < kw + 32 && j < pl.len; ++j) {                               // dk, dv of these keys from the queries that see them alone
+    float ok_[2] = {0.0f, 0.0f}, ov_[2] = {0.0f, 0.0f};
+    for (int gh = 0; gh < group; ++gh) {
+      const int head = kvh * group + gh;
+      const uint16_t* Q = (const uint16_t*)p.q + pl.row0 * p.q_rs + head * p.q_hs;
+      const uint16_t* dO = (const uint16_t*)p.dout + pl.row0 * p.do_rs + head * p.do_hs;
+      const int64_t at = (int64_t)head * p.rows + pl.row0;
+      for (int64_t i0 = j; i0 < pl.len; i0 += 64) {
+        const int n = (int)(pl.len - i0 < 64 ? pl.len - i0 : 64);
+        float wv = 0.0f, wk = 0.0f;
+        if (lane < n) {
+          const int64_t i = i0 + lane;
+          wv = __builtin_amdgcn_exp2f(fmaf(dot_rows<L>(Q + i * p.q_rs, Kp + j * p.k_rs, D), c, -p.lse[at + i]));
+          wk = wv * (dot_rows<L>(dO + i * p.do_rs, V + j * p.v_rs, D) + p.delta[at + i]);       // (delta is stored negative)
+        }
+        add_weighted<L>(ov_, wv, dO + i0 * p.do_rs, p.do_rs, D, n, lane);
+        add_weighted<L>(ok_, wk, Q + i0 * p.q_rs, p.q_rs, D, n, lane);
+        if (all_nan(ov_, D, lane) && all_nan(ok_, D, lane)) break;
+      }
+    }
+    put_row<L>(dK + j * p.dk_rs, ok_, p.scale, D, lane);
+    put_row<L>(dV + j * p.dv_rs, ov_, 1.0f, D, lane);
+  }
 }
 
 int check_common(const ffvc_attn_packed_desc& d, const char* who) {

@@ -210,6 +210,43 @@ def test_attention_packed_matches_single_sequences(cuda, D):
         at += n
 
 
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("lens,H,G,D", [([70], 2, 1, 64), ([200, 45], 4, 2, 128), ([20, 9, 31], 2, 2, 64), ([150], 2, 2, 40)])
+def test_attention_packed_nonfinite_values_stay_behind_the_mask(cuda, lens, H, G, D, value):
+    """An inf / NaN in a token's v or k reaches no earlier query, one in its q or output gradient reaches no later key."""
+    T, scale = sum(lens), D ** -0.5
+    g = gen(17)
+    clean, do = randn(g, T, (H + 2 * G) * D, dtype=BF), randn(g, T, H * D, dtype=BF)
+    cu = offsets(lens)
+
+    def run(x, d):
+        leaf = x.clone().requires_grad_()
+        o = ops.attention_packed(leaf, cu, H, G)
+        return (o.detach().view(T, H, D),) + ops._split_heads(torch.autograd.grad(o, leaf, d)[0], H, G)
+
+    start = 0
+    for n in lens:
+        for t in {start, start + n // 3, start + n - 1}:
+            for what in ("v", "k", "q", "do"):
+                x, d = clean.clone(), do.clone()
+                parts = dict(zip("qkv", ops._split_heads(x, H, G)), do=d.view(T, H, D))
+                parts[what][t, :, 3 % D] = value
+                parts[what][t, -1] = value
+                got = run(x, d)
+                # what must not notice the token: as if it held zeros (64 bits), to the usual bounds
+                parts[what][t] = 0
+                ref, bound = attn_reference(*ops._split_heads(x, H, G), lens, scale, d.view(T, H, D))
+                other = [r for r in range(T) if r < start or r >= start + n]
+                before, after = list(range(start, t)), list(range(t + 1, start + n))
+                rows = {"v": (before, before, [], []), "k": (before, before, [], []), "q": (before + after, before + after, after, after),
+                        "do": (list(range(start, start + n)), before + after, after, after)}[what]
+                for name, a, b, e, keep in zip(("out", "dq", "dk", "dv"), got, ref, bound, rows):
+                    within(a[keep + other], b[keep + other], e[keep + other], f"{name} with {what}[{t}] = {value}")
+                if what == "v":
+                    assert not bool(torch.isfinite(got[0][t:start + n, -1]).any())
+        start += n
+
+
 def test_attention_packed_bad_offsets_stay_inside(cuda):
     """Offsets that descend or leave the tensor are clamped: other rows' values may come out, nothing outside is touched."""
     g = gen(11)
