@@ -7,15 +7,14 @@
 // token per prompt makes thousands of adds collide on one row).  Here the token positions are sorted by id first — stable, so the sum of a
 // row runs over its tokens in their order — and then every table row is produced by one owner: no zero pass, no atomics, the same bits
 // every time.  The work is cut by sorted positions, not by rows (ids come ordered by frequency, so a few neighbouring rows hold most tokens): a
-// wave sums CHUNK of them and writes the rows whose tokens it has all seen, a second kernel joins the parts of longer runs and writes the zeros.
+// wave sums a chunk of them and writes the rows whose tokens it has all seen, a second kernel joins the parts of longer runs and writes the zeros.
 // Sorting: up to RANK_MAX tokens one launch ranks every key against all others out of LDS (n^2 compares spread over the chip); above, a
-// least-significant-digit radix sort, 8 bits per pass, three launches each.
+// least-significant-digit radix sort, 8 bits per pass, two or three launches each.
 #include "common.h"
 
 namespace {
 
 constexpr int RANK_MAX = 8192;      // tokens
-constexpr int CHUNK = 64;
 constexpr int RT = 1024;            // keys per workgroup of a radix pass
 
 template <typename T, int VEC>
@@ -161,7 +160,7 @@ __global__ __launch_bounds__(256) void embed_scan_kernel(uint32_t* __restrict__ 
 // Stable scatter: wave w of a tile owns a quarter of its keys and walks them 64 at a time; lanes of one digit find each other by ballots.
 __global__ __launch_bounds__(256) void embed_scatter_kernel(const int64_t* __restrict__ ids, const uint32_t* __restrict__ keys,
                                                             const uint32_t* __restrict__ vals, int64_t vocab, int64_t n, int shift,
-                                                            const uint32_t* __restrict__ hist, const uint32_t* __restrict__ total, int tiles,
+                                                            const uint32_t* __restrict__ hist, const uint32_t* __restrict__ total, int tiles, int scanned,
                                                             uint32_t* __restrict__ keys_out, uint32_t* __restrict__ vals_out) {
   __shared__ uint32_t at[4][256];                            // next position of each digit, per wave
   __shared__ uint32_t part[4];
@@ -171,7 +170,18 @@ __global__ __launch_bounds__(256) void embed_scatter_kernel(const int64_t* __res
   for (int w = 0; w < 4; ++w) at[w][tid] = 0;
   uint32_t base;                                              // keys of smaller digits, and of this digit in earlier tiles
   {
-    const uint32_t v = total[tid];
+    uint32_t v = 0, mine = 0;                                 // this digit's keys in all tiles, in earlier tiles
+    if (scanned) {
+      v = total[tid];
+      mine = hist[(int64_t)tid * tiles + blockIdx.x];
+    } else {
+#pragma unroll 8
+      for (int t = 0; t < tiles; ++t) {
+        const uint32_t c = hist[(int64_t)tid * tiles + t];
+        mine += t < (int)blockIdx.x ? c : 0u;
+        v += c;
+      }
+    }
     uint32_t s = v;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -180,7 +190,7 @@ __global__ __launch_bounds__(256) void embed_scatter_kernel(const int64_t* __res
     }
     if (lane == 63) part[wave] = s;
     __syncthreads();
-    base = s - v + hist[(int64_t)tid * tiles + blockIdx.x];
+    base = s - v + mine;
     for (int w = 0; w < wave; ++w) base += part[w];
   }
   const int64_t first = (int64_t)blockIdx.x * RT + wave * PW;
@@ -225,18 +235,18 @@ __global__ __launch_bounds__(256) void embed_scatter_kernel(const int64_t* __res
 }
 
 // ---- sums ------------------------------------------------------------------------------------------------------------------------------
-// One wave per chunk of CHUNK sorted positions and block of 64 * VEC columns.  Runs of one id that begin and end inside the chunk go straight
+// One wave per chunk of `chunk` <= 64 sorted positions and block of 64 * VEC columns.  Runs of one id that begin and end inside the chunk go straight
 // to their table row; one that came in from the chunk before leaves its sum in part[2 c], one that goes on into the next in part[2 c + 1].
 // first / end: the sorted positions of each row's tokens (the rows kernel's map).
 template <typename DT, typename TT, int VEC>
 __global__ __launch_bounds__(256) void embed_runs_kernel(const uint32_t* __restrict__ keys, const uint32_t* __restrict__ vals, int n, uint32_t vocab,
                                                          const DT* __restrict__ dout, int64_t ld, int dim, float scale, float* __restrict__ part,
-                                                         int* __restrict__ first, int* __restrict__ end, TT* __restrict__ dtable) {
+                                                         int* __restrict__ first, int* __restrict__ end, TT* __restrict__ dtable, int chunk) {
   const int lane = threadIdx.x & 63;
   const int64_t c = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t p0 = c * CHUNK;
+  const int64_t p0 = c * chunk;
   if (p0 >= n) return;
-  const int m = __builtin_amdgcn_readfirstlane((int)(n - p0 < CHUNK ? n - p0 : CHUNK));
+  const int m = __builtin_amdgcn_readfirstlane((int)(n - p0 < chunk ? n - p0 : chunk));
   const uint32_t key = lane < m ? keys[p0 + lane] : 0xFFFFFFFFu;
   const uint32_t val = lane < m ? vals[p0 + lane] : 0u;
   const uint32_t left = p0 + lane > 0 && lane <= m ? keys[p0 + lane - 1] : 0xFFFFFFFFu;      // (lane m: the chunk's last key)
@@ -248,7 +258,7 @@ __global__ __launch_bounds__(256) void embed_runs_kernel(const uint32_t* __restr
     if (key != right) end[key] = (int)(p0 + lane + 1);
   }
   const bool in = !(starts & 1ull);                            // the chunk's first run came in from the chunk before
-  const bool out = m == CHUNK && __builtin_amdgcn_readlane(key, CHUNK - 1) == __builtin_amdgcn_readfirstlane(next);
+  const bool out = p0 + m < n && __builtin_amdgcn_readlane(key, m - 1) == __builtin_amdgcn_readfirstlane(next);
   const int d = (blockIdx.y * 64 + lane) * VEC;
   const bool live = d < dim;
   float acc[VEC];
@@ -293,7 +303,7 @@ __global__ __launch_bounds__(256) void embed_runs_kernel(const uint32_t* __restr
 constexpr int ROWS = 4, SHORT = 8;
 template <typename TT, int VEC>
 __global__ __launch_bounds__(256) void embed_rows_kernel(const int* __restrict__ first, const int* __restrict__ end, int64_t vocab, int dim, float scale,
-                                                         const float* __restrict__ part, TT* __restrict__ dtable) {
+                                                         const float* __restrict__ part, TT* __restrict__ dtable, int chunk) {
   __shared__ float sums[4][64 * VEC];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t v0 = (int64_t)blockIdx.x * ROWS;
@@ -315,7 +325,7 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const int* __restrict__
   for (int r = 0; r < ROWS; ++r) {
     a[r] = r < nr ? __builtin_amdgcn_readfirstlane(first[v0 + r]) : 0;
     const int b = r < nr && a[r] >= 0 ? __builtin_amdgcn_readfirstlane(end[v0 + r]) : 0;
-    np[r] = r < nr && a[r] >= 0 ? (b - 1) / CHUNK - a[r] / CHUNK + 1 : 0;         // 0: no token; 1: written already
+    np[r] = r < nr && a[r] >= 0 ? (b - 1) / chunk - a[r] / chunk + 1 : 0;         // 0: no token; 1: written already
   }
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
@@ -325,13 +335,13 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const int* __restrict__
     TT* row = dtable + (v0 + r) * dim + d;
     if (np[r] <= SHORT) {
       if (r < nr && r % 4 == wave && np[r] != 1) {
-        add(acc, a[r] / CHUNK, 0, np[r]);
+        add(acc, a[r] / chunk, 0, np[r]);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) acc[e] *= scale;
         if (live) store_vec<TT, VEC>(row, acc);
       }
     } else {
-      add(acc, a[r] / CHUNK, (int)((int64_t)np[r] * wave / 4), (int)((int64_t)np[r] * (wave + 1) / 4));
+      add(acc, a[r] / chunk, (int)((int64_t)np[r] * wave / 4), (int)((int64_t)np[r] * (wave + 1) / 4));
 #pragma unroll
       for (int e = 0; e < VEC; ++e) sums[wave][lane * VEC + e] = acc[e];
       __syncthreads();
@@ -350,10 +360,11 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const int* __restrict__
 
 struct Layout {      // the workspace: two (keys, vals) pairs, first / end of every row, the radix counters, the parts
   int64_t pair, tiles, rows, hist, part, bytes;
+  int chunk;
   bool rank;
   Layout(int64_t n, int64_t vocab, int dim) {
     auto up = [](int64_t b) { return (b + 15) / 16 * 16; };
-    // One ranking launch against one or more radix passes of three: the ranking grows with n^2 (measured 17 us at 8192 tokens, 46 at 13600),
+    // One ranking launch against one or more radix passes of two or three: the ranking grows with n^2 (measured 17 us at 8192 tokens, 46 at 13600),
     // a pass takes about 12 us up to 100000 tokens.
     rank = n <= (vocab < 256 ? RANK_MAX / 2 : RANK_MAX);
     pair = up(n * 4);
@@ -361,18 +372,20 @@ struct Layout {      // the workspace: two (keys, vals) pairs, first / end of ev
     hist = rows + 2 * up(vocab * 4);
     tiles = (n + RT - 1) / RT;
     part = hist + (rank ? 0 : up((256 * tiles + 256) * 4));
-    bytes = part + 2 * ((n + CHUNK - 1) / CHUNK) * dim * 4;
+    // Sorted positions per wave: short chunks until the waves fill the chip, long ones (fewer parts to join) from there.
+    chunk = n < 32768 ? 16 : 64;
+    bytes = part + 2 * ((n + chunk - 1) / chunk) * dim * 4;
   }
 };
 
 template <typename DT, typename TT, int VEC>
 int run_sums(const uint32_t* keys, const uint32_t* vals, int64_t n, int64_t vocab, const void* dout, int64_t ld, int dim, float scale, float* part,
-             int* first, int* end, void* dtable, hipStream_t st) {
+             int* first, int* end, void* dtable, int chunk, hipStream_t st) {
   const int ncb = (dim + 64 * VEC - 1) / (64 * VEC);
-  hipLaunchKernelGGL((embed_runs_kernel<DT, TT, VEC>), dim3((unsigned)((n + 4 * CHUNK - 1) / (4 * CHUNK)), ncb), dim3(256), 0, st, keys, vals, (int)n,
-                     (uint32_t)vocab, (const DT*)dout, ld, dim, scale, part, first, end, (TT*)dtable);
+  hipLaunchKernelGGL((embed_runs_kernel<DT, TT, VEC>), dim3((unsigned)((n + 4 * chunk - 1) / (4 * chunk)), ncb), dim3(256), 0, st, keys, vals, (int)n,
+                     (uint32_t)vocab, (const DT*)dout, ld, dim, scale, part, first, end, (TT*)dtable, chunk);
   hipLaunchKernelGGL((embed_rows_kernel<TT, VEC>), dim3((unsigned)((vocab + ROWS - 1) / ROWS), ncb), dim3(256), 0, st, first, end, vocab, dim, scale, part,
-                     (TT*)dtable);
+                     (TT*)dtable, chunk);
   FFVC_LAUNCH_CHECK();
   return 0;
 }
@@ -436,9 +449,10 @@ extern "C" int ffvc_embed_bwd(const void* dout, int dout_dtype, int64_t ld, cons
       const int64_t* src = first ? ids : nullptr;
       const int nx = first ? 0 : cur ^ 1;
       hipLaunchKernelGGL(embed_hist_kernel, dim3(tiles), dim3(256), 0, st, src, keys[cur], vocab, n, shift, hist, tiles, first ? row_first : nullptr);
-      hipLaunchKernelGGL(embed_scan_kernel, dim3(256), dim3(256), 0, st, hist, total, tiles);
+      const int scanned = tiles > 32;                          // (few tiles: every workgroup adds up the counts itself, a launch less)
+      if (scanned) hipLaunchKernelGGL(embed_scan_kernel, dim3(256), dim3(256), 0, st, hist, total, tiles);
       hipLaunchKernelGGL(embed_scatter_kernel, dim3(tiles), dim3(256), 0, st, src, keys[cur], first ? nullptr : vals[cur], vocab, n, shift, hist, total,
-                         tiles, keys[nx], vals[nx]);
+                         tiles, scanned, keys[nx], vals[nx]);
       cur = nx;
       first = false;
     }
@@ -447,8 +461,8 @@ extern "C" int ffvc_embed_bwd(const void* dout, int dout_dtype, int64_t ld, cons
   const bool vec = dim % 8 == 0 && al(dout, dout_dtype, ld) && al(dtable, table_dtype, dim);
   float* part = (float*)(w + lay.part);
   DISPATCH_DT(dout_dtype, DT, DISPATCH_DT(table_dtype, TT, {
-    return vec ? run_sums<DT, TT, 8>(keys[cur], vals[cur], n, vocab, dout, ld, dim, scale, part, row_first, row_end, dtable, st)
-               : run_sums<DT, TT, 1>(keys[cur], vals[cur], n, vocab, dout, ld, dim, scale, part, row_first, row_end, dtable, st);
+    return vec ? run_sums<DT, TT, 8>(keys[cur], vals[cur], n, vocab, dout, ld, dim, scale, part, row_first, row_end, dtable, lay.chunk, st)
+               : run_sums<DT, TT, 1>(keys[cur], vals[cur], n, vocab, dout, ld, dim, scale, part, row_first, row_end, dtable, lay.chunk, st);
   }));
   return 0;
 }

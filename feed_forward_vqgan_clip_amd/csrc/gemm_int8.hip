@@ -445,6 +445,7 @@ __global__ __launch_bounds__(512) void gemm_int8_skinny_kernel(const I8Args p) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) acc[0][i] = acc[1][i] = 0;
   const u32x4_t z = {0u, 0u, 0u, 0u};
+#pragma unroll 2
   for (int k0 = wave * 128; k0 < p.K; k0 += 1024) {
     u32x4_t a[4], b0[4], b1[4];
 #pragma unroll
