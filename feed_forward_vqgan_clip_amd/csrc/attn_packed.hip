@@ -158,13 +158,53 @@ __device__ __forceinline__ Place find_slot(const int32_t* __restrict__ cu, int s
   return p;
 }
 
-// block -> (slot, head).  Consecutive workgroups go to the 8 XCDs in turn: with a multiple of 8 heads each XCD keeps heads / 8 neighbouring
-// heads, so the heads of one key / value group read it through one L2.  The last tiles of the sequences (the longest rows) go first.
-__device__ __forceinline__ void block_place(int64_t slots, int heads, int64_t& slot, int& head) {
+// The r-th longest piece of work: tiles in the order of their walks' lengths, so that the last ones to start are short (KEYS: a key tile's walk is
+// over the rows from it on, otherwise over the rows up to it).  Among 2 .. 63 sequences, level j holds the tiles with j others of their sequence on
+// their walk; cum(j) = sum_b max(tiles_b - j, 0) counts the levels from j on, 64 probes at a time.  A single sequence is in order as it is.
+template <int BM, bool KEYS>
+__device__ __forceinline__ Place find_tile(const int32_t* __restrict__ cu, int seqs, int64_t rows, int64_t slots, int64_t r) {
+  if (seqs == 1 || seqs > 63) return find_slot<BM>(cu, seqs, rows, KEYS ? r : slots - 1 - r);
+  const int lane = threadIdx.x & 63;
+  const int c0 = (int)(lane <= seqs ? cu_at(cu, lane, rows) : rows);
+  const int c1 = (int)(lane < seqs ? cu_at(cu, lane + 1, rows) : rows);
+  const int tiles = lane < seqs && c1 > c0 ? (int)(((int64_t)c1 - c0 + BM - 1) / BM) : 0;
+  Place p;
+  int lo = 0, n = (int)(rows / BM) + 1, at = 0;        // levels lo .. lo + n - 1; cum(lo)
+  do {
+    const int step = (n + 63) / 64, j = lo + lane * step;
+    int cum = 0;
+    for (int b = 0; b < seqs; ++b) cum += max(__builtin_amdgcn_readlane(tiles, b) - j, 0);
+    const uint64_t m = __ballot(lane * step < n && cum > r);
+    if (m == 0) {                                       // behind all tiles: the rows behind the last sequence
+      p.row0 = __builtin_amdgcn_readlane(c0, seqs);
+      p.len = rows - p.row0;
+      p.tile = r - __builtin_amdgcn_readlane(cum, 0);
+      p.tail = true;
+      return p;
+    }
+    const int k = 63 - __builtin_clzll(m);
+    at = __builtin_amdgcn_readlane(cum, k);
+    lo += k * step;
+    n = min(step, n - k * step);
+  } while (n > 1);
+  const uint64_t level = __ballot(tiles > lo);
+  const int rank = (int)(r - (at - __popcll(level)));
+  const bool mine = ((level >> lane) & 1) && __popcll(level & ((1ull << lane) - 1)) == rank;
+  const int b = __builtin_ctzll(__ballot(mine) | 1ull << 63);
+  p.row0 = __builtin_amdgcn_readlane(c0, b);
+  p.len = __builtin_amdgcn_readlane(c1, b) - p.row0;
+  p.tile = KEYS ? __builtin_amdgcn_readlane(tiles, b) - 1 - lo : lo;
+  p.tail = false;
+  return p;
+}
+
+// block -> (rank of the tile, head).  Consecutive workgroups go to the 8 XCDs in turn: with a multiple of 8 heads each XCD keeps heads / 8
+// neighbouring heads, so the heads of one key / value group read it through one L2.
+__device__ __forceinline__ void block_place(int heads, int64_t& rank, int& head) {
   const int64_t i = blockIdx.x;
   const int j = (int)(i % heads);
   head = heads % 8 == 0 ? (j & 7) * (heads >> 3) + (j >> 3) : j;
-  slot = slots - 1 - i / heads;
+  rank = i / heads;
 }
 
 // o[row0 + lane % 32][32 dt + ...] = acc, rows < n; the wave's tile is transposed (lane = row, registers = features)
@@ -292,10 +332,10 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_fwd_kernel(const ffvc_
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int64_t slot;
+  int64_t rank;
   int head;
-  block_place(slots, p.heads, slot, head);
-  const Place pl = find_slot<BM>(p.cu, p.seqs, p.rows, slot);
+  block_place(p.heads, rank, head);
+  const Place pl = find_slot<BM>(p.cu, p.seqs, p.rows, slots - 1 - rank);      // (a sequence's last tiles, with the longest walks, first)
   const int64_t q0 = pl.tile * BM;
   if (q0 < 0 || q0 >= pl.len) return;
   const int D = p.head_dim;
@@ -430,10 +470,10 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_dq_kernel(const ffvc_a
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int64_t slot;
+  int64_t rank;
   int head;
-  block_place(slots, p.heads, slot, head);
-  const Place pl = find_slot<BM>(p.cu, p.seqs, p.rows, slot);
+  block_place(p.heads, rank, head);
+  const Place pl = find_tile<BM, false>(p.cu, p.seqs, p.rows, slots, rank);
   const int64_t q0 = pl.tile * BM;
   if (q0 < 0 || q0 >= pl.len) return;
   const int D = p.head_dim;
@@ -552,12 +592,12 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_dq_kernel(const ffvc_a
 
 // ---- backward: dk, dv --------------------------------------------------------------------------------------------------------------
 // NW waves x 32 keys of one key / value head; walks the query tiles (QB rows of q and dout, two LDS stages) that see them, for every query head
-// of the group.  K stays in registers as the B operand of s = q k^T; V, the B operand of dp = do v^T, stays in LDS: with both in registers next
-// to the two accumulators a wave needs more than half the register file, and one wave per SIMD cannot hide its own waits (963 us against
-// ... at 8192 rows, 16 heads of 128).
+// of the group.  K stays in registers as the B operand of s = q k^T.  V, the B operand of dp = do v^T, stays there too at 64 features; at 128 both
+// next to the two accumulators would take more than half the register file, and one wave per SIMD cannot hide its own waits: V lies in LDS
+// (8192 rows, 16 heads of 128: 963 us with V in registers, 560 in LDS) and a step takes 32 queries, not 64.
 //
-// SPLIT = 2: eight waves, the second four take every other (head, query tile) of the same keys and their sums join in LDS at the end.  A key tile's
-// walk is as long as its sequence times the group, so with few tiles the longest one alone decides (see run_bwd).
+// SPLIT > 1: SPLIT * NW waves, each NW of them take every SPLIT-th (head, query tile) of the same keys; the sums join in LDS at the end, in order.
+// (run_bwd has the rule and its figures.)
 template <typename L, int DP, int NW, int NST, int QB, bool VLDS, int SPLIT>
 __global__ __launch_bounds__(64 * NW * SPLIT, 2) void attn_packed_dkv_kernel(const ffvc_attn_packed_desc p, int64_t slots) {
   constexpr int BM = 32 * NW, NS = DP / 16, ND = DP / 32, TB = QB * DP * 2, VB = VLDS ? BM * DP * 2 : 0;
@@ -567,11 +607,10 @@ __global__ __launch_bounds__(64 * NW * SPLIT, 2) void attn_packed_dkv_kernel(con
   unsigned char* smem = smem_all + part * (NST * 2 * TB);
   unsigned char* vmem = smem_all + SPLIT * (NST * 2 * TB);
   float* stat = (float*)(vmem + VB) + part * (NST * 2 * 64); // [slots][lse | delta][64]
-  int64_t slot;
+  int64_t rank;
   int kvh;
-  block_place(slots, p.kv_heads, slot, kvh);
-  slot = slots - 1 - slot;                                  // the first keys are seen by the most queries: they go first
-  const Place pl = find_slot<BM>(p.cu, p.seqs, p.rows, slot);
+  block_place(p.kv_heads, rank, kvh);
+  const Place pl = find_tile<BM, true>(p.cu, p.seqs, p.rows, slots, rank);
   const int64_t k0 = pl.tile * BM;
   if (k0 < 0 || k0 >= pl.len) return;
   const int D = p.head_dim;
@@ -716,20 +755,23 @@ __global__ __launch_bounds__(64 * NW * SPLIT, 2) void attn_packed_dkv_kernel(con
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   if constexpr (SPLIT > 1) {
-    float* join = (float*)smem_all + wave * (ND * 16 * 64) + lane;      // [wave][register][lane] over the stages nobody reads any more
+    constexpr int W = ND * 16 * 64;
+    float* join = (float*)smem_all + wave * W + lane;                    // [part - 1][wave][register][lane] over the stages nobody reads any more
     auto add = [&](f32x16_t (&acc)[ND]) {
       __syncthreads();
       if (part)
 #pragma unroll
         for (int t = 0; t < ND; ++t)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) join[(t * 16 + r) * 64] = acc[t][r];
+          for (int r = 0; r < 16; ++r) join[(part - 1) * NW * W + (t * 16 + r) * 64] = acc[t][r];
       __syncthreads();
       if (!part)
 #pragma unroll
-        for (int t = 0; t < ND; ++t)
+        for (int o = 0; o < SPLIT - 1; ++o)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) acc[t][r] += join[(t * 16 + r) * 64];
+          for (int t = 0; t < ND; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[t][r] += join[o * NW * W + (t * 16 + r) * 64];
     };
     add(aK);
     add(aV);
@@ -835,12 +877,19 @@ int run_bwd(const ffvc_attn_packed_desc& d, hipStream_t st) {
     constexpr int NW = 4, NST = 2, KB = 64, QB = DP == 64 ? 64 : 32;
     const int64_t slots = d.rows / (32 * NW) + d.seqs + 1;
     LAUNCH_PACKED((attn_packed_dq_kernel<L, DP, NW, NST, KB>), NST * 2 * KB * DP * 2, d.heads, 64 * NW);
-    // Two halves per key tile while the tiles do not fill the chip's 512 places one and a half times: 208 -> 143 us on 24 ragged sequences of up to
-    // 2100 rows with 4 key heads (520 tiles), but 594 -> 655 us on one of 8192 rows with 16 (1056 tiles).
-    if (slots * d.kv_heads < 768)
-      LAUNCH_PACKED((attn_packed_dkv_kernel<L, DP, NW, NST, QB, VLDS, 2>), dkv_lds(DP, NW, NST, QB, VLDS, 2), d.kv_heads, 128 * NW);
-    else
-      LAUNCH_PACKED((attn_packed_dkv_kernel<L, DP, NW, NST, QB, VLDS, 1>), dkv_lds(DP, NW, NST, QB, VLDS, 1), d.kv_heads, 64 * NW);
+    // A key tile's walk is as long as its sequence times the group: while the tiles are few for the chip's 512 places the longest walk alone decides,
+    // so it is split over the workgroup's waves.  Measured (1 / 2 / 4 parts; the last with tiles of 64 keys), us:
+    //   520 tiles, 24 ragged sequences of up to 2100 rows, 64 features: 208 / 143 / 108; 128 features: 397 / 248 / 236; one sequence, 264 tiles: 1520 / 935 / 614
+    //   884 tiles, 40 ragged sequences: 247 / 213 / 229; 128 features: 424 / 316 / 434; 12 sequences of 2048 rows, 820 tiles: 233 / 252 / 276
+    //   1056 tiles, one sequence of 8192 rows: 298 / 311 / 347; 128 features: 540 / 562 / 757
+    if (slots * d.kv_heads < 768) {
+      const int64_t slots = d.rows / 64 + d.seqs + 1;
+      LAUNCH_PACKED((attn_packed_dkv_kernel<L, DP, 2, NST, QB, VLDS, 4>), dkv_lds(DP, 2, NST, QB, VLDS, 4), d.kv_heads, 512);
+    } else if (slots * d.kv_heads < 1024) {
+      LAUNCH_PACKED((attn_packed_dkv_kernel<L, DP, 4, NST, QB, VLDS, 2>), dkv_lds(DP, 4, NST, QB, VLDS, 2), d.kv_heads, 512);
+    } else {
+      LAUNCH_PACKED((attn_packed_dkv_kernel<L, DP, 4, NST, QB, VLDS, 1>), dkv_lds(DP, 4, NST, QB, VLDS, 1), d.kv_heads, 256);
+    }
   }
   return 0;
 }

@@ -136,6 +136,41 @@ def test_attention_packed_forward_and_gradients(cuda, case, dtype):
     assert torch.equal(again, dqkv)
 
 
+# the backward splits a key tile's walk in four, in two or not at all, by the number of tiles times key heads; among 2 .. 63 sequences it takes
+# the tiles by the length of their walks, otherwise in order
+MIXED = [300, 200, 129, 0, 511, 33, 256]
+SPLITS = [  # lens, rows behind them, heads, kv_heads, head_dim
+    (MIXED, 37, 4, 2, 64),
+    (MIXED, 300, 4, 2, 128),
+    (MIXED, 37, 48, 48, 64),
+    (MIXED, 37, 96, 48, 128),
+    (MIXED, 37, 64, 64, 72),
+    ([1500], 0, 96, 96, 64),
+    ([68, 72] * 35, 3, 8, 4, 64),
+    ([68, 72] * 35, 3, 8, 8, 128),
+    ([68, 72] * 35, 3, 16, 16, 64),
+    ([0, 900] + [64] * 61, 130, 4, 4, 64),
+]
+
+
+@pytest.mark.parametrize("case", range(len(SPLITS)))
+def test_attention_packed_gradients_at_every_split(cuda, case):
+    lens, spare, H, G, D = SPLITS[case]
+    g = gen(900 + case)
+    T = sum(lens) + spare
+    qkv = randn(g, T, (H + 2 * G) * D, dtype=BF).requires_grad_()
+    do = randn(g, T, H * D, dtype=BF)
+    q, k, v = ops._split_heads(qkv.detach(), H, G)
+    (o, dq, dk, dv), (bo, bq, bk, bv) = attn_reference(q, k, v, lens, D ** -0.5, do.view(T, H, D))
+    got = ops.attention_packed(qkv, offsets(lens), H, G)
+    within(got.view(T, H, D), o, bo, "out")
+    (dqkv,) = torch.autograd.grad(got, qkv, do)
+    for name, a, b, c in zip(("dq", "dk", "dv"), ops._split_heads(dqkv, H, G), (dq, dk, dv), (bq, bk, bv)):
+        within(a, b, c, name)
+    if spare:
+        assert float(got[T - spare:].abs().max()) == 0 and float(dqkv[T - spare:].abs().max()) == 0
+
+
 def test_attention_packed_gradient_by_differences(cuda):
     """The change of sum(out * w) along the gradient's own signs, through the forward kernel alone.  What the difference may be off by: the
     truncation (the 64-bit forward's own difference against its gradient), every output's bound on both sides, every gradient's bound."""
