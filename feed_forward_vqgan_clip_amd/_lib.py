@@ -241,6 +241,9 @@ _SIGNATURES = {
                                c_int64, c_int, c_void_p]),
     "ffvc_embed_bwd_ws_bytes": (c_int64, [c_int64, c_int64, c_int]),
     "ffvc_embed_bwd": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int64, c_int64, c_int, c_float, c_void_p, c_int, c_void_p, c_int64, c_void_p]),
+    "ffvc_embed_bwd_pair_ws_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int]),
+    "ffvc_embed_bwd_pair": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int64, c_int64, c_int, c_float, c_void_p, c_void_p, c_int64, c_void_p, c_int,
+                                    c_void_p, c_int64, c_void_p]),
     "ffvc_attn_packed_fwd": (c_int, [POINTER(AttnPackedDesc), c_void_p]),
     "ffvc_attn_packed_bwd": (c_int, [POINTER(AttnPackedDesc), c_void_p]),
     "ffvc_int8_quant": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p]),

@@ -8,8 +8,12 @@
 // row runs over its tokens in their order — and then every table row is produced by one owner: no zero pass, no atomics, the same bits
 // every time.  The work is cut by sorted positions, not by rows (ids come ordered by frequency, so a few neighbouring rows hold most tokens): a
 // wave sums a chunk of them and writes the rows whose tokens it has all seen, a second kernel joins the parts of longer runs and writes the zeros.
+// Bound by bytes: 113000 tokens of 1024 bf16 read for both tables in 99 us (4.7 TB/s); the rows kernel (41 us there) by its workgroups' launches and
+// the longest runs' joins.  The lookup is one wave per token and bound by its writes (82 us there: 232 MB out, about 100 in).
 // Sorting: up to RANK_MAX tokens one launch ranks every key against all others out of LDS (n^2 compares spread over the chip); above, a
 // least-significant-digit radix sort, 8 bits per pass, two or three launches each.
+#include <type_traits>
+
 #include "common.h"
 
 namespace {
@@ -71,24 +75,46 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const TT* __restrict__ t
   }
 }
 
-// first[v] = -1 (no token) for every row, by the first kernel of the chain
-__device__ __forceinline__ void clear_first(int* __restrict__ first, int64_t vocab) {
-  for (int64_t v = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; v < vocab; v += (int64_t)gridDim.x * blockDim.x) first[v] = -1;
+// One table's gradient.  The token table's and the position table's are two chains of small launches over the same dout: they go through every
+// launch together, blockIdx.z (or the block's place) picks the table (509 prompts, 21000 tokens of 512, 77 positions: 52 us for both, 50 for the
+// token table alone, 32 more for the positions in launches of their own).
+struct Job {
+  const int64_t* ids;          // null: row t for token t
+  int64_t vocab;
+  float scale;
+  void* dtable;
+  uint32_t *keys[2], *vals[2];
+  uint32_t *hist, *total;      // radix counters
+  int* span;                   // [vocab][2]: each row's first sorted token and the place after its last
+  float* part;
+  int sorted;                  // which pair holds the sorted tokens
+};
+struct Jobs {
+  Job j[2];
+};
+
+// span[v][0] = -1 (no token) for every row, by the first kernel of the chain
+__device__ __forceinline__ void clear_span(const Job& job) {
+  for (int64_t v = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; v < job.vocab; v += (int64_t)gridDim.x * blockDim.x) job.span[2 * v] = -1;
 }
 
 // ids outside the table sort behind every row
-__device__ __forceinline__ uint32_t key_of(int64_t id, int64_t vocab) { return id >= 0 && id < vocab ? (uint32_t)id : (uint32_t)vocab; }
+__device__ __forceinline__ uint32_t key_of(const Job& job, int64_t t) {
+  const int64_t id = job.ids ? job.ids[t] : t;
+  return (uint32_t)(id >= 0 && id < job.vocab ? id : job.vocab);
+}
 
 // ---- sort, small: position of token t = #{keys below its own} + #{equal keys before it}.  A workgroup ranks 32 tokens; its 32 half-waves
 // split the keys (all of a half-wave's lanes read the same key: an LDS broadcast).
-__global__ __launch_bounds__(1024) void embed_rank_kernel(const int64_t* __restrict__ ids, int64_t vocab, int n, uint32_t* __restrict__ keys,
-                                                          uint32_t* __restrict__ vals, int* __restrict__ first) {
-  clear_first(first, vocab);
+__global__ __launch_bounds__(1024) void embed_rank_kernel(const Jobs jobs, int n) {
+  const Job& job = jobs.j[blockIdx.z];
+  uint32_t *keys = job.keys[0], *vals = job.vals[0];
+  clear_span(job);
   extern __shared__ __attribute__((aligned(16))) uint32_t k[];
   const int tid = threadIdx.x;
   const int np = (n + 127) / 128 * 128;                       // whole groups of 4 keys per part
   int* cnt = (int*)(k + np);                                  // [32]
-  for (int i = tid; i < np; i += 1024) k[i] = i < n ? key_of(ids[i], vocab) : 0xFFFFFFFFu;
+  for (int i = tid; i < np; i += 1024) k[i] = i < n ? key_of(job, i) : 0xFFFFFFFFu;
   if (tid < 32) cnt[tid] = 0;
   __syncthreads();
   const int t = blockIdx.x * 32 + (tid & 31), part = tid >> 5;
@@ -115,10 +141,15 @@ __global__ __launch_bounds__(1024) void embed_rank_kernel(const int64_t* __restr
 }
 
 // ---- sort, large ----------------------------------------------------------------------------------------------------------------------
+// A table's passes are those of its own bits: the other one's further launches find nothing to do.
+__device__ __forceinline__ bool pass_done(const Job& job, int shift) { return shift > 0 && (job.vocab >> shift) == 0; }
+
 // hist[digit][tile] of the 8 bits at `shift`
-__global__ __launch_bounds__(256) void embed_hist_kernel(const int64_t* __restrict__ ids, const uint32_t* __restrict__ keys, int64_t vocab, int64_t n,
-                                                         int shift, uint32_t* __restrict__ hist, int tiles, int* __restrict__ first) {
-  if (first) clear_first(first, vocab);
+__global__ __launch_bounds__(256) void embed_hist_kernel(const Jobs jobs, int64_t n, int shift, int tiles) {
+  const Job& job = jobs.j[blockIdx.z];
+  if (pass_done(job, shift)) return;
+  const uint32_t* keys = job.keys[(shift / 8 + 1) & 1];
+  if (shift == 0) clear_span(job);
   __shared__ uint32_t h[256];
   const int tid = threadIdx.x;
   h[tid] = 0;
@@ -126,16 +157,18 @@ __global__ __launch_bounds__(256) void embed_hist_kernel(const int64_t* __restri
   const int64_t base = (int64_t)blockIdx.x * RT;
   for (int i = tid; i < RT; i += 256) {
     const int64_t t = base + i;
-    if (t < n) atomicAdd(&h[((ids ? key_of(ids[t], vocab) : keys[t]) >> shift) & 255u], 1u);
+    if (t < n) atomicAdd(&h[((shift == 0 ? key_of(job, t) : keys[t]) >> shift) & 255u], 1u);
   }
   __syncthreads();
-  hist[(int64_t)tid * tiles + blockIdx.x] = h[tid];
+  job.hist[(int64_t)tid * tiles + blockIdx.x] = h[tid];
 }
 
 // exclusive scan of one digit's row of `hist`; the digit's total
-__global__ __launch_bounds__(256) void embed_scan_kernel(uint32_t* __restrict__ hist, uint32_t* __restrict__ total, int tiles) {
+__global__ __launch_bounds__(256) void embed_scan_kernel(const Jobs jobs, int shift, int tiles) {
   __shared__ uint32_t part[4];
-  uint32_t* row = hist + (int64_t)blockIdx.x * tiles;
+  const Job& job = jobs.j[blockIdx.z];
+  if (pass_done(job, shift)) return;
+  uint32_t* row = job.hist + (int64_t)blockIdx.x * tiles;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   uint32_t run = 0;
   for (int b = 0; b < tiles; b += 256) {
@@ -154,14 +187,16 @@ __global__ __launch_bounds__(256) void embed_scan_kernel(uint32_t* __restrict__ 
     run += part[0] + part[1] + part[2] + part[3];
     __syncthreads();
   }
-  if (tid == 0) total[blockIdx.x] = run;
+  if (tid == 0) job.total[blockIdx.x] = run;
 }
 
 // Stable scatter: wave w of a tile owns a quarter of its keys and walks them 64 at a time; lanes of one digit find each other by ballots.
-__global__ __launch_bounds__(256) void embed_scatter_kernel(const int64_t* __restrict__ ids, const uint32_t* __restrict__ keys,
-                                                            const uint32_t* __restrict__ vals, int64_t vocab, int64_t n, int shift,
-                                                            const uint32_t* __restrict__ hist, const uint32_t* __restrict__ total, int tiles, int scanned,
-                                                            uint32_t* __restrict__ keys_out, uint32_t* __restrict__ vals_out) {
+__global__ __launch_bounds__(256) void embed_scatter_kernel(const Jobs jobs, int64_t n, int shift, int tiles, int scanned) {
+  const Job& job = jobs.j[blockIdx.z];
+  if (pass_done(job, shift)) return;
+  const int to = (shift / 8) & 1;
+  const uint32_t *keys = job.keys[to ^ 1], *vals = job.vals[to ^ 1], *hist = job.hist;
+  uint32_t *keys_out = job.keys[to], *vals_out = job.vals[to];
   __shared__ uint32_t at[4][256];                            // next position of each digit, per wave
   __shared__ uint32_t part[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -172,7 +207,7 @@ __global__ __launch_bounds__(256) void embed_scatter_kernel(const int64_t* __res
   {
     uint32_t v = 0, mine = 0;                                 // this digit's keys in all tiles, in earlier tiles
     if (scanned) {
-      v = total[tid];
+      v = job.total[tid];
       mine = hist[(int64_t)tid * tiles + blockIdx.x];
     } else {
 #pragma unroll 8
@@ -196,7 +231,7 @@ __global__ __launch_bounds__(256) void embed_scatter_kernel(const int64_t* __res
   const int64_t first = (int64_t)blockIdx.x * RT + wave * PW;
   for (int i = 0; i < PW; i += 64) {
     const int64_t t = first + i + lane;
-    if (t < n) atomicAdd(&at[wave][((ids ? key_of(ids[t], vocab) : keys[t]) >> shift) & 255u], 1u);
+    if (t < n) atomicAdd(&at[wave][((shift == 0 ? key_of(job, t) : keys[t]) >> shift) & 255u], 1u);
   }
   __syncthreads();
   {   // counts -> starts
@@ -212,8 +247,8 @@ __global__ __launch_bounds__(256) void embed_scatter_kernel(const int64_t* __res
   for (int i = 0; i < PW; i += 64) {
     const int64_t t = first + i + lane;
     const bool in = t < n;
-    const uint32_t key = in ? (ids ? key_of(ids[t], vocab) : keys[t]) : 0u;
-    const uint32_t val = in ? (vals ? vals[t] : (uint32_t)t) : 0u;
+    const uint32_t key = in ? (shift == 0 ? key_of(job, t) : keys[t]) : 0u;
+    const uint32_t val = in ? (shift == 0 ? (uint32_t)t : vals[t]) : 0u;
     const uint32_t d = (key >> shift) & 255u;
     uint64_t same = __ballot(in);
 #pragma unroll
@@ -237,11 +272,16 @@ __global__ __launch_bounds__(256) void embed_scatter_kernel(const int64_t* __res
 // ---- sums ------------------------------------------------------------------------------------------------------------------------------
 // One wave per chunk of `chunk` <= 64 sorted positions and block of 64 * VEC columns.  Runs of one id that begin and end inside the chunk go straight
 // to their table row; one that came in from the chunk before leaves its sum in part[2 c], one that goes on into the next in part[2 c + 1].
-// first / end: the sorted positions of each row's tokens (the rows kernel's map).
+// span: the rows kernel's map.
 template <typename DT, typename TT, int VEC>
-__global__ __launch_bounds__(256) void embed_runs_kernel(const uint32_t* __restrict__ keys, const uint32_t* __restrict__ vals, int n, uint32_t vocab,
-                                                         const DT* __restrict__ dout, int64_t ld, int dim, float scale, float* __restrict__ part,
-                                                         int* __restrict__ first, int* __restrict__ end, TT* __restrict__ dtable, int chunk) {
+__global__ __launch_bounds__(256) void embed_runs_kernel(const Jobs jobs, int n, const DT* __restrict__ dout, int64_t ld, int dim, int chunk) {
+  const Job& job = jobs.j[blockIdx.z];
+  const uint32_t* __restrict__ keys = job.keys[job.sorted];
+  const uint32_t* __restrict__ vals = job.vals[job.sorted];
+  const uint32_t vocab = (uint32_t)job.vocab;
+  const float scale = job.scale;
+  float* __restrict__ part = job.part;
+  TT* __restrict__ dtable = (TT*)job.dtable;
   const int lane = threadIdx.x & 63;
   const int64_t c = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t p0 = c * chunk;
@@ -253,9 +293,9 @@ __global__ __launch_bounds__(256) void embed_runs_kernel(const uint32_t* __restr
   const uint32_t next = p0 + m < n ? keys[p0 + m] : 0xFFFFFFFFu;                              // first key of the next chunk
   const uint64_t starts = __ballot(lane < m && key != left);
   if (blockIdx.y == 0 && lane < m && key < vocab) {
-    if (key != left) first[key] = (int)(p0 + lane);
+    if (key != left) job.span[2 * (int64_t)key] = (int)(p0 + lane);
     const uint32_t right = lane + 1 < m ? keys[p0 + lane + 1] : next;
-    if (key != right) end[key] = (int)(p0 + lane + 1);
+    if (key != right) job.span[2 * (int64_t)key + 1] = (int)(p0 + lane + 1);
   }
   const bool in = !(starts & 1ull);                            // the chunk's first run came in from the chunk before
   const bool out = p0 + m < n && __builtin_amdgcn_readlane(key, m - 1) == __builtin_amdgcn_readfirstlane(next);
@@ -286,7 +326,7 @@ __global__ __launch_bounds__(256) void embed_runs_kernel(const uint32_t* __restr
     Vec<DT, VEC> x[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (j0 + u < m && live) x[u] = load_vec<DT, VEC>(dout + (int64_t)__builtin_amdgcn_readlane(val, j0 + u) * ld + d);
+      x[u] = load_vec<DT, VEC>(dout + (int64_t)__builtin_amdgcn_readlane(val, j0 + u < m ? j0 + u : m - 1) * ld + (live ? d : 0));
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (j0 + u < m) {
@@ -298,50 +338,57 @@ __global__ __launch_bounds__(256) void embed_runs_kernel(const uint32_t* __restr
   flush(m);
 }
 
-// The rows the runs kernel has not written: zeros where no token asked for the row, the sum of the parts where its run crosses chunks.  R rows per
-// workgroup; up to SHORT parts one wave sums them, more are taken by the four waves in consecutive shares that meet in LDS in order.
+// The rows the runs kernel has not written: zeros where no token asked for the row, the sum of the parts where its run crosses chunks.  ROWS rows
+// per workgroup (the long case 2 / 4 / 8 / 16 of them: 42 / 39 / 43 / 52 us: launches against the few longest runs, which are neighbours); up to SHORT
+// parts one wave sums them, more are taken by the four waves in consecutive shares that meet in LDS in order.
 constexpr int ROWS = 4, SHORT = 8;
 template <typename TT, int VEC>
-__global__ __launch_bounds__(256) void embed_rows_kernel(const int* __restrict__ first, const int* __restrict__ end, int64_t vocab, int dim, float scale,
-                                                         const float* __restrict__ part, TT* __restrict__ dtable, int chunk) {
+__global__ __launch_bounds__(256) void embed_rows_kernel(const Jobs jobs, int dim, int chunk, int blocks1) {
   __shared__ float sums[4][64 * VEC];
+  const int which = (int)blockIdx.x < blocks1;                 // the second table's (fewer and longer) rows first
+  const Job& job = jobs.j[which];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t v0 = (int64_t)blockIdx.x * ROWS;
+  const int64_t v0 = (int64_t)(blockIdx.x - (which ? 0 : blocks1)) * ROWS, vocab = job.vocab;
+  const float scale = job.scale;
+  const float* __restrict__ part = job.part;
+  TT* __restrict__ dtable = (TT*)job.dtable;
   const int nr = (int)(vocab - v0 < ROWS ? vocab - v0 : ROWS);
   const int d = (blockIdx.y * 64 + lane) * VEC;
   const bool live = d < dim;
-  // parts of a row: part[2 ca + 1], then part[2 c] of the chunks ca + 1 .. cb
-  auto add = [&](float (&acc)[VEC], int ca, int i0, int i1) {
-#pragma unroll 8
-    for (int i = i0; i < i1; ++i)
-      if (live) {
-        const Vec<float, VEC> x = load_vec<float, VEC>(part + (i ? 2 * (int64_t)(ca + i) : 2 * (int64_t)ca + 1) * dim + d);
+  // parts of a row: part[2 ca + 1], then part[2 c] of the chunks ca + 1 .. cb; U loads under way (the last one again past the end, not added)
+  auto add = [&](auto U, float (&acc)[VEC], int ca, int i0, int i1) {
+    const float* p = part + 2 * (int64_t)ca * dim + (live ? d : 0);
+    for (int i = i0; i < i1; i += U) {
+      Vec<float, VEC> x[U];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) acc[e] += x.v[e];
+      for (int u = 0; u < U; ++u) {
+        const int k = i + u < i1 ? i + u : i1 - 1;
+        x[u] = load_vec<float, VEC>(p + (k ? 2 * (int64_t)k : 1) * dim);
       }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[e] += i + u < i1 ? x[u].v[e] : 0.0f;
+    }
   };
-  int a[ROWS], np[ROWS];
-#pragma unroll
-  for (int r = 0; r < ROWS; ++r) {
-    a[r] = r < nr ? __builtin_amdgcn_readfirstlane(first[v0 + r]) : 0;
-    const int b = r < nr && a[r] >= 0 ? __builtin_amdgcn_readfirstlane(end[v0 + r]) : 0;
-    np[r] = r < nr && a[r] >= 0 ? (b - 1) / chunk - a[r] / chunk + 1 : 0;         // 0: no token; 1: written already
-  }
-#pragma unroll
-  for (int r = 0; r < ROWS; ++r) {
+  const int2 at = lane < nr ? ((const int2*)job.span)[v0 + lane] : make_int2(-1, 0);
+  const int av = at.x;
+  const int npv = av >= 0 ? (at.y - 1) / chunk - av / chunk + 1 : 0;               // 0: no token; 1: written already
+  for (int r = 0; r < nr; ++r) {
+    const int a = __builtin_amdgcn_readlane(av, r), np = __builtin_amdgcn_readlane(npv, r);
     float acc[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) acc[e] = 0.0f;
     TT* row = dtable + (v0 + r) * dim + d;
-    if (np[r] <= SHORT) {
-      if (r < nr && r % 4 == wave && np[r] != 1) {
-        add(acc, a[r] / chunk, 0, np[r]);
+    if (np <= SHORT) {
+      if (r % 4 == wave && np != 1) {
+        add(std::integral_constant<int, 2>{}, acc, a / chunk, 0, np);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) acc[e] *= scale;
         if (live) store_vec<TT, VEC>(row, acc);
       }
     } else {
-      add(acc, a[r] / chunk, (int)((int64_t)np[r] * wave / 4), (int)((int64_t)np[r] * (wave + 1) / 4));
+      add(std::integral_constant<int, 8>{}, acc, a / chunk, (int)((int64_t)np * wave / 4), (int)((int64_t)np * (wave + 1) / 4));
 #pragma unroll
       for (int e = 0; e < VEC; ++e) sums[wave][lane * VEC + e] = acc[e];
       __syncthreads();
@@ -358,35 +405,95 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const int* __restrict__
   }
 }
 
-struct Layout {      // the workspace: two (keys, vals) pairs, first / end of every row, the radix counters, the parts
-  int64_t pair, tiles, rows, hist, part, bytes;
+// The workspace of `count` tables: for each two (keys, vals) pairs, the span of every row, the radix counters, the parts.
+struct Layout {
+  int64_t n, tiles, bytes;
   int chunk;
   bool rank;
-  Layout(int64_t n, int64_t vocab, int dim) {
-    auto up = [](int64_t b) { return (b + 15) / 16 * 16; };
+  Jobs jobs;
+  Layout(int64_t n_, int dim, int count, const int64_t (&vocab)[2], char* ws) : n(n_), bytes(0), jobs() {
     // One ranking launch against one or more radix passes of two or three: the ranking grows with n^2 (measured 17 us at 8192 tokens, 46 at 13600),
-    // a pass takes about 12 us up to 100000 tokens.
-    rank = n <= (vocab < 256 ? RANK_MAX / 2 : RANK_MAX);
-    pair = up(n * 4);
-    rows = 4 * pair;
-    hist = rows + 2 * up(vocab * 4);
+    // a pass takes 7 us up to 32768 tokens and about 15 at 100000.
+    rank = n <= (vocab[0] < 256 && (count < 2 || vocab[1] < 256) ? RANK_MAX / 2 : RANK_MAX);
     tiles = (n + RT - 1) / RT;
-    part = hist + (rank ? 0 : up((256 * tiles + 256) * 4));
-    // Sorted positions per wave: short chunks until the waves fill the chip, long ones (fewer parts to join) from there.
+    // Sorted positions per wave: short chunks until the waves fill the chip (21000 tokens: runs kernel 19 us with 64, 11 with 16), long ones, with
+    // fewer parts to join, from there.
     chunk = n < 32768 ? 16 : 64;
-    bytes = part + 2 * ((n + chunk - 1) / chunk) * dim * 4;
+    auto take = [&](int64_t b) {
+      char* p = ws + bytes;
+      bytes += (b + 15) / 16 * 16;
+      return p;
+    };
+    for (int i = 0; i < count; ++i) {
+      Job& j = jobs.j[i];
+      j.vocab = vocab[i];
+      for (int k = 0; k < 2; ++k) {
+        j.keys[k] = (uint32_t*)take(n * 4);
+        j.vals[k] = (uint32_t*)take(n * 4);
+      }
+      j.span = (int*)take(vocab[i] * 8);
+      j.hist = (uint32_t*)take(rank ? 0 : 256 * tiles * 4);
+      j.total = (uint32_t*)take(rank ? 0 : 256 * 4);
+      j.part = (float*)take(2 * ((n + chunk - 1) / chunk) * dim * 4);
+      j.sorted = rank ? 0 : (passes(vocab[i]) - 1) & 1;
+    }
+  }
+  static int passes(int64_t vocab) {                           // keys run up to vocab itself
+    int p = 1;
+    while (vocab >> (8 * p)) ++p;
+    return p;
   }
 };
 
 template <typename DT, typename TT, int VEC>
-int run_sums(const uint32_t* keys, const uint32_t* vals, int64_t n, int64_t vocab, const void* dout, int64_t ld, int dim, float scale, float* part,
-             int* first, int* end, void* dtable, int chunk, hipStream_t st) {
+int run_sums(const Layout& lay, int count, const void* dout, int64_t ld, int dim, hipStream_t st) {
   const int ncb = (dim + 64 * VEC - 1) / (64 * VEC);
-  hipLaunchKernelGGL((embed_runs_kernel<DT, TT, VEC>), dim3((unsigned)((n + 4 * chunk - 1) / (4 * chunk)), ncb), dim3(256), 0, st, keys, vals, (int)n,
-                     (uint32_t)vocab, (const DT*)dout, ld, dim, scale, part, first, end, (TT*)dtable, chunk);
-  hipLaunchKernelGGL((embed_rows_kernel<TT, VEC>), dim3((unsigned)((vocab + ROWS - 1) / ROWS), ncb), dim3(256), 0, st, first, end, vocab, dim, scale, part,
-                     (TT*)dtable, chunk);
+  const unsigned blocks0 = (unsigned)((lay.jobs.j[0].vocab + ROWS - 1) / ROWS), blocks1 = (unsigned)((lay.jobs.j[1].vocab + ROWS - 1) / ROWS);
+  hipLaunchKernelGGL((embed_runs_kernel<DT, TT, VEC>), dim3((unsigned)((lay.n + 4 * lay.chunk - 1) / (4 * lay.chunk)), ncb, count), dim3(256), 0, st,
+                     lay.jobs, (int)lay.n, (const DT*)dout, ld, dim, lay.chunk);
+  hipLaunchKernelGGL((embed_rows_kernel<TT, VEC>), dim3(blocks0 + blocks1, ncb), dim3(256), 0, st, lay.jobs, dim, lay.chunk, (int)blocks1);
   FFVC_LAUNCH_CHECK();
+  return 0;
+}
+
+int embed_bwd(const char* who, const void* dout, int dout_dtype, int64_t ld, int64_t n, int dim, int count, const int64_t* const (&ids)[2],
+              const int64_t (&vocab)[2], const float (&scale)[2], void* const (&dtable)[2], int table_dtype, void* ws, int64_t ws_bytes, hipStream_t st) {
+  FFVC_CHECK_ARG(dout && ws && n > 0 && dim > 0, "%s: bad args", who);
+  FFVC_CHECK_ARG(ffvc_dtype_ok(dout_dtype) && ffvc_dtype_ok(table_dtype), "%s: bad dtype", who);
+  FFVC_CHECK_ARG(ld >= dim, "%s: rows shorter than dim", who);
+  for (int i = 0; i < count; ++i) FFVC_CHECK_ARG(dtable[i] && vocab[i] > 0, "%s: bad args", who);
+  FFVC_CHECK_ARG(n < (1ll << 31) && vocab[0] < (1ll << 31) && vocab[1] < (1ll << 31), "%s: token count and vocabulary must stay below 2^31", who);
+  Layout lay(n, dim, count, vocab, (char*)ws);
+  FFVC_CHECK_ARG((uintptr_t)ws % 16 == 0 && ws_bytes >= lay.bytes, "%s: workspace of %lld bytes needed, got %lld", who, (long long)lay.bytes,
+                 (long long)ws_bytes);
+  auto al = [](const void* p, int dt, int64_t l) { return (uintptr_t)p % 16 == 0 && l % (16 / ffvc_dtype_size(dt)) == 0; };
+  bool vec = dim % 8 == 0 && al(dout, dout_dtype, ld);
+  int passes = 0;
+  for (int i = 0; i < count; ++i) {
+    Job& j = lay.jobs.j[i];
+    j.ids = ids[i];
+    j.scale = scale[i];
+    j.dtable = dtable[i];
+    vec = vec && al(dtable[i], table_dtype, dim);
+    passes = Layout::passes(vocab[i]) > passes ? Layout::passes(vocab[i]) : passes;
+  }
+  if (lay.rank) {
+    const int lds = (int)((n + 127) / 128 * 128 * 4 + 32 * 4);
+    static ffvc_lds_once once;
+    const int rc = once.set((const void*)embed_rank_kernel, RANK_MAX * 4 + 32 * 4);
+    if (rc) return rc;
+    hipLaunchKernelGGL(embed_rank_kernel, dim3((unsigned)((n + 31) / 32), 1, count), dim3(1024), lds, st, lay.jobs, (int)n);
+  } else {
+    const int tiles = (int)lay.tiles, scanned = tiles > 32;    // (few tiles: every workgroup adds up the counts itself, a launch less)
+    for (int shift = 0; shift < 8 * passes; shift += 8) {
+      hipLaunchKernelGGL(embed_hist_kernel, dim3(tiles, 1, count), dim3(256), 0, st, lay.jobs, n, shift, tiles);
+      if (scanned) hipLaunchKernelGGL(embed_scan_kernel, dim3(256, 1, count), dim3(256), 0, st, lay.jobs, shift, tiles);
+      hipLaunchKernelGGL(embed_scatter_kernel, dim3(tiles, 1, count), dim3(256), 0, st, lay.jobs, n, shift, tiles, scanned);
+    }
+  }
+  DISPATCH_DT(dout_dtype, DT, DISPATCH_DT(table_dtype, TT, {
+    return vec ? run_sums<DT, TT, 8>(lay, count, dout, ld, dim, st) : run_sums<DT, TT, 1>(lay, count, dout, ld, dim, st);
+  }));
   return 0;
 }
 
@@ -415,54 +522,24 @@ extern "C" int ffvc_embed_fwd(const void* table, int table_dtype, int64_t ld, in
 }
 
 extern "C" int64_t ffvc_embed_bwd_ws_bytes(int64_t n, int64_t vocab, int dim) {
-  return n > 0 && vocab > 0 && dim > 0 ? Layout(n, vocab, dim).bytes : 0;
+  return n > 0 && vocab > 0 && dim > 0 ? Layout(n, dim, 1, {vocab, 0}, nullptr).bytes : 0;
 }
 
 extern "C" int ffvc_embed_bwd(const void* dout, int dout_dtype, int64_t ld, const int64_t* ids, int64_t n, int64_t vocab, int dim, float scale,
                               void* dtable, int table_dtype, void* ws, int64_t ws_bytes, void* stream) {
-  FFVC_CHECK_ARG(dout && ids && dtable && ws && n > 0 && dim > 0 && vocab > 0, "ffvc_embed_bwd: bad args");
-  FFVC_CHECK_ARG(ffvc_dtype_ok(dout_dtype) && ffvc_dtype_ok(table_dtype), "ffvc_embed_bwd: bad dtype");
-  FFVC_CHECK_ARG(ld >= dim, "ffvc_embed_bwd: rows shorter than dim");
-  FFVC_CHECK_ARG(n < (1ll << 31) && vocab < (1ll << 31), "ffvc_embed_bwd: token count and vocabulary must stay below 2^31");
-  const Layout lay(n, vocab, dim);
-  FFVC_CHECK_ARG((uintptr_t)ws % 16 == 0 && ws_bytes >= lay.bytes, "ffvc_embed_bwd: workspace of %lld bytes needed, got %lld", (long long)lay.bytes,
-                 (long long)ws_bytes);
-  hipStream_t st = (hipStream_t)stream;
-  char* w = (char*)ws;
-  uint32_t* keys[2] = {(uint32_t*)w, (uint32_t*)(w + 2 * lay.pair)};
-  uint32_t* vals[2] = {(uint32_t*)(w + lay.pair), (uint32_t*)(w + 3 * lay.pair)};
-  int* row_first = (int*)(w + lay.rows);
-  int* row_end = (int*)(w + lay.rows + (lay.hist - lay.rows) / 2);
-  int cur = 0;
-  if (lay.rank) {
-    const int lds = (int)((n + 127) / 128 * 128 * 4 + 32 * 4);
-    static ffvc_lds_once once;
-    const int rc = once.set((const void*)embed_rank_kernel, RANK_MAX * 4 + 32 * 4);
-    if (rc) return rc;
-    hipLaunchKernelGGL(embed_rank_kernel, dim3((unsigned)((n + 31) / 32)), dim3(1024), lds, st, ids, vocab, (int)n, keys[0], vals[0], row_first);
-  } else {
-    uint32_t* hist = (uint32_t*)(w + lay.hist);
-    uint32_t* total = hist + 256 * lay.tiles;
-    const int tiles = (int)lay.tiles;
-    bool first = true;
-    for (int shift = 0; shift == 0 || (shift < 32 && (vocab >> shift) != 0); shift += 8) {
-      const int64_t* src = first ? ids : nullptr;
-      const int nx = first ? 0 : cur ^ 1;
-      hipLaunchKernelGGL(embed_hist_kernel, dim3(tiles), dim3(256), 0, st, src, keys[cur], vocab, n, shift, hist, tiles, first ? row_first : nullptr);
-      const int scanned = tiles > 32;                          // (few tiles: every workgroup adds up the counts itself, a launch less)
-      if (scanned) hipLaunchKernelGGL(embed_scan_kernel, dim3(256), dim3(256), 0, st, hist, total, tiles);
-      hipLaunchKernelGGL(embed_scatter_kernel, dim3(tiles), dim3(256), 0, st, src, keys[cur], first ? nullptr : vals[cur], vocab, n, shift, hist, total,
-                         tiles, scanned, keys[nx], vals[nx]);
-      cur = nx;
-      first = false;
-    }
-  }
-  auto al = [](const void* p, int dt, int64_t l) { return (uintptr_t)p % 16 == 0 && l % (16 / ffvc_dtype_size(dt)) == 0; };
-  const bool vec = dim % 8 == 0 && al(dout, dout_dtype, ld) && al(dtable, table_dtype, dim);
-  float* part = (float*)(w + lay.part);
-  DISPATCH_DT(dout_dtype, DT, DISPATCH_DT(table_dtype, TT, {
-    return vec ? run_sums<DT, TT, 8>(keys[cur], vals[cur], n, vocab, dout, ld, dim, scale, part, row_first, row_end, dtable, lay.chunk, st)
-               : run_sums<DT, TT, 1>(keys[cur], vals[cur], n, vocab, dout, ld, dim, scale, part, row_first, row_end, dtable, lay.chunk, st);
-  }));
-  return 0;
+  FFVC_CHECK_ARG(ids, "ffvc_embed_bwd: bad args");
+  return embed_bwd("ffvc_embed_bwd", dout, dout_dtype, ld, n, dim, 1, {ids, nullptr}, {vocab, 0}, {scale, 0.0f}, {dtable, nullptr}, table_dtype, ws, ws_bytes,
+                   (hipStream_t)stream);
+}
+
+extern "C" int64_t ffvc_embed_bwd_pair_ws_bytes(int64_t n, int64_t vocab, int64_t npos, int dim) {
+  return n > 0 && vocab > 0 && npos > 0 && dim > 0 ? Layout(n, dim, 2, {vocab, npos}, nullptr).bytes : 0;
+}
+
+extern "C" int ffvc_embed_bwd_pair(const void* dout, int dout_dtype, int64_t ld, const int64_t* ids, int64_t n, int64_t vocab, int dim, float scale,
+                                   void* dtable, const int64_t* place, int64_t npos, void* dpos, int table_dtype, void* ws, int64_t ws_bytes,
+                                   void* stream) {
+  FFVC_CHECK_ARG(ids, "ffvc_embed_bwd_pair: bad args");
+  return embed_bwd("ffvc_embed_bwd_pair", dout, dout_dtype, ld, n, dim, 2, {ids, place}, {vocab, npos}, {scale, 1.0f}, {dtable, dpos}, table_dtype, ws,
+                   ws_bytes, (hipStream_t)stream);
 }

@@ -1634,8 +1634,10 @@ def embed_fwd(ids, table, scale=1.0, pos=None, pos_ids=None, out_dtype=None):
     return out
 
 
-def embed_bwd(dout, ids, rows, scale=1.0, out_dtype=None):
-    """The gradient of a table of `rows` rows that was read with `ids`: scale * sum of the tokens' dout rows, every row written."""
+def embed_bwd(dout, ids, rows, scale=1.0, out_dtype=None, pos_rows=None, pos_ids=None):
+    """The gradient of a table of `rows` rows that was read with `ids`: scale * sum of the tokens' dout rows, every row written.
+
+    With pos_rows: (that, the gradient of the position table of pos_rows rows, read with pos_ids or row t for token t), in the same launches."""
     _ids("embed_bwd", ids)
     dim = dout.shape[-1]
     if tuple(dout.shape[:-1]) != tuple(ids.shape):
@@ -1643,16 +1645,28 @@ def embed_bwd(dout, ids, rows, scale=1.0, out_dtype=None):
     d2 = dout.reshape(-1, dim)
     ld = _rows2d("embed_bwd: dout", d2)
     n = ids.numel()
-    with _same_device(dout, ids):
+    if pos_ids is not None:
+        if pos_rows is None:
+            raise ValueError("embed_bwd: pos_ids without pos_rows")
+        _ids("embed_bwd: pos_ids", pos_ids, n)
+    with _same_device(dout, ids, pos_ids):
         dt = out_dtype or dout.dtype
-        if n == 0 or rows == 0 or dim == 0:
-            return torch.zeros(rows, dim, dtype=dt, device=dout.device)
-        grad = torch.empty(rows, dim, dtype=dt, device=dout.device)
-        nb = int(_lib.load().ffvc_embed_bwd_ws_bytes(n, rows, dim))
-        ws = torch.empty(nb, dtype=torch.uint8, device=dout.device)
-        _call("ffvc_embed_bwd", d2.data_ptr(), dtype_code(d2.dtype), ld, ids.data_ptr(), n, rows, dim, scale, grad.data_ptr(), dtype_code(dt),
-              ws.data_ptr(), nb, _stream_of(dout))
-    return grad
+        if n and dim and pos_rows is not None and (rows < 1 or pos_rows < 1):
+            raise ValueError("embed_bwd: empty table")
+        make = torch.empty if n and dim and rows else torch.zeros
+        grad = make(rows, dim, dtype=dt, device=dout.device)
+        dpos = None if pos_rows is None else make(pos_rows, dim, dtype=dt, device=dout.device)
+        if make is torch.empty:
+            lib, code = _lib.load(), dtype_code(dt)
+            nb = int(lib.ffvc_embed_bwd_ws_bytes(n, rows, dim) if dpos is None else lib.ffvc_embed_bwd_pair_ws_bytes(n, rows, pos_rows, dim))
+            ws = torch.empty(nb, dtype=torch.uint8, device=dout.device)
+            head = (d2.data_ptr(), dtype_code(d2.dtype), ld, ids.data_ptr(), n, rows, dim, scale, grad.data_ptr())
+            tail = (code, ws.data_ptr(), nb, _stream_of(dout))
+            if dpos is None:
+                _call("ffvc_embed_bwd", *head, *tail)
+            else:
+                _call("ffvc_embed_bwd_pair", *head, _ptr(pos_ids), pos_rows, dpos.data_ptr(), *tail)
+    return grad if dpos is None else (grad, dpos)
 
 
 def _heads3d(name, t, like=None):

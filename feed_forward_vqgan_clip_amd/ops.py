@@ -1102,9 +1102,13 @@ class _EmbeddingFn(Function):
         ids, pos_ids = ctx.saved_tensors
         V, dt, P, scale = ctx.cfg
         g = _contig(g)
-        dtable = K.embed_bwd(g, ids, V, scale, dt) if ctx.needs_input_grad[0] else None
-        dpos = None
-        if P is not None and ctx.needs_input_grad[1]:
+        want_table, want_pos = ctx.needs_input_grad[0], P is not None and ctx.needs_input_grad[1]
+        dtable = dpos = None
+        if want_table and want_pos:
+            dtable, dpos = K.embed_bwd(g, ids, V, scale, dt, P, pos_ids)
+        elif want_table:
+            dtable = K.embed_bwd(g, ids, V, scale, dt)
+        elif want_pos:
             at = pos_ids if pos_ids is not None else torch.arange(ids.numel(), device=ids.device)
             dpos = K.embed_bwd(g, at.view(ids.shape), P, 1.0, dt)
         return dtable, dpos, None, None, None, None

@@ -567,6 +567,11 @@ int ffvc_embed_fwd(const void* table, int table_dtype, int64_t ld, int64_t vocab
 int64_t ffvc_embed_bwd_ws_bytes(int64_t n, int64_t vocab, int dim);
 int ffvc_embed_bwd(const void* dout, int dout_dtype, int64_t ld, const int64_t* ids, int64_t n, int64_t vocab, int dim, float scale, void* dtable,
                    int table_dtype, void* ws, int64_t ws_bytes, void* stream);
+/* Both gradients in the launches of one: dtable as above, and the position table's dpos[p] = sum_{t: place[t] = p} dout[t], [npos, dim] of dtable's
+ * dtype (place NULL: t itself). */
+int64_t ffvc_embed_bwd_pair_ws_bytes(int64_t n, int64_t vocab, int64_t npos, int dim);
+int ffvc_embed_bwd_pair(const void* dout, int dout_dtype, int64_t ld, const int64_t* ids, int64_t n, int64_t vocab, int dim, float scale, void* dtable,
+                        const int64_t* place, int64_t npos, void* dpos, int table_dtype, void* ws, int64_t ws_bytes, void* stream);
 
 /* Causal attention over packed sequences with grouped heads (cloob.py:199-200 under :510-516, one launch for prompts of any lengths).
  * Rows cu[b] .. cu[b+1]-1 are sequence b (cu: int32 [seqs + 1] on the device, ascending from 0; offsets outside [0, rows] are clamped); query i of a

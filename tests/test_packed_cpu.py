@@ -81,6 +81,10 @@ def test_embedding_refusals():
         ops.embedding(ids, t)
     with pytest.raises(ValueError):
         K.embed_bwd(torch.zeros(4, 8), ids, 5)
+    with pytest.raises(ValueError):
+        K.embed_bwd(torch.zeros(3, 8), ids, 5, pos_ids=ids)
+    with pytest.raises(ValueError):
+        K.embed_bwd(torch.zeros(3, 8), ids, 5, pos_rows=4, pos_ids=torch.zeros(2, dtype=torch.long))
 
 
 def test_int8_refusals():
@@ -136,6 +140,13 @@ def test_c_entry_points_refuse_bad_arguments():
     for kw in (dict(dout=0), dict(dt=9), dict(ld=7), dict(ids=0), dict(n=0), dict(n=1 << 31), dict(V=0), dict(V=1 << 31), dict(grad=0), dict(ws=0),
                dict(ws=A + 4), dict(nb=need - 1)):
         assert embed_bwd(**kw) != 0, kw
+    both = lib.ffvc_embed_bwd_pair_ws_bytes(100, 5, 7, 8)
+    assert both > need and lib.ffvc_embed_bwd_pair_ws_bytes(100, 5, 0, 8) == 0
+
+    def pair(dout=A, dt=1, ld=8, ids=A, n=100, V=5, dim=8, grad=A, place=A, P=7, dpos=A, gdt=1, ws=A, nb=both):
+        return lib.ffvc_embed_bwd_pair(dout, dt, ld, ids, n, V, dim, 1.0, grad, place, P, dpos, gdt, ws, nb, None)
+    for kw in (dict(dout=0), dict(ids=0), dict(n=0), dict(V=0), dict(P=0), dict(P=1 << 31), dict(grad=0), dict(dpos=0), dict(gdt=8), dict(ws=A + 8), dict(nb=both - 1)):
+        assert pair(**kw) != 0, kw
 
     def quant(x=A, dt=0, ldx=32, q=A, ldq=32, s=A, rows=4, k=32):
         return lib.ffvc_int8_quant(x, dt, ldx, q, ldq, s, rows, k, None)

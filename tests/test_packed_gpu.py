@@ -404,6 +404,23 @@ def test_embedding_and_gradients(cuda, case):
     embed_check(V, W, ids, place, P, td, od, scale, case)
 
 
+@pytest.mark.parametrize("n, V, P, dim", [(1, 1, 1, 8), (700, 300, 77, 24), (5000, 90, 200, 8), (9000, 70000, 3, 16), (9000, 20, 9000, 40), (40000, 300, 66000, 8)])
+@pytest.mark.parametrize("places", [False, True])
+def test_embedding_both_gradients_at_once(cuda, n, V, P, dim, places):
+    """Both tables' gradients in the same launches: the bits of each on its own (the tables sort in one to three passes, or by ranks)."""
+    g = gen(n + dim)
+    ids = torch.randint(-1, V + 1, (n,), generator=g, device="cuda")
+    at = torch.randint(-2, P + 2, (n,), generator=g, device="cuda") if places else torch.arange(n, device="cuda")
+    d = randn(g, n, dim, dtype=BF)
+    dtable, dpos = K.embed_bwd(d, ids, V, 0.5, F32, P, at if places else None)
+    assert torch.equal(dtable, K.embed_bwd(d, ids, V, 0.5, F32))
+    ok = (at >= 0) & (at < P)
+    want = torch.zeros(P, dim, dtype=F64, device="cuda").index_add_(0, at[ok], d[ok].double())
+    size = torch.zeros(P, dim, dtype=F64, device="cuda").index_add_(0, at[ok], d[ok].double().abs())
+    within(dpos, want, n * E * size, "dpos")
+    assert torch.equal(dpos, K.embed_bwd(d, at, P, 1.0, F32))
+
+
 def test_embedding_shapes_strides_and_default_places(cuda):
     g = gen(60)
     embed_check(40, 64, torch.randint(0, 40, (6, 9), generator=g, device="cuda"), None, 54, F32, F32, 1.0, 61)
