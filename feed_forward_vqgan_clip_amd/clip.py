@@ -294,6 +294,8 @@ class CLIP:
         if text.dtype != torch.long:
             raise TypeError("encode_text expects int64 token ids (main.py:733 dispatches on torch.long)")
         if self.text_packed:
+            if text.dim() == 2 and text.shape[1] > self.tpos.shape[0]:
+                raise ValueError(f"encode_text: prompts of up to {text.shape[1]} tokens for a context of {self.tpos.shape[0]}")
             ids, cu = pack_tokens(text)
             return self.encode_text_packed(ids.cuda(), cu.cuda())
         return self._encode_text_padded(text)
@@ -312,7 +314,8 @@ class CLIP:
 
     def encode_text_packed(self, ids, cu_seqlens, table=None):
         """Features of prompts packed behind one another (pack_tokens): ids int64 [rows], cu_seqlens int32 [B + 1], both on the device ->
-        (B, embed_dim) fp32.  Rows behind the last prompt are ignored, a prompt without tokens gives the features of a zero row.
+        (B, embed_dim) fp32.  Rows behind the last prompt are ignored, a prompt without tokens gives the features of a zero row, tokens past the
+        tower's context get no position (the offsets stay on the device: nothing checks them).
         table: a token embedding to use instead of the checkpoint's (vocab, width) fp32; gradients flow to it (and through the frozen tower)."""
         if not self.text_packed:
             raise RuntimeError("this CLIP was built without text_packed=True")

@@ -1774,6 +1774,8 @@ def attn_packed_qkv_bwd(qkv, out, dout, lse, cu_seqlens, heads, kv_heads, scale)
         raise ValueError("attn_packed_qkv_bwd: shape mismatch")
     seqs = _packed_cu(cu_seqlens)
     with _same_device(qkv, out, dout, lse, cu_seqlens):
+        if dout.data_ptr() % 16:
+            dout = dout.clone()
         dqkv = torch.empty(T, W, dtype=qkv.dtype, device=qkv.device)
         delta = torch.empty_like(lse)
         if T:
@@ -1795,8 +1797,8 @@ def int8_quant(x):
     code = dtype_code(x.dtype)
     ld = _rows2d("int8_quant", x2)
     with _same_device(x):
-        if x2.data_ptr() % 16 or (ld * x2.element_size()) % 16:
-            x2, ld = x2.contiguous() if x2.data_ptr() % 16 == 0 else x2.clone(), K
+        if x2.data_ptr() % 16 or (ld * x2.element_size()) % 16 or ld < K:
+            x2, ld = x2.clone(memory_format=torch.contiguous_format), K
         q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
         s = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
         if x2.shape[0]:
@@ -1829,8 +1831,10 @@ def linear_int8(x, wq, ws, bias=None, act=ACT_NONE, residual=None, out_dtype=Non
     x2 = x if x.dim() == 2 else x.reshape(-1, K)
     ld = _rows2d("linear_int8: x", x2)
     M = x2.shape[0]
+    if M >= (1 << 31) - 256:
+        raise ValueError(f"linear_int8: {M} rows in one call")
     with _same_device(x, wq, ws, bias, residual):
-        if x2.data_ptr() % 16 or ld % 8:
+        if x2.data_ptr() % 16 or ld % 8 or ld < K:
             x2, ld = x2.clone(memory_format=torch.contiguous_format), K
         y = torch.empty(shape, dtype=out_dtype, device=x.device)
         g = torch.empty(shape, dtype=x.dtype, device=x.device) if want_actgrad else None

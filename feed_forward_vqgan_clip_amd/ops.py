@@ -1075,7 +1075,7 @@ def attention_packed(qkv, cu_seqlens, heads, kv_heads=None, scale=None):
     """Causal attention over sequences packed behind one another (the text tower without its padding, cloob.py:199-200,510-516).
 
     qkv: [rows, (heads + 2 * kv_heads) * dh] 16-bit, the packed projection q | k | v (kv_heads None: as many as heads; otherwise consecutive groups
-    of heads / kv_heads query heads share one key / value head); a slice of wider rows is fine.  cu_seqlens: int32 [sequences + 1] on the device,
+    of heads / kv_heads query heads share one key / value head); a slice of wider rows is fine where it starts on 16 bytes.  cu_seqlens: int32 [sequences + 1] on the device,
     rows cu[b] .. cu[b+1]-1 are sequence b; empty sequences and rows behind the last one are allowed (those come out as zeros, and so do
     their gradients).  -> [rows, heads * dh]; gradients flow to qkv."""
     kv_heads = heads if kv_heads is None else kv_heads

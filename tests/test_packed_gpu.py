@@ -307,6 +307,20 @@ def test_attention_packed_large_scores(cuda):
     assert bool(torch.isfinite(lse).all())
 
 
+def test_attention_packed_gradient_that_starts_anywhere(cuda):
+    """An incoming gradient that is a piece of a larger buffer, at an odd offset."""
+    g = gen(77)
+    lens, H, D = [5, 40, 3], 2, 24
+    qkv = randn(g, 48, 3 * H * D, dtype=HF).requires_grad_()
+    buf = randn(g, 48 * H * D + 3, dtype=HF)
+    o = ops.attention_packed(qkv, offsets(lens), H)
+    (want,) = torch.autograd.grad(o, qkv, buf[3:].view(48, H * D).clone(), retain_graph=True)
+    (got,) = torch.autograd.grad(o, qkv, buf[3:].view(48, H * D), retain_graph=True)
+    assert torch.equal(got, want)
+    (ones,) = torch.autograd.grad(o.sum(), qkv, retain_graph=True)
+    assert torch.equal(ones, torch.autograd.grad(o, qkv, torch.ones_like(o))[0])
+
+
 def test_attention_packed_other_stream_and_graph(cuda):
     g = gen(15)
     lens, H, G, D = [60, 5, 130], 4, 2, 64
@@ -515,6 +529,7 @@ INT8 = [  # rows, N, K, act, residual dtype, output
     (1, 16, 16, 0, None, None), (1, 2048, 512, 2, None, None), (3, 17, 48, 1, F32, F32), (16, 100, 1024, 0, BF, None), (16, 4096, 4080, 2, F32, F32),
     (17, 128, 128, 0, None, None), (17, 33, 144, 1, None, F32), (130, 129, 272, 2, F32, F32), (257, 512, 512, 1, BF, None), (1000, 1000, 1008, 2, None, None),
     (5000, 2055, 400, 0, None, F32), (6200, 2304, 256, 1, None, None), (8000, 1600, 768, 2, F32, F32), (70, 72, 8208, 0, None, None),
+    (8193, 2048, 80, 1, BF, None), (8256, 1930, 192, 0, F32, F32), (8257, 1928, 64, 2, None, None),
 ]
 
 
@@ -552,6 +567,10 @@ def test_linear_int8_rows_are_independent(cuda):
     odd = torch.zeros(40 * Kd + 3, dtype=HF, device="cuda")
     odd[3:] = x.reshape(-1)
     assert torch.equal(K.linear_int8(odd[3:].view(40, Kd), wq, ws), y)
+    assert torch.equal(K.linear_int8(x[:1].expand(40, Kd), wq, ws), y[:1].expand(40, N))
+    for t in (odd[3:].view(40, Kd), x[:1].expand(40, Kd), wide[:, :Kd], wide.view(-1)[5:5 + 39 * Kd].view(39, Kd)):
+        for a, b in zip(K.int8_quant(t), K.int8_quant(t.clone(memory_format=torch.contiguous_format))):
+            assert torch.equal(a, b)
     assert torch.equal(K.linear_int8(x.view(4, 10, Kd), wq, ws), y.view(4, 10, N))
     assert tuple(K.linear_int8(x[:0], wq, ws).shape) == (0, N)
     bad = x.clone()
@@ -577,3 +596,56 @@ def test_linear_int8_graph_replays(cuda):
             want = K.linear_int8(x, wq, ws, act=K.ACT_GELU)
             torch.cuda.synchronize()
             assert torch.equal(y, want)
+
+
+# ---- together --------------------------------------------------------------------------------------------------------------------
+def test_packed_operators_two_graphs_and_two_streams(cuda):
+    """Embedding, 8-bit projection and attention with their gradients: two captured graphs replayed in turn, two streams at once; the workspaces
+    belong to a call, so each gives its eager results."""
+    g = gen(400)
+    V, W, H = 600, 128, 2
+    lens = [30, 1, 0, 200, 64]
+    T, cu = sum(lens), offsets(lens)
+    table, pos = randn(g, V, W), randn(g, T, W)
+    wq, ws = K.int8_quant(randn(g, 3 * W, W, mul=W ** -0.5))
+    scale = (W // H) ** -0.5
+
+    def step(ids, do):
+        x = K.embed_fwd(ids, table, 1.0, pos, None, BF)
+        qkv = K.linear_int8(x, wq, ws)
+        o, lse = K.attn_packed_qkv_fwd(qkv, cu, H, H, scale, want_lse=True)
+        dqkv = K.attn_packed_qkv_bwd(qkv, o, do, lse, cu, H, H, scale)
+        return (x, qkv, o, dqkv, *K.embed_bwd(dqkv[:, :W].contiguous(), ids, V, 1.0, F32, T))
+
+    def inputs(seed):
+        r = gen(seed)
+        return torch.randint(0, V, (T,), generator=r, device="cuda"), randn(r, T, W, dtype=BF)
+
+    ins = [inputs(401), inputs(402)]
+    step(*ins[0])
+    graphs, outs = [], []
+    for a in ins:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(step(*a))
+        graphs.append(graph)
+    for i in range(3):
+        for a, new in zip(ins, (inputs(410 + i), inputs(420 + i))):
+            for t, n in zip(a, new):
+                t.copy_(n)
+        graphs[0].replay()
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        want = [step(*a) for a in ins]
+        torch.cuda.synchronize()
+        for got, w in zip(outs, want):
+            assert all(torch.equal(p, q) for p, q in zip(got, w))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    res = []
+    for st, a in zip(streams, ins):
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            res.append([step(*a) for _ in range(3)][-1])
+    torch.cuda.synchronize()
+    for got, w in zip(res, want):
+        assert all(torch.equal(p, q) for p, q in zip(got, w))

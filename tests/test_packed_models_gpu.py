@@ -111,6 +111,8 @@ def test_constructor_and_argument_refusals(cuda):
     with pytest.raises(TypeError):
         packed.encode_text_packed(torch.zeros(4, dtype=torch.int32, device="cuda"), torch.tensor([0, 4], dtype=torch.int32, device="cuda"))
     with pytest.raises(ValueError):
+        packed.encode_text(torch.zeros(2, packed.context_length + 1, dtype=torch.long))
+    with pytest.raises(ValueError):
         fmain.encode_text("synthetic:2", int8=True)
 
 
