@@ -96,6 +96,7 @@ __device__ __forceinline__ int8_t* q_at(int8_t* q, int64_t ldq, int64_t rows, in
 }
 
 // One wave per row; a row of up to 64 * 8 * CH values stays in registers between the two passes, longer ones are read again (from L2).
+// Bound by bytes: 16448 rows of 4096 bf16 in 45 us (202 MB, 4.5 TB/s; 56 us with a branch around each load), of 1024 in 13.
 template <typename T, int CH>
 __global__ __launch_bounds__(256) void int8_quant_kernel(const T* __restrict__ x, int64_t ldx, int8_t* __restrict__ q, int64_t ldq,
                                                          float* __restrict__ scale, int64_t rows, int K) {
@@ -109,11 +110,16 @@ __global__ __launch_bounds__(256) void int8_quant_kernel(const T* __restrict__ x
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
     const int k = (i * 64 + lane) * 8;
+    v[i] = load8(xr + (k < K ? k : 0));                       // (no branch: all loads under way at once)
+  }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[i].v[j] = 0.0f;
-    if (k < K) v[i] = load8(xr + k);
+  for (int i = 0; i < CH; ++i) {
+    const bool in = (i * 64 + lane) * 8 < K;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m = amax_with_nan(m, v[i].v[j]);
+    for (int j = 0; j < 8; ++j) {
+      v[i].v[j] = in ? v[i].v[j] : 0.0f;
+      m = amax_with_nan(m, v[i].v[j]);
+    }
   }
   for (int k = (CH * 64 + lane) * 8; k < K; k += 512) {
     const f32x8 t = load8(xr + k);
@@ -205,7 +211,10 @@ __device__ __forceinline__ void store_one(const I8Args& p, float v, int64_t m, i
 // contiguous block, three LDS slots; w keeps its rows, two steps (128 bytes, a whole cache line of each row) at a time, two slots.  LDS-DMA
 // runs two steps ahead with one barrier per step, the youngest pieces may still be under way.  Two workgroups share a CU (BM = 256: 80 KiB
 // each), so the epilogue of one, as long as its K loop where K is 1024 and an activation is due, runs under the products of the other.
-// (With 64-byte steps of plain rows every step fetched each line twice: 104 us at 16448 x 4096 x 1024.)
+// (With 64-byte steps of plain rows every step fetched each line twice: 104 us at 16384 x 4096 x 1024, 96 as it is; 86 at 16384 x 1024 x 4096.)
+// What bounds it is the stream from L2 into LDS, about 9.5 TB/s over the chip (137 GOP at 86 us are 0.8 GB): the matrix units are busy half the
+// time.  Tiles of 256 x 256, one per CU and two K steps of 128 bytes under way, move two thirds of the bytes at the same rate and cannot run an
+// epilogue beside a K loop: 73 us for 16384 x 1024 x 4096, but 119 for 16384 x 4096 x 1024; not kept.
 // 16-byte chunks are XOR-swizzled inside 256-byte lines (4 rows of x, 2 of w): the fragment reads hit every bank evenly.
 constexpr int BN = 128, BK = 64;
 
