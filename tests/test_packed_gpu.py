@@ -649,3 +649,39 @@ def test_packed_operators_two_graphs_and_two_streams(cuda):
     torch.cuda.synchronize()
     for got, w in zip(res, want):
         assert all(torch.equal(p, q) for p, q in zip(got, w))
+
+
+def test_packed_operators_past_32_bit_offsets(cuda):
+    """More than 2^31 elements per tensor: the last rows equal a call on them alone (zeros before them)."""
+    g = gen(500)
+    # attention: 1.1 million rows of 2048 columns, sequences of 64
+    H, G, D, n, last = 16, 8, 64, 64, 640
+    T = 1100032
+    qkv = torch.zeros(T, (H + 2 * G) * D, dtype=BF, device="cuda")
+    qkv[-last:] = randn(g, last, qkv.shape[1], dtype=BF)
+    assert qkv.numel() > 1 << 31
+    cu = torch.arange(0, T + 1, n, dtype=torch.int32, device="cuda")
+    part = qkv[-last:].clone()
+    o, lse = K.attn_packed_qkv_fwd(qkv, cu, H, G, 0.125, want_lse=True)
+    o2, lse2 = K.attn_packed_qkv_fwd(part, cu[:last // n + 1].clone(), H, G, 0.125, want_lse=True)
+    assert torch.equal(o[-last:], o2) and torch.equal(lse[:, -last:], lse2) and float(o[:T - last].abs().max()) == 0
+    do = torch.zeros_like(o)
+    do[-last:] = randn(g, last, H * D, dtype=BF)
+    dqkv = K.attn_packed_qkv_bwd(qkv, o, do, lse, cu, H, G, 0.125)
+    want = K.attn_packed_qkv_bwd(part, o2, do[-last:].clone(), lse2, cu[:last // n + 1].clone(), H, G, 0.125)
+    assert torch.equal(dqkv[-last:], want) and float(dqkv[:T - last].abs().max()) == 0
+    del o, do, dqkv
+    # 8-bit Linear on the same rows: x, its panels and y
+    wq, ws = K.int8_quant(randn(g, 2048, 2048, mul=0.02))
+    y = K.linear_int8(qkv, wq, ws)
+    assert torch.equal(y[-last:], K.linear_int8(part, wq, ws)) and float(y[:T - last].abs().max()) == 0
+    del y
+    # embedding: a table and a token buffer of that size
+    ids = torch.full((T,), -1, device="cuda")
+    ids[-last:] = torch.randint(T - last, T, (last,), generator=g, device="cuda")
+    out = K.embed_fwd(ids, qkv)
+    assert torch.equal(out[-last:], qkv[ids[-last:]]) and float(out[:T - last].abs().max()) == 0
+    grad = K.embed_bwd(out, ids, T)
+    small = K.embed_bwd(out[-last:].clone(), ids[-last:] - (T - last), last)
+    assert torch.allclose(grad[-last:].double(), small.double(), rtol=2.0 ** -7, atol=last * E * float(out.abs().max()))
+    assert float(grad[:T - last].abs().max()) == 0
