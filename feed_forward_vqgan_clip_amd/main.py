@@ -249,7 +249,7 @@ def clip_arch(model_type):
 
 def load_clip_model(model_type, path=None, cdt=torch.float16, fp8=False, int8=False, text_packed=False):
     """main.py:1308-1333 for the OpenAI / OpenCLIP ViT families (state_dict in clip.model.CLIP layout).
-    fp8: image-tower linears on the fp8 MFMA path (config key `clip_fp8`, BASELINE.json configs[4]).
+    fp8: image-tower linears on the fp8 MFMA path (config key `clip_fp8`).
     int8: the same linears in 8-bit integers, scales per token and channel (config key `clip_int8`); text_packed: the text tower over packed
     prompts in the compute dtype (the `encode_text` command's --packed)."""
     arch, quick = clip_arch(model_type)
