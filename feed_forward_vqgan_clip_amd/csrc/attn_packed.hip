@@ -464,12 +464,35 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_fwd_kernel(const ffvc_
 }
 
 // ---- backward: dq (and delta) ----------------------------------------------------------------------------------------------------
-template <typename L, int DP, int NW, int NST, int KB>
-__global__ __launch_bounds__(64 * NW, 2) void attn_packed_dq_kernel(const ffvc_attn_packed_desc p, int64_t slots) {
+// acc of part 0 += the other parts', in order, through [part - 1][wave][register][lane] over the stages nobody reads any more
+template <int ND, int NW, int SPLIT>
+__device__ __forceinline__ void join_parts(f32x16_t (&acc)[ND], float* mem, int wave, int part, int lane) {
+  constexpr int W = ND * 16 * 64;
+  float* join = mem + wave * W + lane;
+  __syncthreads();
+  if (part)
+#pragma unroll
+    for (int t = 0; t < ND; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) join[(part - 1) * NW * W + (t * 16 + r) * 64] = acc[t][r];
+  __syncthreads();
+  if (!part)
+#pragma unroll
+    for (int o = 0; o < SPLIT - 1; ++o)
+#pragma unroll
+      for (int t = 0; t < ND; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[t][r] += join[o * NW * W + (t * 16 + r) * 64];
+}
+
+// SPLIT = 2: twice NW waves, each NW of them take every other key tile of the same queries; the sums join in LDS at the end (run_bwd has the rule).
+template <typename L, int DP, int NW, int NST, int KB, int SPLIT>
+__global__ __launch_bounds__(64 * NW * SPLIT, 2) void attn_packed_dq_kernel(const ffvc_attn_packed_desc p, int64_t slots) {
   constexpr int BM = 32 * NW, NS = DP / 16, ND = DP / 32, TB = KB * DP * 2;
-  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem_all[];
   const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave_all = __builtin_amdgcn_readfirstlane(tid >> 6), wave = wave_all % NW, part = wave_all / NW;
+  unsigned char* smem = smem_all + part * (NST * 2 * TB);
   int64_t rank;
   int head;
   block_place(p.heads, rank, head);
@@ -479,7 +502,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_dq_kernel(const ffvc_a
   const int D = p.head_dim;
   uint16_t* dQ = (uint16_t*)p.dq + pl.row0 * p.dq_rs + head * p.dq_hs;
   if (pl.tail) {
-    if (p.zero_tail) zero_rows(dQ + q0 * p.dq_rs, p.dq_rs, D, pl.len - q0 < BM ? pl.len - q0 : BM, tid, 64 * NW);
+    if (p.zero_tail) zero_rows(dQ + q0 * p.dq_rs, p.dq_rs, D, pl.len - q0 < BM ? pl.len - q0 : BM, tid, 64 * NW * SPLIT);
     return;
   }
   const int kvh = head / (p.heads / p.kv_heads);
@@ -493,10 +516,11 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_dq_kernel(const ffvc_a
   dk.init(p.k_rs, D, wave, lane);
   dv.init(p.v_rs, D, wave, lane);
   const int64_t qend = q0 + BM < pl.len ? q0 + BM : pl.len;
-  const int nkb = (int)((qend + KB - 1) / KB);
+  const int nkb = (int)((qend + KB - 1) / KB), steps = (nkb + SPLIT - 1) / SPLIT;
   constexpr int PIECES = 2 * TileDma<DP, NW, KB>::NP;
   int slot_in = 0, slot_out = 0;                           // LDS slots filled / read next
-  auto issue = [&](int kb) {                               // (tiles past the last one fetch zeros: the counts stay the same)
+  auto issue = [&](int it) {                               // (tiles past the last one fetch zeros: the counts stay the same)
+    const int kb = it * SPLIT + part;
     const int64_t k0 = kb < nkb ? (int64_t)kb * KB : 0, live = kb < nkb ? pl.len - k0 : 0;
     unsigned char* st = smem + slot_in * 2 * TB;
     dk.issue(Kp + k0 * p.k_rs, p.k_rs, D, live, st, wave);
@@ -521,18 +545,18 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_dq_kernel(const ffvc_a
   }
   dl += other_half(dl);
   const float ls = ok ? p.lse[stat] : 0.0f;
-  if (ok && h == 0) p.delta[stat] = -dl;                   // (negative: the accumulator of dp starts from it)
+  if (ok && h == 0 && part == 0) p.delta[stat] = -dl;                   // (negative: the accumulator of dp starts from it)
   f32x16_t acc[ND];
 #pragma unroll
   for (int t = 0; t < ND; ++t) zero16(acc[t]);
 #pragma unroll 1
-  for (int kb = 0; kb < nkb; ++kb) {
+  for (int it = 0; it < steps; ++it) {
     arrive<(NST - 2) * PIECES>();
-    issue(kb + NST - 1);
+    issue(it + NST - 1);
     const unsigned char* sk = smem + slot_out * 2 * TB;
     const unsigned char* sv = sk + TB;
     slot_out = slot_out + 1 == NST ? 0 : slot_out + 1;
-    const int64_t k0 = (int64_t)kb * KB;
+    const int64_t k0 = (int64_t)(it * SPLIT + part) * KB;
     if (k0 > qw + 31 || qw >= pl.len) continue;
     const bool diag = k0 + KB - 1 > qw;
     const int lim = (int)(qi - k0);
@@ -563,6 +587,10 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_dq_kernel(const ffvc_a
     }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  if constexpr (SPLIT > 1) {
+    join_parts<ND, NW, SPLIT>(acc, (float*)smem_all, wave, part, lane);
+    if (part) return;
+  }
 #pragma unroll
   for (int t = 0; t < ND; ++t)
 #pragma unroll
@@ -755,26 +783,8 @@ __global__ __launch_bounds__(64 * NW * SPLIT, 2) void attn_packed_dkv_kernel(con
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   if constexpr (SPLIT > 1) {
-    constexpr int W = ND * 16 * 64;
-    float* join = (float*)smem_all + wave * W + lane;                    // [part - 1][wave][register][lane] over the stages nobody reads any more
-    auto add = [&](f32x16_t (&acc)[ND]) {
-      __syncthreads();
-      if (part)
-#pragma unroll
-        for (int t = 0; t < ND; ++t)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) join[(part - 1) * NW * W + (t * 16 + r) * 64] = acc[t][r];
-      __syncthreads();
-      if (!part)
-#pragma unroll
-        for (int o = 0; o < SPLIT - 1; ++o)
-#pragma unroll
-          for (int t = 0; t < ND; ++t)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[t][r] += join[o * NW * W + (t * 16 + r) * 64];
-    };
-    add(aK);
-    add(aV);
+    join_parts<ND, NW, SPLIT>(aK, (float*)smem_all, wave, part, lane);
+    join_parts<ND, NW, SPLIT>(aV, (float*)smem_all, wave, part, lane);
     if (part) return;
   }
 #pragma unroll
@@ -871,12 +881,20 @@ int run_bwd(const ffvc_attn_packed_desc& d, hipStream_t st) {
   constexpr bool VLDS = DP == 128;
   if (short_rows(d)) {
     const int64_t slots = d.rows / 32 + d.seqs + 1;
-    LAUNCH_PACKED((attn_packed_dq_kernel<L, DP, 1, 2, 32>), 2 * 2 * 32 * DP * 2, d.heads, 64);
+    LAUNCH_PACKED((attn_packed_dq_kernel<L, DP, 1, 2, 32, 1>), 2 * 2 * 32 * DP * 2, d.heads, 64);
     LAUNCH_PACKED((attn_packed_dkv_kernel<L, DP, 1, 2, 32, VLDS, 1>), dkv_lds(DP, 1, 2, 32, VLDS, 1), d.kv_heads, 64);
   } else {
     constexpr int NW = 4, NST = 2, KB = 64, QB = DP == 64 ? 64 : 32;
     const int64_t slots = d.rows / (32 * NW) + d.seqs + 1;
-    LAUNCH_PACKED((attn_packed_dq_kernel<L, DP, NW, NST, KB>), NST * 2 * KB * DP * 2, d.heads, 64 * NW);
+    // Few query tiles for the chip's places: each split over two halves of its keys, tiles of 64 queries.  Measured (1 / 2 parts), us: 560 tiles, 8 ragged
+    // sequences with 16 heads 28 / 22, 128 features 42 / 37; 288 tiles, one of 2048 rows 39 / 30, 62 / 43; but 1056 tiles, one of 8192 198 / 217,
+    // 380 / 394; 2064 tiles, 24 ragged ones 72 / 90, 128 / 157 (the halves fetch every key and value twice as often).
+    if (slots * d.heads < 768) {
+      const int64_t slots = d.rows / 64 + d.seqs + 1;
+      LAUNCH_PACKED((attn_packed_dq_kernel<L, DP, 2, 2, 32, 2>), 2 * 2 * 2 * 32 * DP * 2, d.heads, 256);
+    } else {
+      LAUNCH_PACKED((attn_packed_dq_kernel<L, DP, 4, NST, KB, 1>), NST * 2 * KB * DP * 2, d.heads, 256);
+    }
     // A key tile's walk is as long as its sequence times the group: while the tiles are few for the chip's 512 places the longest walk alone decides,
     // so it is split over the workgroup's waves.  Measured (1 / 2 / 4 parts; the last with tiles of 64 keys), us:
     //   520 tiles, 24 ragged sequences of up to 2100 rows, 64 features: 208 / 143 / 108; 128 features: 397 / 248 / 236; one sequence, 264 tiles: 1520 / 935 / 614
