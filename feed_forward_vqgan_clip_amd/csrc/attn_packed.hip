@@ -843,6 +843,14 @@ int check_tensor(const void* ptr, int64_t rs, int64_t hs, int D, const char* who
   FFVC_CHECK_ARG(rs < (1ll << 23), "%s: %s row stride too long", who, what);       // a tile of 64 rows stays below 2 GiB
   return 0;
 }
+// a tensor that is written: no element belongs to two (row, head) pairs
+int check_written(const void* ptr, int64_t rs, int64_t hs, const ffvc_attn_packed_desc& d, int heads, const char* who, const char* what) {
+  const int rc = check_tensor(ptr, rs, hs, d.head_dim, who, what);
+  if (rc) return rc;
+  FFVC_CHECK_ARG(rs >= (heads - 1) * hs + d.head_dim || hs >= (d.rows - 1) * rs + d.head_dim, "%s: rows and heads of %s overlap (strides %lld, %lld)", who,
+                 what, (long long)rs, (long long)hs);
+  return 0;
+}
 
 // one launch of KERNEL (a template-id in parentheses) over slots x HEADS workgroups
 #define LAUNCH_PACKED(KERNEL, LDS, HEADS, THREADS)                                                                                              \
@@ -922,7 +930,7 @@ extern "C" int ffvc_attn_packed_fwd(const ffvc_attn_packed_desc* dp, void* strea
   if (!rc) rc = check_tensor(d.q, d.q_rs, d.q_hs, d.head_dim, who, "q");
   if (!rc) rc = check_tensor(d.k, d.k_rs, d.k_hs, d.head_dim, who, "k");
   if (!rc) rc = check_tensor(d.v, d.v_rs, d.v_hs, d.head_dim, who, "v");
-  if (!rc) rc = check_tensor(d.out, d.o_rs, d.o_hs, d.head_dim, who, "out");
+  if (!rc) rc = check_written(d.out, d.o_rs, d.o_hs, d, d.heads, who, "out");
   if (rc) return rc;
   hipStream_t st = (hipStream_t)stream;
   if (d.head_dim <= 64) return d.dtype == FFVC_F16 ? run_fwd<f16_t, 64>(d, st) : run_fwd<uint16_t, 64>(d, st);
@@ -939,9 +947,9 @@ extern "C" int ffvc_attn_packed_bwd(const ffvc_attn_packed_desc* dp, void* strea
   if (!rc) rc = check_tensor(d.v, d.v_rs, d.v_hs, d.head_dim, who, "v");
   if (!rc) rc = check_tensor(d.out, d.o_rs, d.o_hs, d.head_dim, who, "out");
   if (!rc) rc = check_tensor(d.dout, d.do_rs, d.do_hs, d.head_dim, who, "dout");
-  if (!rc) rc = check_tensor(d.dq, d.dq_rs, d.dq_hs, d.head_dim, who, "dq");
-  if (!rc) rc = check_tensor(d.dk, d.dk_rs, d.dk_hs, d.head_dim, who, "dk");
-  if (!rc) rc = check_tensor(d.dv, d.dv_rs, d.dv_hs, d.head_dim, who, "dv");
+  if (!rc) rc = check_written(d.dq, d.dq_rs, d.dq_hs, d, d.heads, who, "dq");
+  if (!rc) rc = check_written(d.dk, d.dk_rs, d.dk_hs, d, d.kv_heads, who, "dk");
+  if (!rc) rc = check_written(d.dv, d.dv_rs, d.dv_hs, d, d.kv_heads, who, "dv");
   if (rc) return rc;
   FFVC_CHECK_ARG(d.lse && d.delta, "ffvc_attn_packed_bwd: needs the forward's lse and the delta workspace");
   hipStream_t st = (hipStream_t)stream;

@@ -122,10 +122,14 @@ def test_c_entry_points_refuse_bad_arguments():
         assert lib.ffvc_attn_packed_fwd(ctypes.byref(e), None) != 0, (field, value)
         assert lib.ffvc_attn_packed_bwd(ctypes.byref(e), None) != 0, (field, value)
         assert lib.ffvc_last_error()
-    for field, value in (("dout", 0), ("dq", A + 8), ("dk_rs", 4), ("dv_hs", 1), ("lse", 0), ("delta", 0)):
+    for field, value in (("dout", 0), ("dq", A + 8), ("dk_rs", 4), ("dv_hs", 1), ("lse", 0), ("delta", 0), ("dq_hs", 0), ("dk_rs", 64), ("dv_hs", 128)):
         e = _lib.AttnPackedDesc.from_buffer_copy(d)
         setattr(e, field, value)
         assert lib.ffvc_attn_packed_bwd(ctypes.byref(e), None) != 0, (field, value)
+    for field, value in (("o_hs", 0), ("o_hs", 128), ("o_rs", 64)):                                # written rows and heads that overlap
+        e = _lib.AttnPackedDesc.from_buffer_copy(d)
+        setattr(e, field, value)
+        assert lib.ffvc_attn_packed_fwd(ctypes.byref(e), None) != 0, (field, value)
     assert lib.ffvc_attn_packed_fwd(None, None) != 0 and lib.ffvc_attn_packed_bwd(None, None) != 0
 
     def embed_fwd(table=A, dt=1, ld=8, V=5, ids=A, pos=0, pld=0, npos=0, out=A, odt=1, ldo=8, n=3, dim=8):
