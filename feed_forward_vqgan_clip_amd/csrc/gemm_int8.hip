@@ -435,64 +435,55 @@ __global__ __launch_bounds__(256, 2) void gemm_int8_kernel(const I8Args p, int t
   }
 }
 
-// ---- up to 64 rows of quantised x ----------------------------------------------------------------------------------------------------------
-// A workgroup owns 32 output columns, its eight waves take pairs of K panels (a 128-byte line of every weight row) in turn, operands straight
-// from global memory (a lane reads the 16 bytes of its row that its MFMA needs); the partial sums meet in LDS, exactly.  For small calls, and
-// for the last up to 64 rows of large ones: as a row of nearly empty tiles those walk the whole K loop alone once everything else is done.
-constexpr int SKINNY_M = 64;
+// ---- few outputs ------------------------------------------------------------------------------------------------------------------------------
+// A workgroup owns 16 rows x 16 columns, its eight waves take pairs of K panels (a 128-byte line of every weight row) in turn, operands straight
+// from global memory (a lane reads the 16 bytes of its row that its MFMA needs); the partial sums meet in LDS, exactly.  Where tiles would be few
+// they walk K alone, one after the other's latency: 64 x 1024 x 4096 takes 19.3 us in tiles, 4.9 here (22 with 64 x 32 outputs per workgroup: it is
+// bound by the loads a CU can have under way, so by the CUs that it reaches).
+// Measured, us in tiles / here: 256 x 2048 x 512 6.6 / 5.9, 384 x 2048 x 512 6.6 / 7.5, 128 x 4096 x 1024 8.7 / 8.5, 192 x 4096 x 1024 8.8 / 11.1,
+// 384 x 1024 x 4096 20.1 / 18.4: up to eight workgroups per CU.
+inline bool few_outputs(int64_t M, int64_t N) { return (M + 15) / 16 * ((N + 15) / 16) <= 2048; }
+
 template <typename L, typename YT>
 __global__ __launch_bounds__(512) void gemm_int8_skinny_kernel(const I8Args p) {
-  __shared__ int part[8][32][64];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, h = lane >> 5;
-  const int n0 = blockIdx.x * 32;
-  const int8_t* wr = p.w + (int64_t)(n0 + l31 < p.N ? n0 + l31 : p.N - 1) * p.ldw;
-  const bool in0 = l31 < p.M, in1 = 32 + l31 < p.M, two = p.M > 32;
-  const int8_t* x0 = p.x + (in0 ? l31 : 0) * 64 + 16 * h;
-  const int8_t* x1 = p.x + (in1 ? 32 + l31 : 0) * 64 + 16 * h;
+  __shared__ int part[8][4][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l15 = lane & 15, q = lane >> 4;
+  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16;
+  const int8_t* wr = p.w + (int64_t)(n0 + l15 < p.N ? n0 + l15 : p.N - 1) * p.ldw;
+  const int8_t* xr = p.x + (m0 + l15 < p.M ? m0 + l15 : p.M - 1) * 64;      // (rows past the last give outputs that nobody stores)
   const int64_t panel = p.xrows * 64;
-  i32x16_t acc[2];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) acc[0][i] = acc[1][i] = 0;
+  i32x4_t acc = {0, 0, 0, 0};
   const u32x4_t z = {0u, 0u, 0u, 0u};
-#pragma unroll 2
+#pragma unroll 4
   for (int k0 = wave * 128; k0 < p.K; k0 += 1024) {
-    u32x4_t a[4], b0[4], b1[4];
+    u32x4_t a[2], b[2];
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const int kk = k0 + 32 * s + 16 * h;                   // K % 16 == 0: a 16-byte chunk is inside or outside
-      const bool in = kk < p.K;
-      const int64_t at = (k0 / 64 + s / 2) * panel + 32 * (s & 1);
-      a[s] = in ? *(const u32x4_t*)(wr + kk) : z;
-      b0[s] = in && in0 ? *(const u32x4_t*)(x0 + at) : z;
-      b1[s] = in && in1 ? *(const u32x4_t*)(x1 + at) : z;
+    for (int s = 0; s < 2; ++s) {
+      const int kk = k0 + 64 * s + 16 * q, kc = kk < p.K ? kk : k0;         // K % 16 == 0: a 16-byte chunk is inside or outside (then zeros of w)
+      a[s] = *(const u32x4_t*)(wr + kc);
+      b[s] = *(const u32x4_t*)(xr + (kc >> 6) * panel + (kc & 63));
     }
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      acc[0] = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4_t, a[s]), __builtin_bit_cast(i32x4_t, b0[s]), acc[0], 0, 0, 0);
-      if (two) acc[1] = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4_t, a[s]), __builtin_bit_cast(i32x4_t, b1[s]), acc[1], 0, 0, 0);
-    }
+    for (int s = 0; s < 2; ++s)
+      acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, k0 + 64 * s + 16 * q < p.K ? a[s] : z), __builtin_bit_cast(i32x4_t, b[s]), acc, 0, 0, 0);
   }
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    part[wave][i][lane] = acc[0][i];
-    part[wave][16 + i][lane] = acc[1][i];
-  }
+  for (int i = 0; i < 4; ++i) part[wave][i][lane] = acc[i];
   __syncthreads();
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int x = tid + 512 * j, col = x & 31, m = x >> 5;   // consecutive lanes -> consecutive columns
-    // where the product's (column, row) sits: register 8 q + 4 h + e of the column's block, lane 32 h + row
-    const int reg = 16 * (m >> 5) + 4 * (col >> 3) + (col & 3), ln = 32 * ((col >> 2) & 1) + (m & 31);
+  if (tid < 256) {
+    const int col = tid & 15, row = tid >> 4;                 // consecutive lanes -> consecutive columns
+    const int reg = col & 3, ln = 16 * (col >> 2) + row;      // where the product's (column, row) sits
     int sum = 0;
 #pragma unroll
     for (int w = 0; w < 8; ++w) sum += part[w][reg][ln];
+    const int m = m0 + row;
     if (m < p.M && n0 + col < p.N) store_one<L, YT>(p, (float)sum * p.xs[m], m, n0 + col);
   }
 }
 
 template <typename L, typename YT>
 int launch_skinny(const I8Args& p, hipStream_t st) {
-  hipLaunchKernelGGL((gemm_int8_skinny_kernel<L, YT>), dim3(ceil_div(p.N, 32)), dim3(512), 0, st, p);
+  hipLaunchKernelGGL((gemm_int8_skinny_kernel<L, YT>), dim3(ceil_div(p.N, 16), ceil_div(p.M, 16)), dim3(512), 0, st, p);
   FFVC_LAUNCH_CHECK();
   return 0;
 }
@@ -513,14 +504,14 @@ int launch_tile(const I8Args& p, hipStream_t st) {
 
 template <typename L, typename YT, int ACT>
 int launch_gemm(const I8Args& p, hipStream_t st) {
-  if (p.M <= SKINNY_M) return launch_skinny<L, YT>(p, st);
+  if (few_outputs(p.M, p.N)) return launch_skinny<L, YT>(p, st);
   // 256-row tiles from one per CU on (2056 x 4096 x 1024, 256 whole tiles: 19.3 against 22.8 us with 128 rows; 4617 x 512 x 2048, 72 tiles: 20.6
-  // against 13.5).  Up to 64 rows past the last whole tile go to the skinny kernel where the whole tiles fill the chip's two places per CU
-  // (16448 x 4096 x 1024: 103 against 108 us); with fewer they run beside the others anyway.
+  // against 13.5).  Up to 64 rows past the last whole tile go to the kernel above where the whole tiles fill the chip's two places per CU (16448 x
+  // 4096 x 1024: 100 against 108 us; but 224 rows of 12000 x 2048 x 1024 45 against 38); with fewer they run beside the others anyway.
   const int64_t whole = (int64_t)(p.M / 256) * ceil_div(p.N, BN);
   if (whole < 256) return launch_tile<L, YT, ACT, 128>(p, st);
   const int rest = p.M % 256;
-  if (rest == 0 || rest > SKINNY_M || whole < 512) return launch_tile<L, YT, ACT, 256>(p, st);
+  if (rest == 0 || rest > 64 || !few_outputs(rest, p.N) || whole < 512) return launch_tile<L, YT, ACT, 256>(p, st);
   I8Args head = p, tail = p;
   head.M = p.M - rest;
   const int64_t m = head.M;

@@ -530,6 +530,7 @@ INT8 = [  # rows, N, K, act, residual dtype, output
     (17, 128, 128, 0, None, None), (17, 33, 144, 1, None, F32), (130, 129, 272, 2, F32, F32), (257, 512, 512, 1, BF, None), (1000, 1000, 1008, 2, None, None),
     (5000, 2055, 400, 0, None, F32), (6200, 2304, 256, 1, None, None), (8000, 1600, 768, 2, F32, F32), (70, 72, 8208, 0, None, None),
     (8193, 2048, 80, 1, BF, None), (8256, 1930, 192, 0, F32, F32), (8257, 1928, 64, 2, None, None),
+    (8392, 2600, 96, 2, None, F32), (600, 2055, 400, 1, F32, None), (300, 1000, 2064, 2, BF, None), (4000, 16, 208, 0, None, None),
 ]
 
 
