@@ -326,6 +326,8 @@ __device__ __forceinline__ void redo_out(const uint16_t* Q, int64_t q_rs, const 
 // ---- forward -------------------------------------------------------------------------------------------------------------------
 // NW waves x 32 queries; key / value tiles of KB = 64 rows in a ring of NST LDS slots, filled by LDS-DMA NST - 1 tiles ahead.  Every variant takes a
 // row's keys 64 at a time in the same steps, so a sequence's output does not depend on what it is packed with.
+// Bound by the softmax arithmetic beside the matrix instructions at two (128 features) or three waves per SIMD: 8192 rows, 16 heads of 128, 320 us
+// (860 TFLOP/s of visible pairs); two sequences of 16000, 32 heads, 4.2 ms (985); of 64 features 200 us (690).
 template <typename L, int DP, int NW, int NST, int KB>
 __global__ __launch_bounds__(64 * NW, 2) void attn_packed_fwd_kernel(const ffvc_attn_packed_desc p, int64_t slots) {
   constexpr int BM = 32 * NW, NS = DP / 16, ND = DP / 32, TB = KB * DP * 2;
@@ -485,6 +487,7 @@ __device__ __forceinline__ void join_parts(f32x16_t (&acc)[ND], float* mem, int 
         for (int r = 0; r < 16; ++r) acc[t][r] += join[o * NW * W + (t * 16 + r) * 64];
 }
 
+// The forward's walk once more with three products per tile (s, dp, dq): 8192 rows, 16 heads of 128, 395 us (1040 TFLOP/s); of 64 features 200 us.
 // SPLIT = 2: twice NW waves, each NW of them take every other key tile of the same queries; the sums join in LDS at the end (run_bwd has the rule).
 template <typename L, int DP, int NW, int NST, int KB, int SPLIT>
 __global__ __launch_bounds__(64 * NW * SPLIT, 2) void attn_packed_dq_kernel(const ffvc_attn_packed_desc p, int64_t slots) {
@@ -625,7 +628,7 @@ __global__ __launch_bounds__(64 * NW * SPLIT, 2) void attn_packed_dq_kernel(cons
 // (8192 rows, 16 heads of 128: 963 us with V in registers, 560 in LDS) and a step takes 32 queries, not 64.
 //
 // SPLIT > 1: SPLIT * NW waves, each NW of them take every SPLIT-th (head, query tile) of the same keys; the sums join in LDS at the end, in order.
-// (run_bwd has the rule and its figures.)
+// (run_bwd has the rule and its figures.)  Four products per tile: 8192 rows, 16 heads of 128, 565 us (970 TFLOP/s).
 template <typename L, int DP, int NW, int NST, int QB, bool VLDS, int SPLIT>
 __global__ __launch_bounds__(64 * NW * SPLIT, 2) void attn_packed_dkv_kernel(const ffvc_attn_packed_desc p, int64_t slots) {
   constexpr int BM = 32 * NW, NS = DP / 16, ND = DP / 32, TB = QB * DP * 2, VB = VLDS ? BM * DP * 2 : 0;
@@ -864,12 +867,14 @@ int check_written(const void* ptr, int64_t rs, int64_t hs, const ffvc_attn_packe
     FFVC_LAUNCH_CHECK();                                                                                                                        \
   } while (0)
 
-// Short sequences (64 rows or fewer on average): one wave per workgroup, so that a prompt does not pay for rows it has not.
-inline bool short_rows(const ffvc_attn_packed_desc& d) { return d.rows <= 64 * (int64_t)d.seqs; }
+// Short sequences on average: one wave per workgroup, so that a prompt does not pay for rows it has not.  Forward, four waves / one, us, 256 sequences with
+// 8 heads, of 20 / 48 / 64 / 100 / 128 rows: 20 / 9.7, 28 / 17, 26 / 20, 37 / 32, 62 / 36 with 64 features; 26 / 18, 32 / 31, 35 / 35, 53 / 66, 89 / 68 with 128 (and
+// 128 of 200 rows 38 / 36, 56 / 69).  A long sequence among short ones costs little: one of 4096 rows and 63 of 10, 74 / 79 and 105 / 115.
+inline bool short_rows(const ffvc_attn_packed_desc& d, int rows) { return d.rows <= rows * (int64_t)d.seqs; }
 
 template <typename L, int DP>
 int run_fwd(const ffvc_attn_packed_desc& d, hipStream_t st) {
-  if (short_rows(d)) {
+  if (short_rows(d, DP == 64 ? 128 : 64)) {
     const int64_t slots = d.rows / 32 + d.seqs + 1;
     LAUNCH_PACKED((attn_packed_fwd_kernel<L, DP, 1, 1, 64>), 2 * 64 * DP * 2, d.heads, 64);
   } else {
@@ -887,7 +892,7 @@ constexpr int dkv_lds(int DP, int NW, int NST, int QB, bool VLDS, int SPLIT) {
 template <typename L, int DP>
 int run_bwd(const ffvc_attn_packed_desc& d, hipStream_t st) {
   constexpr bool VLDS = DP == 128;
-  if (short_rows(d)) {
+  if (short_rows(d, 64)) {
     const int64_t slots = d.rows / 32 + d.seqs + 1;
     LAUNCH_PACKED((attn_packed_dq_kernel<L, DP, 1, 2, 32, 1>), 2 * 2 * 32 * DP * 2, d.heads, 64);
     LAUNCH_PACKED((attn_packed_dkv_kernel<L, DP, 1, 2, 32, VLDS, 1>), dkv_lds(DP, 1, 2, 32, VLDS, 1), d.kv_heads, 64);

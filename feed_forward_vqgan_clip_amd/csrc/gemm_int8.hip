@@ -528,7 +528,9 @@ int launch_gemm(const I8Args& p, hipStream_t st) {
 // ---- a handful of rows ---------------------------------------------------------------------------------------------------------------------
 // M <= 16 rows in ONE launch: every workgroup quantises the rows itself (a few KiB out of L2) and owns 16 output columns; its four waves
 // split K.  v_mfma_i32_16x16x64_i8: A = 16 weight rows straight from global memory, B = the quantised rows from LDS.
-constexpr int FEW_M = 16;
+// Against quantisation and the kernel above, us on the device: 1 x 2048 x 512 4.3 / 5.1, 16 x 2048 x 512 7.9 / 5.4, 16 x 4096 x 1024 10.8 / 6.6, 4 x 1024 x 4080
+// 11.6 / 10.4, 16 x 1024 x 4080 31 / 11.5.  A launch less is worth 4 us to a caller: up to 16384 elements of x.
+constexpr int FEW_M = 16, FEW_MK = 16384;
 
 template <typename L, typename YT>
 __global__ __launch_bounds__(256) void linear_int8_few_kernel(const L* __restrict__ x, const I8Args p) {
@@ -581,9 +583,6 @@ __global__ __launch_bounds__(256) void linear_int8_few_kernel(const L* __restric
 template <typename L, typename YT>
 int launch_few(const void* x, const I8Args& p, hipStream_t st) {
   const int lds = p.M * (p.K + 16) + FEW_M * 4 + 4 * 4 * 64 * 4;
-  static ffvc_lds_once once;
-  const int rc = once.set((const void*)linear_int8_few_kernel<L, YT>, 160 * 1024);
-  if (rc) return rc;
   hipLaunchKernelGGL((linear_int8_few_kernel<L, YT>), dim3(ceil_div(p.N, 16)), dim3(256), lds, st, (const L*)x, p);
   FFVC_LAUNCH_CHECK();
   return 0;
@@ -651,7 +650,7 @@ extern "C" int ffvc_gemm_int8(const int8_t* x, const float* xs, const int8_t* w,
 }
 
 extern "C" int ffvc_linear_int8_few_ok(int M, int K) {
-  return M >= 1 && M <= FEW_M && K >= 16 && K % 16 == 0 && (int64_t)M * (K + 16) <= 64 * 1024;
+  return M >= 1 && M <= FEW_M && K >= 16 && K % 16 == 0 && (int64_t)M * K <= FEW_MK;
 }
 
 extern "C" int ffvc_linear_int8_few(const void* x, int lo_dtype, int64_t ldx, const int8_t* w, int64_t ldw, const float* ws, const float* bias, int act,

@@ -608,7 +608,7 @@ int ffvc_attn_packed_bwd(const ffvc_attn_packed_desc* d, void* stream);
  * ldq: bytes between the rows of q, or 0 for K panels: [ceil(K / 64)][rows][64], the last panel filled up with zeros — the layout in which
  * ffvc_gemm_int8 takes x (M rows per panel); w keeps plain rows of ldw bytes.  The integer sum is exact.  A row with an inf or NaN gets a NaN scale.  act: NONE | GELU | QUICKGELU; actgrad (may be NULL): contiguous
  * [M, N] of lo_dtype <- act'(pre-activation); y / residual fp32 or lo_dtype; K a multiple of 16 up to 131072, any M and N.
- * ffvc_linear_int8_few: the same for up to 16 rows straight from 16-bit x, quantised inside the launch (ffvc_linear_int8_few_ok). */
+ * ffvc_linear_int8_few: the same for up to 16 rows and 16384 elements of 16-bit x, quantised inside the launch (ffvc_linear_int8_few_ok). */
 int ffvc_int8_quant(const void* x, int x_dtype, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t rows, int K, void* stream);
 int ffvc_gemm_int8(const int8_t* x, const float* xs, const int8_t* w, int64_t ldw, const float* ws, const float* bias, int act,
                    const void* residual, int res_dtype, int64_t ldr, void* y, int y_dtype, int64_t ldy, void* actgrad, int lo_dtype, int M, int N, int K,
