@@ -734,8 +734,9 @@ __global__ __launch_bounds__(64 * NW * SPLIT, 2) void attn_packed_dkv_kernel(con
     advance(head_o, qb_o, SPLIT);
     if (SPLIT > 1 && it * SPLIT + part >= total) continue;
     if (r0 + QB - 1 < kw || kw >= pl.len) continue;          // every query of the tile is earlier than this wave's keys
-    const bool diag = r0 < kw + 31;
     const int lim = (int)(ki - r0);                           // first query of the tile that sees this lane's key
+    const int end = (int)(pl.len - r0 < QB ? pl.len - r0 : QB);       // rows past the sequence are zeros: against a key with an inf they would give NaN
+    const bool edge = r0 < kw + 31 || end < QB;
 #pragma unroll
     for (int qt = 0; qt < QB / 32; ++qt) {
       if (r0 + 32 * qt + 31 < kw) continue;                  // a half of earlier queries only
@@ -765,10 +766,11 @@ __global__ __launch_bounds__(64 * NW * SPLIT, 2) void attn_packed_dkv_kernel(con
           dP[r] *= S[r];                                      // ds / scale
         }
       }
-      if (diag) {
+      if (edge) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const bool see = 32 * qt + acc_row(r, h) >= lim;
+          const int i = 32 * qt + acc_row(r, h);
+          const bool see = i >= lim && i < end;
           S[r] = see ? S[r] : 0.0f;
           dP[r] = see ? dP[r] : 0.0f;
         }
