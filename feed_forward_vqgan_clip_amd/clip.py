@@ -314,7 +314,7 @@ class CLIP:
 
     def encode_text_packed(self, ids, cu_seqlens, table=None):
         """Features of prompts packed behind one another (pack_tokens): ids int64 [rows], cu_seqlens int32 [B + 1], both on the device ->
-        (B, embed_dim) fp32.  Rows behind the last prompt are ignored, a prompt without tokens gives the features of a zero row, tokens past the
+        (B, embed_dim) fp32.  Rows before the first and behind the last prompt are ignored, a prompt without tokens gives the features of a zero row, tokens past the
         tower's context get no position (the offsets stay on the device: nothing checks them).
         table: a token embedding to use instead of the checkpoint's (vocab, width) fp32; gradients flow to it (and through the frozen tower)."""
         if not self.text_packed:
@@ -325,9 +325,9 @@ class CLIP:
         first, end = cu_seqlens[:-1].long(), cu_seqlens[1:].long()
         row = torch.arange(ids.numel(), device=ids.device)
         seq = torch.searchsorted(end, row, right=True)                              # the prompt of a row; B behind the last one
-        behind = seq >= first.numel()
-        place = torch.where(behind, -1, row - first[seq.clamp(max=first.numel() - 1)])
-        x = ops.embedding(torch.where(behind, -1, ids), self.tok_emb if table is None else table, pos=self.tpos, pos_ids=place, out_dtype=f32)
+        outside = (seq >= first.numel()) | (row < first[0])
+        place = torch.where(outside, -1, row - first[seq.clamp(max=first.numel() - 1)])
+        x = ops.embedding(torch.where(outside, -1, ids), self.tok_emb if table is None else table, pos=self.tpos, pos_ids=place, out_dtype=f32)
         for blk in self.pblocks:
             x = blk(x, self.text_heads, self.cdt, True, cu_seqlens)
         eot = ops.embedding(torch.where(end > first, end - 1, -1), x)               # the rows the features are read at

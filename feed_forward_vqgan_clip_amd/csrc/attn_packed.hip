@@ -6,10 +6,11 @@
 //     dv_j = sum_i p_ij do_i      dp_ij = do_i . v_j      delta_i = do_i . o_i      ds_ij = scale p_ij (dp_ij - delta_i)
 //     dq_i = sum_j ds_ij k_j      dk_j = sum_i ds_ij q_i  (over the heads / kv_heads query heads that share key head j's group)
 //
-// Work is cut without knowing the lengths on the host: with tiles of BM rows, sequence b owns the tile slots from
-// cu[b] / BM + b on.  Consecutive sequences never overlap (floor((c + l) / BM) + 1 - floor(c / BM) >= ceil(l / BM)), so the grid is
-// rows / BM + seqs + 1 slots and a workgroup finds its sequence by a search over the slot starts; a slot past its sequence's last tile has
-// nothing to do.  The rows behind the last sequence are a pseudo-sequence of their own (zero-filled on request, otherwise left alone).
+// Work is cut without knowing the lengths on the host.  The offsets with 0 put before and `rows` behind them bound seqs + 2 pieces: the rows before the
+// first sequence, the sequences, the rows behind the last one.  With tiles of BM rows the piece that starts at row c and has i pieces before it owns the
+// tile slots from c / BM + i on.  Consecutive pieces never overlap (floor((c + l) / BM) + 1 - floor(c / BM) >= ceil(l / BM)), so the grid is
+// rows / BM + seqs + 2 slots and a workgroup finds its piece by a search over the slot starts; a slot past its piece's last tile has
+// nothing to do.  Rows of no sequence are zero-filled on request, otherwise left alone.
 // Offsets into a tensor are 64 bits wide; inside a tile the buffer descriptor's 32-bit offsets are enough, its record count ends with the
 // sequence, so rows past the end (and features past head_dim) read as zeros without a branch.
 #include <type_traits>
@@ -126,7 +127,7 @@ struct Place {
   int64_t row0;      // first row of the sequence
   int64_t len;       // its rows
   int64_t tile;      // tile inside the sequence
-  bool tail;         // the rows behind the last sequence
+  bool outside;      // rows of no sequence: before the first or behind the last one
 };
 
 __device__ __forceinline__ int64_t cu_at(const int32_t* cu, int b, int64_t rows) {
@@ -134,15 +135,15 @@ __device__ __forceinline__ int64_t cu_at(const int32_t* cu, int b, int64_t rows)
   return c < 0 ? 0 : (c > rows ? rows : c);
 }
 
-// slot -> (sequence, tile).  64 probes at a time; a cu that is not ascending gives some sequence's clamped rows, never one outside [0, rows).
+// slot -> (piece, tile).  64 probes at a time; a cu that is not ascending gives some sequence's clamped rows, never one outside [0, rows).
 template <int BM>
 __device__ __forceinline__ Place find_slot(const int32_t* __restrict__ cu, int seqs, int64_t rows, int64_t slot) {
   const int lane = threadIdx.x & 63;
-  int lo = 0, n = seqs + 1;                       // candidates lo .. lo + n - 1; sequence `seqs` is the tail
+  int lo = 0, n = seqs + 2;                       // candidates lo .. lo + n - 1; piece i is sequence i - 1
   while (n > 1) {
     const int step = (n + 63) / 64;
     const int b = lo + lane * step;
-    const bool le = lane * step < n && cu_at(cu, b, rows) / BM + b <= slot;
+    const bool le = lane * step < n && (b ? cu_at(cu, b - 1, rows) : 0) / BM + b <= slot;
     const uint64_t m = __ballot(le) | 1ull;       // (candidate lo always holds)
     const int k = 63 - __builtin_clzll(m);
     lo += k * step;
@@ -150,11 +151,11 @@ __device__ __forceinline__ Place find_slot(const int32_t* __restrict__ cu, int s
   }
   lo = __builtin_amdgcn_readfirstlane(lo);
   Place p;
-  p.row0 = cu_at(cu, lo, rows);
-  const int64_t end = lo < seqs ? cu_at(cu, lo + 1, rows) : rows;
+  p.row0 = lo ? cu_at(cu, lo - 1, rows) : 0;
+  const int64_t end = lo <= seqs ? cu_at(cu, lo, rows) : rows;
   p.len = end > p.row0 ? end - p.row0 : 0;
   p.tile = slot - (p.row0 / BM + lo);
-  p.tail = lo == seqs;
+  p.outside = lo == 0 || lo > seqs;
   return p;
 }
 
@@ -175,11 +176,15 @@ __device__ __forceinline__ Place find_tile(const int32_t* __restrict__ cu, int s
     int cum = 0;
     for (int b = 0; b < seqs; ++b) cum += max(__builtin_amdgcn_readlane(tiles, b) - j, 0);
     const uint64_t m = __ballot(lane * step < n && cum > r);
-    if (m == 0) {                                       // behind all tiles: the rows behind the last sequence
-      p.row0 = __builtin_amdgcn_readlane(c0, seqs);
-      p.len = rows - p.row0;
+    if (m == 0) {                                       // behind all tiles: the rows behind the last sequence, then those before the first one
+      const int last = __builtin_amdgcn_readlane(c0, seqs);
+      const int64_t behind = (rows - last + BM - 1) / BM;
       p.tile = r - __builtin_amdgcn_readlane(cum, 0);
-      p.tail = true;
+      const bool head = p.tile >= behind;
+      p.row0 = head ? 0 : last;
+      p.len = head ? __builtin_amdgcn_readlane(c0, 0) : rows - last;
+      p.tile -= head ? behind : 0;
+      p.outside = true;
       return p;
     }
     const int k = 63 - __builtin_clzll(m);
@@ -194,7 +199,7 @@ __device__ __forceinline__ Place find_tile(const int32_t* __restrict__ cu, int s
   p.row0 = __builtin_amdgcn_readlane(c0, b);
   p.len = __builtin_amdgcn_readlane(c1, b) - p.row0;
   p.tile = KEYS ? __builtin_amdgcn_readlane(tiles, b) - 1 - lo : lo;
-  p.tail = false;
+  p.outside = false;
   return p;
 }
 
@@ -342,7 +347,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_fwd_kernel(const ffvc_
   if (q0 < 0 || q0 >= pl.len) return;
   const int D = p.head_dim;
   uint16_t* O = (uint16_t*)p.out + pl.row0 * p.o_rs + head * p.o_hs;
-  if (pl.tail) {
+  if (pl.outside) {
     if (p.zero_tail) zero_rows(O + q0 * p.o_rs, p.o_rs, D, pl.len - q0 < BM ? pl.len - q0 : BM, tid, 64 * NW);
     return;
   }
@@ -504,7 +509,7 @@ __global__ __launch_bounds__(64 * NW * SPLIT, 2) void attn_packed_dq_kernel(cons
   if (q0 < 0 || q0 >= pl.len) return;
   const int D = p.head_dim;
   uint16_t* dQ = (uint16_t*)p.dq + pl.row0 * p.dq_rs + head * p.dq_hs;
-  if (pl.tail) {
+  if (pl.outside) {
     if (p.zero_tail) zero_rows(dQ + q0 * p.dq_rs, p.dq_rs, D, pl.len - q0 < BM ? pl.len - q0 : BM, tid, 64 * NW * SPLIT);
     return;
   }
@@ -647,7 +652,7 @@ __global__ __launch_bounds__(64 * NW * SPLIT, 2) void attn_packed_dkv_kernel(con
   const int D = p.head_dim;
   uint16_t* dK = (uint16_t*)p.dk + pl.row0 * p.dk_rs + kvh * p.dk_hs;
   uint16_t* dV = (uint16_t*)p.dv + pl.row0 * p.dv_rs + kvh * p.dv_hs;
-  if (pl.tail) {
+  if (pl.outside) {
     if (p.zero_tail) {
       const int64_t n = pl.len - k0 < BM ? pl.len - k0 : BM;
       zero_rows(dK + k0 * p.dk_rs, p.dk_rs, D, n, tid, 64 * NW * SPLIT);
@@ -877,11 +882,11 @@ inline bool short_rows(const ffvc_attn_packed_desc& d, int rows) { return d.rows
 template <typename L, int DP>
 int run_fwd(const ffvc_attn_packed_desc& d, hipStream_t st) {
   if (short_rows(d, DP == 64 ? 128 : 64)) {
-    const int64_t slots = d.rows / 32 + d.seqs + 1;
+    const int64_t slots = d.rows / 32 + d.seqs + 2;
     LAUNCH_PACKED((attn_packed_fwd_kernel<L, DP, 1, 1, 64>), 2 * 64 * DP * 2, d.heads, 64);
   } else {
     constexpr int NW = 4, NST = 2, KB = 64;
-    const int64_t slots = d.rows / (32 * NW) + d.seqs + 1;
+    const int64_t slots = d.rows / (32 * NW) + d.seqs + 2;
     LAUNCH_PACKED((attn_packed_fwd_kernel<L, DP, NW, NST, KB>), NST * 2 * KB * DP * 2, d.heads, 64 * NW);
   }
   return 0;
@@ -895,17 +900,17 @@ template <typename L, int DP>
 int run_bwd(const ffvc_attn_packed_desc& d, hipStream_t st) {
   constexpr bool VLDS = DP == 128;
   if (short_rows(d, 64)) {
-    const int64_t slots = d.rows / 32 + d.seqs + 1;
+    const int64_t slots = d.rows / 32 + d.seqs + 2;
     LAUNCH_PACKED((attn_packed_dq_kernel<L, DP, 1, 2, 32, 1>), 2 * 2 * 32 * DP * 2, d.heads, 64);
     LAUNCH_PACKED((attn_packed_dkv_kernel<L, DP, 1, 2, 32, VLDS, 1>), dkv_lds(DP, 1, 2, 32, VLDS, 1), d.kv_heads, 64);
   } else {
     constexpr int NW = 4, NST = 2, KB = 64, QB = DP == 64 ? 64 : 32;
-    const int64_t slots = d.rows / (32 * NW) + d.seqs + 1;
-    // Few query tiles for the chip's places: each split over two halves of its keys, tiles of 64 queries.  Measured (1 / 2 parts), us: 560 tiles, 8 ragged
+    const int64_t slots = d.rows / (32 * NW) + d.seqs + 2;
+    // (Tiles are counted as rows / 128 + seqs + 1 per head.)  Few query tiles for the chip's places: each split over two halves of its keys, tiles of 64 queries.  Measured (1 / 2 parts), us: 560 tiles, 8 ragged
     // sequences with 16 heads 28 / 22, 128 features 42 / 37; 288 tiles, one of 2048 rows 39 / 30, 62 / 43; but 1056 tiles, one of 8192 198 / 217,
     // 380 / 394; 2064 tiles, 24 ragged ones 72 / 90, 128 / 157 (the halves fetch every key and value twice as often).
-    if (slots * d.heads < 768) {
-      const int64_t slots = d.rows / 64 + d.seqs + 1;
+    if ((slots - 1) * d.heads < 768) {
+      const int64_t slots = d.rows / 64 + d.seqs + 2;
       LAUNCH_PACKED((attn_packed_dq_kernel<L, DP, 2, 2, 32, 2>), 2 * 2 * 2 * 32 * DP * 2, d.heads, 256);
     } else {
       LAUNCH_PACKED((attn_packed_dq_kernel<L, DP, 4, NST, KB, 1>), NST * 2 * KB * DP * 2, d.heads, 256);
@@ -915,10 +920,10 @@ int run_bwd(const ffvc_attn_packed_desc& d, hipStream_t st) {
     //   520 tiles, 24 ragged sequences of up to 2100 rows, 64 features: 208 / 143 / 108; 128 features: 397 / 248 / 236; one sequence, 264 tiles: 1520 / 935 / 614
     //   884 tiles, 40 ragged sequences: 247 / 213 / 229; 128 features: 424 / 316 / 434; 12 sequences of 2048 rows, 820 tiles: 233 / 252 / 276
     //   1056 tiles, one sequence of 8192 rows: 298 / 311 / 347; 128 features: 540 / 562 / 757
-    if (slots * d.kv_heads < 768) {
-      const int64_t slots = d.rows / 64 + d.seqs + 1;
+    if ((slots - 1) * d.kv_heads < 768) {
+      const int64_t slots = d.rows / 64 + d.seqs + 2;
       LAUNCH_PACKED((attn_packed_dkv_kernel<L, DP, 2, NST, QB, VLDS, 4>), dkv_lds(DP, 2, NST, QB, VLDS, 4), d.kv_heads, 512);
-    } else if (slots * d.kv_heads < 1024) {
+    } else if ((slots - 1) * d.kv_heads < 1024) {
       LAUNCH_PACKED((attn_packed_dkv_kernel<L, DP, 4, NST, QB, VLDS, 2>), dkv_lds(DP, 4, NST, QB, VLDS, 2), d.kv_heads, 512);
     } else {
       LAUNCH_PACKED((attn_packed_dkv_kernel<L, DP, 4, NST, QB, VLDS, 1>), dkv_lds(DP, 4, NST, QB, VLDS, 1), d.kv_heads, 256);

@@ -1703,8 +1703,8 @@ def _attn_packed_desc(q, k, v, cu, scale):
 
 def attn_packed_fwd(q, k, v, cu_seqlens, scale, out=None, want_lse=False):
     """Causal attention over packed sequences: q (rows, heads, head_dim), k / v (rows, kv_heads, head_dim), views of one projection included;
-    cu_seqlens int32 [sequences + 1] on the device -> (out (rows, heads, head_dim), lse fp32 (heads, rows) or None).  Without `out` the rows
-    behind the last sequence come as zeros; a given `out` keeps what it holds there."""
+    cu_seqlens int32 [sequences + 1] on the device -> (out (rows, heads, head_dim), lse fp32 (heads, rows) or None).  Without `out` the rows of
+    no sequence (before cu_seqlens[0], from cu_seqlens[-1] on) come as zeros; a given `out` keeps what it holds there.  lse is not written there."""
     d = _attn_packed_desc(q, k, v, cu_seqlens, scale)
     T, H, D = q.shape
     with _same_device(q, k, v, cu_seqlens, out):
@@ -1722,7 +1722,7 @@ def attn_packed_fwd(q, k, v, cu_seqlens, scale, out=None, want_lse=False):
 
 
 def attn_packed_bwd(q, k, v, out, dout, lse, cu_seqlens, scale, dq, dk, dv):
-    """Gradients of attn_packed_fwd into dq, dk, dv (views of one packed gradient included); rows behind the last sequence become zeros."""
+    """Gradients of attn_packed_fwd into dq, dk, dv (views of one packed gradient included); rows of no sequence become zeros."""
     d = _attn_packed_desc(q, k, v, cu_seqlens, scale)
     T, H, D = q.shape
     for n, t, like in (("out", out, q), ("dout", dout, q), ("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):

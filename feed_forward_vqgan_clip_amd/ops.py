@@ -1076,8 +1076,8 @@ def attention_packed(qkv, cu_seqlens, heads, kv_heads=None, scale=None):
 
     qkv: [rows, (heads + 2 * kv_heads) * dh] 16-bit, the packed projection q | k | v (kv_heads None: as many as heads; otherwise consecutive groups
     of heads / kv_heads query heads share one key / value head); a slice of wider rows is fine where it starts on 16 bytes.  cu_seqlens: int32 [sequences + 1] on the device,
-    rows cu[b] .. cu[b+1]-1 are sequence b; empty sequences and rows behind the last one are allowed (those come out as zeros, and so do
-    their gradients).  -> [rows, heads * dh]; gradients flow to qkv."""
+    ascending: rows cu[b] .. cu[b+1]-1 are sequence b; empty sequences and rows before the first or behind the last one are allowed (those rows
+    come out as zeros, and so do their gradients).  -> [rows, heads * dh]; gradients flow to qkv."""
     kv_heads = heads if kv_heads is None else kv_heads
     if qkv.dim() != 2 or heads < 1 or kv_heads < 1 or heads % kv_heads or qkv.shape[1] % (heads + 2 * kv_heads):
         raise ValueError(f"attention_packed: a [rows, (heads + 2 kv_heads) * dh] projection is expected, got {tuple(qkv.shape)} for {heads} / {kv_heads} heads")

@@ -574,10 +574,10 @@ int ffvc_embed_bwd_pair(const void* dout, int dout_dtype, int64_t ld, const int6
                         const int64_t* place, int64_t npos, void* dpos, int table_dtype, void* ws, int64_t ws_bytes, void* stream);
 
 /* Causal attention over packed sequences with grouped heads (cloob.py:199-200 under :510-516, one launch for prompts of any lengths).
- * Rows cu[b] .. cu[b+1]-1 are sequence b (cu: int32 [seqs + 1] on the device, ascending from 0; offsets outside [0, rows] are clamped); query i of a
+ * Rows cu[b] .. cu[b+1]-1 are sequence b (cu: int32 [seqs + 1] on the device, ascending; offsets outside [0, rows] are clamped); query i of a
  * sequence sees its keys 0 .. i; query heads h share key / value head h / (heads / kv_heads).  Element (row, head, feature) of a tensor sits
- * at row * ?_rs + head * ?_hs + feature: any of them may be a slice of a packed projection.  Rows behind cu[seqs]: left as they were, or
- * zeroed with zero_tail (out; dq, dk, dv).  head_dim: a multiple of 8 up to 128; strides multiples of 8, 16-byte aligned pointers; dtype
+ * at row * ?_rs + head * ?_hs + feature: any of them may be a slice of a packed projection.  Rows of no sequence (before cu[0],
+ * from cu[seqs] on): left as they were, or zeroed with zero_tail (out; dq, dk, dv); their lse and delta are not written.  head_dim: a multiple of 8 up to 128; strides multiples of 8, 16-byte aligned pointers; dtype
  * FFVC_BF16 | FFVC_F16, statistics and accumulators fp32.
  * Forward: q, k, v, out, cu; lse (may be NULL) fp32 [heads][rows] <- base-2 log-sum-exp.  Backward: also dout, dq, dk, dv, the forward's out
  * and lse, and delta: fp32 [heads][rows] scratch.  No atomics: the same bits on every call. */

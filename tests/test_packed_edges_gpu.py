@@ -2,6 +2,8 @@
 import pytest
 import torch
 
+from feed_forward_vqgan_clip_amd import clip as fclip
+from feed_forward_vqgan_clip_amd import kernels as K
 from feed_forward_vqgan_clip_amd import ops
 
 pytestmark = pytest.mark.gpu
@@ -56,3 +58,68 @@ def test_a_key_that_every_query_rejects(cuda, lens, H, G, D, dtype):
             rest = [r for r in range(T) if r < start or r >= start + n]
             assert torch.equal(dq[rest], dq2[rest]), (n, t)
         start += n
+
+
+def refill(like, value):
+    """Leave `value` in memory of this size, so that whatever a call does not write is likely to show it."""
+    t = torch.full_like(like, value)
+    torch.cuda.synchronize()
+    del t
+
+
+@pytest.mark.parametrize("first", [1, 5, 31, 32, 200, 700])
+@pytest.mark.parametrize("lens,H,G,D", [([5, 9, 30], 2, 2, 64), ([0, 7, 0], 2, 1, 64), ([300], 8, 2, 128), ([130, 90], 4, 4, 64), ([20] * 70, 2, 2, 64), ([900, 400], 48, 48, 64)])
+def test_offsets_that_begin_behind_row_0(cuda, lens, H, G, D, first):
+    """A slice of a batch's offsets: the sequences' rows as if they stood alone, zeros before the first and behind the last."""
+    n, spare = sum(lens), first % 3
+    T = first + n + spare
+    g = gen(first * 100 + n)
+    qkv, do = randn(g, T, (H + 2 * G) * D, dtype=BF), randn(g, T, H * D, dtype=BF)
+    alone = attend(qkv[first:first + n].contiguous(), offsets(lens), H, G, do[first:first + n].contiguous())
+    refill(qkv, 3.0)
+    refill(do, 3.0)
+    got = attend(qkv, offsets(lens, first), H, G, do)
+    for name, a, b in zip(("out", "dq", "dk", "dv"), got, alone):
+        assert not bool(a[:first].any()) and not bool(a[first + n:].any()), name
+        # (more rows may choose another split of the backward's sums: equal up to their rounding)
+        assert torch.equal(a[first:first + n], b) if name == "out" else torch.allclose(a[first:first + n].double(), b.double(), rtol=2.0 ** -7, atol=1e-2), name
+    # buffers that are given: forward leaves those rows alone, backward zeroes them; nothing beside the views is written
+    q, k, v = ops._split_heads(qkv, H, G)
+    buf = torch.full((T + 2, H * D + 8), 5.0, dtype=BF, device="cuda")
+    out, lse = K.attn_packed_fwd(q, k, v, offsets(lens, first), D ** -0.5, out=buf[1:-1, :H * D].unflatten(1, (H, D)), want_lse=True)
+    assert torch.equal(out[first:first + n], got[0][first:first + n])
+    keep = buf.clone()
+    keep[1 + first:1 + first + n, :H * D] = 5.0
+    assert bool((keep == 5.0).all())
+    grad = torch.full((T + 2, (H + 2 * G) * D + 8), 5.0, dtype=BF, device="cuda")
+    views = ops._split_heads(grad[1:-1, :-8], H, G)
+    K.attn_packed_bwd(q, k, v, got[0].contiguous(), do.unflatten(1, (H, D)), lse, offsets(lens, first), D ** -0.5, *views)
+    assert all(torch.equal(a, b) for a, b in zip(views, got[1:]))
+    grad[1:-1, :-8] = 5.0
+    assert bool((grad == 5.0).all())
+
+
+def test_packed_text_tower_on_a_slice_of_the_offsets(cuda):
+    """Prompts 2 .. of a batch through the whole batch's rows: their features, and no gradient for the tokens of the prompts before them."""
+    cfg = dict(embed_dim=64, image_resolution=32, vision_layers=1, vision_width=128, vision_patch_size=8, context_length=77, vocab_size=500,
+               transformer_width=128, transformer_heads=2, transformer_layers=2)
+    model = fclip.CLIP(fclip.random_state_dict(cfg, 3), HF, text_packed=True)
+    g = torch.Generator().manual_seed(2)
+    text = torch.zeros(6, 77, dtype=torch.long)
+    for i in range(6):
+        text[i, :9 + i] = torch.arange(60 * i, 60 * i + 9 + i) + 1
+        text[i, 9 + i] = 499
+    w = torch.randn(6, 64, generator=g).cuda()
+    ids, cu = fclip.pack_tokens(text)
+    ids, cu = ids.cuda(), cu.cuda()
+    table = model.tok_emb.clone().requires_grad_()
+    full = model.encode_text_packed(ids, cu, table)
+    (gf,) = torch.autograd.grad((full[2:] * w[2:]).sum(), table)
+    part = model.encode_text_packed(ids, cu[2:].clone(), table)
+    (gp,) = torch.autograd.grad((part * w[2:]).sum(), table)
+    # the same rows through the same products (the forward does not depend on company); sums of the backward may be cut differently
+    assert torch.allclose(part, full[2:], rtol=1e-5, atol=1e-6)
+    before = ids[:int(cu[2])].unique()
+    before = before[before != 499]
+    assert not bool(gp[before].any()) and bool(torch.isfinite(gp).all())
+    assert float((gp - gf).norm() / gf.norm()) < 20 * torch.finfo(HF).eps / 2
