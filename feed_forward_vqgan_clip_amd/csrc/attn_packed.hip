@@ -470,6 +470,33 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_fwd_kernel(const ffvc_
   }
 }
 
+// ---- the range of f16 in the backward -----------------------------------------------------------------------------------------------------
+// P and dS are rounded to the 16-bit type, for the matrix instructions that multiply them with 16-bit rows: one rounding per weight.  bf16 has the range
+// of fp32; in f16 a dS of 65520 is infinite and one below 2^-24 has no bits left, though the sums that it belongs to fit.  So f16 weights carry a
+// power of two, 2^F16_UP at first, per query (dq) or key (dk, dv): it enters through the exponent, or through the accumulator that the scores start
+// from, and is taken out of the sums.  A tile whose largest |f dS| passes 2^15 (|dS| > 1: loss-scaled gradients) lowers the factor and what has
+// been summed so far.  Cost, dq + dk / dv of 8192 rows with 16 heads: 516 -> 556 us with 64 features, 967 -> 993 with 128 (the maximum; the branch is
+// taken a few times per walk at most); bf16 compiles without it.
+constexpr int F16_UP = 15;
+template <typename L>
+constexpr bool IS_F16 = std::is_same<L, f16_t>::value;
+// 0, or the (negative) power by which the lane's factor has to change; the half-waves share their column
+__device__ __forceinline__ int lower_by(const f32x16_t& t) {
+  float mx = 0.0f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) mx = fmaxf(mx, fabsf(t[r]));
+  if (__builtin_expect(!__any(mx > 32768.0f), 1)) return 0;
+  mx = fmaxf(mx, other_half(mx));
+  return mx > 32768.0f && mx < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(mx) : 0;         // (an inf stays one)
+}
+template <int N>
+__device__ __forceinline__ void scale_all(f32x16_t (&t)[N], float by) {
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) t[i][r] *= by;
+}
+
 // ---- backward: dq (and delta) ----------------------------------------------------------------------------------------------------
 // acc of part 0 += the other parts', in order, through [part - 1][wave][register][lane] over the stages nobody reads any more
 template <int ND, int NW, int SPLIT>
@@ -495,7 +522,7 @@ __device__ __forceinline__ void join_parts(f32x16_t (&acc)[ND], float* mem, int 
 // The forward's walk once more with three products per tile (s, dp, dq): 8192 rows, 16 heads of 128, 395 us (1040 TFLOP/s); of 64 features 200 us.
 // SPLIT = 2: twice NW waves, each NW of them take every other key tile of the same queries; the sums join in LDS at the end (run_bwd has the rule).
 template <typename L, int DP, int NW, int NST, int KB, int SPLIT>
-__global__ __launch_bounds__(64 * NW * SPLIT, 2) void attn_packed_dq_kernel(const ffvc_attn_packed_desc p, int64_t slots) {
+__global__ __launch_bounds__(64 * NW * SPLIT, DP == 64 && SPLIT == 1 ? 3 : 2) void attn_packed_dq_kernel(const ffvc_attn_packed_desc p, int64_t slots) {
   constexpr int BM = 32 * NW, NS = DP / 16, ND = DP / 32, TB = KB * DP * 2;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem_all[];
   const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
@@ -552,7 +579,8 @@ __global__ __launch_bounds__(64 * NW * SPLIT, 2) void attn_packed_dq_kernel(cons
     for (int e = 0; e < 8; ++e) dl = fmaf(a.v[e], b.v[e], dl);
   }
   dl += other_half(dl);
-  const float ls = ok ? p.lse[stat] : 0.0f;
+  float ls = ok ? p.lse[stat] : 0.0f;
+  if constexpr (IS_F16<L>) ls -= (float)F16_UP;
   if (ok && h == 0 && part == 0) p.delta[stat] = -dl;                   // (negative: the accumulator of dp starts from it)
   f32x16_t acc[ND];
 #pragma unroll
@@ -586,6 +614,16 @@ __global__ __launch_bounds__(64 * NW * SPLIT, 2) void attn_packed_dq_kernel(cons
 #pragma unroll
         for (int r = 0; r < 16; ++r) dP[r] = 32 * kt + acc_row(r, h) > lim ? 0.0f : dP[r];
       }
+      if constexpr (IS_F16<L>) {
+        const int e = lower_by(dP);
+        if (__builtin_expect(__any(e != 0), 0)) {
+          const float by = ldexpf(1.0f, e);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) dP[r] *= by;
+          scale_all<ND>(acc, by);
+          ls -= (float)e;
+        }
+      }
 #pragma unroll
       for (int sg = 0; sg < 2; ++sg) {
         const u32x4_t fs = pack8<L>(dP, 8 * sg);
@@ -595,6 +633,7 @@ __global__ __launch_bounds__(64 * NW * SPLIT, 2) void attn_packed_dq_kernel(cons
     }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  if constexpr (IS_F16<L>) scale_all<ND>(acc, ldexpf(1.0f, (int)rintf(ls - (ok ? p.lse[stat] : 0.0f))));
   if constexpr (SPLIT > 1) {
     join_parts<ND, NW, SPLIT>(acc, (float*)smem_all, wave, part, lane);
     if (part) return;
@@ -727,6 +766,8 @@ __global__ __launch_bounds__(64 * NW * SPLIT, 2) void attn_packed_dkv_kernel(con
     zero16(aK[t]);
     zero16(aV[t]);
   }
+  const bool ranged = IS_F16<L> && c > 0x1p-100f;
+  float up = ranged ? F16_UP / c : 0.0f;                     // the scores start from `up`: the lane's factor is 2^(c up)
 #pragma unroll 1
   for (int it = 0; it < steps; ++it) {
     arrive<(NST - 2) * PIECES>();
@@ -746,7 +787,8 @@ __global__ __launch_bounds__(64 * NW * SPLIT, 2) void attn_packed_dkv_kernel(con
     for (int qt = 0; qt < QB / 32; ++qt) {
       if (r0 + 32 * qt + 31 < kw) continue;                  // a half of earlier queries only
       f32x16_t S, dP;
-      zero16(S);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) S[r] = up;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {                          // dp starts from -delta
         const f32x4_t d4 = *(const f32x4_t*)(st + 64 + 32 * qt + 8 * g + 4 * h);
@@ -780,6 +822,20 @@ __global__ __launch_bounds__(64 * NW * SPLIT, 2) void attn_packed_dkv_kernel(con
           dP[r] = see ? dP[r] : 0.0f;
         }
       }
+      if constexpr (IS_F16<L>) {
+        const int e = ranged ? lower_by(dP) : 0;
+        if (__builtin_expect(__any(e != 0), 0)) {
+          const float by = ldexpf(1.0f, e);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            S[r] *= by;
+            dP[r] *= by;
+          }
+          scale_all<ND>(aK, by);
+          scale_all<ND>(aV, by);
+          up = (rintf(up * c) + (float)e) / c;
+        }
+      }
 #pragma unroll
       for (int sg = 0; sg < 2; ++sg) {
         const u32x4_t fp = pack8<L>(S, 8 * sg), fs = pack8<L>(dP, 8 * sg);
@@ -792,6 +848,11 @@ __global__ __launch_bounds__(64 * NW * SPLIT, 2) void attn_packed_dkv_kernel(con
     }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  if constexpr (IS_F16<L>) {
+    const float undo = ldexpf(1.0f, -(int)rintf(up * c));
+    scale_all<ND>(aK, undo);
+    scale_all<ND>(aV, undo);
+  }
   if constexpr (SPLIT > 1) {
     join_parts<ND, NW, SPLIT>(aK, (float*)smem_all, wave, part, lane);
     join_parts<ND, NW, SPLIT>(aV, (float*)smem_all, wave, part, lane);

@@ -5,6 +5,7 @@ import torch
 from feed_forward_vqgan_clip_amd import clip as fclip
 from feed_forward_vqgan_clip_amd import kernels as K
 from feed_forward_vqgan_clip_amd import ops
+from test_packed_gpu import attn_reference, within
 
 pytestmark = pytest.mark.gpu
 BF, HF, F32, F64 = torch.bfloat16, torch.float16, torch.float32, torch.float64
@@ -123,3 +124,60 @@ def test_packed_text_tower_on_a_slice_of_the_offsets(cuda):
     before = before[before != 499]
     assert not bool(gp[before].any()) and bool(torch.isfinite(gp).all())
     assert float((gp - gf).norm() / gf.norm()) < 20 * torch.finfo(HF).eps / 2
+
+
+# every form of the backward: one-wave tiles; dq in halves and dk / dv in four parts; dq whole and dk / dv in two; both whole
+FORMS = [([64], 2, 2), ([30, 9, 64, 17], 4, 2), ([70, 200], 4, 2), ([900], 96, 96), ([1500], 96, 96)]
+
+
+def hold_gradients(lens, H, G, D, scale, do_size, seed, size=1.0):
+    """f16 gradients of a call with output gradients of this size, against the 64-bit formulas and their bounds (which know one rounding of dS to 11
+    bits and one of the result, and nothing of overflow or lost bits below it)."""
+    g = gen(seed)
+    T = sum(lens)
+    qkv, do = randn(g, T, (H + 2 * G) * D, dtype=HF, mul=size), randn(g, T, H * D, dtype=HF, mul=do_size).clamp(-6e4, 6e4)
+    q, k, v = ops._split_heads(qkv, H, G)
+    (o, dq, dk, dv), (bo, bq, bk, bv) = attn_reference(q, k, v, lens, scale, do.view(T, H, D))
+    leaf = qkv.clone().requires_grad_()
+    got = ops.attention_packed(leaf, offsets(lens), H, G, scale=scale)
+    within(got.view(T, H, D), o, bo, "out")
+    (d,) = torch.autograd.grad(got, leaf, do)
+    for name, a, b, c in zip(("dq", "dk", "dv"), ops._split_heads(d, H, G), (dq, dk, dv), (bq, bk, bv)):
+        fits = b.abs() < 65000                                       # (the few others, sums over a group's heads, round to an infinity)
+        within(a[fits], b[fits], c[fits], name)
+        assert float(fits.double().mean()) > 0.999
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("form", range(len(FORMS)))
+def test_f16_gradients_of_a_scaled_loss(cuda, form, D):
+    """p (dP - delta) passes 65504 although ds = scale p (dP - delta) and all three gradients fit."""
+    lens, H, G = FORMS[form]
+    hold_gradients(lens, H, G, D, 1.0 / 128, 12000.0, 70 + form)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("form", range(len(FORMS)))
+def test_f16_gradients_that_grow_along_the_walk(cuda, form, D):
+    """Output gradients of 1e-3 for most queries and of thousands for a few: the factor is lowered in the middle of a walk, for some rows and not for others."""
+    lens, H, G = FORMS[form]
+    g = gen(170 + form)
+    T, scale = sum(lens), D ** -0.5
+    qkv, do = randn(g, T, (H + 2 * G) * D, dtype=HF), randn(g, T, H * D, dtype=HF, mul=1e-3)
+    do[T // 2::7] *= 4e6
+    v = ops._split_heads(qkv, H, G)[2]
+    v[T // 3::5] *= 8
+    q, k, v = ops._split_heads(qkv, H, G)
+    (o, dq, dk, dv), (bo, bq, bk, bv) = attn_reference(q, k, v, lens, scale, do.view(T, H, D))
+    leaf = qkv.clone().requires_grad_()
+    (d,) = torch.autograd.grad(ops.attention_packed(leaf, offsets(lens), H, G), leaf, do)
+    for name, a, b, c in zip(("dq", "dk", "dv"), ops._split_heads(d, H, G), (dq, dk, dv), (bq, bk, bv)):
+        fits = b.abs() < 65000                                       # (the others round to an infinity)
+        within(a[fits], b[fits], c[fits], name)
+        assert float(fits.double().mean()) > 0.9
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_f16_gradients_of_a_mean_over_many_keys(cuda, D):
+    """Output gradients of 1e-4 over 2000 keys: dS of a few 1e-8, sums of a few 1e-6 that f16 holds to its subnormal step."""
+    hold_gradients([2000, 40], 2, 2, D, D ** -0.5, 1e-4, 270, size=0.3)
