@@ -27,6 +27,10 @@ typedef __attribute__((address_space(3))) s16x4_t* lds_tr;
 constexpr uint32_t OOB = 0xFFFFFFF0u;
 constexpr float LOG2E = 1.44269504088896341f;
 constexpr float NEG_BIG = -3.0e38f;
+// f16 weights are held times 2^F16_UP where a product reads them: below 2^-24 f16 has no bits left, and many small weights are one output
+constexpr int F16_UP = 15;
+template <typename L>
+constexpr bool IS_F16 = std::is_same<L, f16_t>::value;
 // 64 lanes x 16 (4) bytes from a bounded buffer into consecutive LDS
 __device__ __forceinline__ void dma16(rsrc_t r, uint32_t off, unsigned char* lds) { __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_vp)lds, 16, off, 0, 0, 0); }
 __device__ __forceinline__ void dma4(rsrc_t r, uint32_t off, float* lds) { __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_vp)lds, 4, off, 0, 0, 0); }
@@ -415,7 +419,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_fwd_kernel(const ffvc_
         for (int r = 0; r < 16; ++r) acc[t][r] *= a;
       m = mx;
     }
-    const float mc = m * c;
+    const float mc = IS_F16<L> ? fmaf(m, c, -(float)F16_UP) : m * c;
     float sum = 0.0f;
 #pragma unroll
     for (int kt = 0; kt < NH; ++kt)
@@ -461,7 +465,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_fwd_kernel(const ffvc_
   for (int t = 0; t < ND; ++t)
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[t][r] *= inv;
-  if (p.lse && ok && h == 0) p.lse[(int64_t)head * p.rows + pl.row0 + qi] = m * c + __builtin_amdgcn_logf(l);
+  if (p.lse && ok && h == 0) p.lse[(int64_t)head * p.rows + pl.row0 + qi] = m * c + (__builtin_amdgcn_logf(l) - (IS_F16<L> ? (float)F16_UP : 0.0f));
   store_rows<L, DP>(O + qw * p.o_rs, p.o_rs, D, acc, l31, ok, h);
   if (__any(ok && nonfinite<ND>(acc))) {
     const int64_t far = (qw / KB + 1) * KB, last = far < pl.len ? far : pl.len;       // keys past qw that its last tile holds
@@ -477,9 +481,6 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_fwd_kernel(const ffvc_
 // from, and is taken out of the sums.  A tile whose largest |f dS| passes 2^15 (|dS| > 1: loss-scaled gradients) lowers the factor and what has
 // been summed so far.  Cost, dq + dk / dv of 8192 rows with 16 heads: 516 -> 556 us with 64 features, 967 -> 993 with 128 (the maximum; the branch is
 // taken a few times per walk at most); bf16 compiles without it.
-constexpr int F16_UP = 15;
-template <typename L>
-constexpr bool IS_F16 = std::is_same<L, f16_t>::value;
 // 0, or the (negative) power by which the lane's factor has to change; the half-waves share their column
 __device__ __forceinline__ int lower_by(const f32x16_t& t) {
   float mx = 0.0f;

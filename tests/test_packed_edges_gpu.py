@@ -1,4 +1,6 @@
 """Packed-prompt operators at their edges: values, offsets, widths and gradients that the ordinary cases do not reach."""
+import math
+
 import pytest
 import torch
 
@@ -181,3 +183,23 @@ def test_f16_gradients_that_grow_along_the_walk(cuda, form, D):
 def test_f16_gradients_of_a_mean_over_many_keys(cuda, D):
     """Output gradients of 1e-4 over 2000 keys: dS of a few 1e-8, sums of a few 1e-6 that f16 holds to its subnormal step."""
     hold_gradients([2000, 40], 2, 2, D, D ** -0.5, 1e-4, 270, size=0.3)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lens", [[3000], [3000] + [2] * 60])
+def test_many_small_weights_beside_a_large_one(cuda, lens, D, dtype):
+    """3000 keys of weight 2^-26 behind one of weight 1: their sum is the output wherever the large key's value is 0."""
+    g = gen(370 + D)
+    T, scale = sum(lens), D ** -0.5
+    q, k = torch.zeros(T, 2, D, dtype=dtype, device="cuda"), torch.zeros(T, 2, D, dtype=dtype, device="cuda")
+    q[:, :, 5] = 8.0
+    k[0, :, 5] = 18.0 / (8.0 * scale)
+    v = randn(g, T, 2, D).abs().add(0.5).to(dtype)
+    v[0] = 0
+    o, lse = K.attn_packed_fwd(q, k, v, offsets(lens), scale, want_lse=True)
+    ref, bound = attn_reference(q, k, v, lens, scale)
+    assert float(ref[2000:3000].min()) > 1e-5
+    within(o, ref, bound + (2.0 ** -25 if dtype == HF else 0.0), "out")          # (half a step of a subnormal output)
+    s = (q[2999].double() * k[:3000].double()).sum(-1) * scale
+    assert float((lse[:, 2999].double() - torch.logsumexp(s, 0) / math.log(2)).abs().max()) < 2e-5   # (26 in fp32, l to n 2^-24)
