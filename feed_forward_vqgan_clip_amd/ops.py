@@ -24,7 +24,7 @@ import math
 import os
 
 import torch
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 
 from . import kernels as K
 from .kernels import ACT_GELU, ACT_NONE, ACT_QUICKGELU  # noqa: F401
@@ -1049,6 +1049,12 @@ def attention(qkv, heads, scale, causal=False, f8_for=None):
     return _AttentionFn.apply(qkv, heads, scale, causal, f8_for)
 
 
+def _plain(*tensors):
+    """No derivative of either mode is asked for: the call may do without its autograd node (46 us of host time, for kernels of a few).  Forward mode
+    counts wherever a dual level is open; the node then refuses a tangent, which a bare launch would drop."""
+    return forward_ad._current_level < 0 and not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors))
+
+
 class _AttentionPackedFn(Function):
     """Causal attention over packed sequences; keeps qkv, the output and the row statistics (no score matrix)."""
 
@@ -1085,7 +1091,7 @@ def attention_packed(qkv, cu_seqlens, heads, kv_heads=None, scale=None):
     if dh % 8 or not 8 <= dh <= 128:
         raise ValueError(f"attention_packed: head width {dh} unsupported (a multiple of 8, at most 128)")
     scale = default_scale(dh) if scale is None else float(scale)
-    if not (qkv.requires_grad and torch.is_grad_enabled()):
+    if _plain(qkv):
         return K.attn_packed_qkv_fwd(qkv, cu_seqlens, heads, kv_heads, scale)[0]
     return _AttentionPackedFn.apply(qkv, cu_seqlens, heads, kv_heads, scale)
 
@@ -1119,7 +1125,7 @@ def embedding(ids, table, scale=1.0, pos=None, pos_ids=None, out_dtype=None):
 
     ids (and pos_ids): int64; an index outside its table (e.g. -1 for the unused rows of a buffer) reads a zero row and gets no gradient.
     pos without pos_ids: row t for the t-th token.  The gradients are sums over the sorted tokens: no atomics, the same bits every time."""
-    if not (torch.is_grad_enabled() and (table.requires_grad or (pos is not None and pos.requires_grad))):
+    if _plain(table, pos):
         return K.embed_fwd(ids, table, float(scale), pos, pos_ids, out_dtype)
     return _EmbeddingFn.apply(table, pos, ids, pos_ids, float(scale), out_dtype)
 
