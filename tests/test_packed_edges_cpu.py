@@ -9,6 +9,58 @@ from feed_forward_vqgan_clip_amd import ops
 BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
 
 
+class Pack:
+    """The part of ops.Weights that the autograd nodes read, on the CPU (Weights.frozen uploads)."""
+
+    def __new__(cls, N, Kd, cdt, int8):
+        w = torch.randn(N, Kd)
+        W = ops.Weights(None, torch.zeros(N), w.to(cdt), w.t().contiguous().to(cdt))
+        if int8:
+            W.int8 = (torch.zeros(N, Kd, dtype=torch.int8), torch.ones(N))
+        return W
+
+
+@pytest.fixture
+def linear_stubs(monkeypatch):
+    """Products that return zeros of the right shape (and the residual they are given); the outputs that were allocated for them."""
+    made = []
+
+    def linear_int8(x, wq, ws, bias=None, act=0, residual=None, out_dtype=None, want_actgrad=False):
+        y = torch.zeros(*x.shape[:-1], wq.shape[0], dtype=out_dtype or x.dtype)
+        if residual is not None:
+            y += residual
+        made.append(y)
+        return (y, torch.ones_like(y)) if want_actgrad else y
+
+    def gemm(x, w, y, *a, residual=None, aux=None, **kw):
+        y.zero_()
+        if residual is not None:
+            y += residual
+        made.append(y)
+
+    monkeypatch.setattr(K, "linear_int8", linear_int8)
+    monkeypatch.setattr(K, "gemm", gemm)
+    monkeypatch.setattr(K, "cast", lambda t, dt: t.to(dt))
+    return made
+
+
+@pytest.mark.parametrize("int8", [False, True])
+def test_mlp_gradient_of_the_residual_alone(linear_stubs, int8):
+    """A frozen or detached x beside a trainable residual stream: the residual's gradient is the output's, with no product in the backward."""
+    W1, W2 = Pack(64, 32, HF, int8), Pack(32, 64, HF, int8)
+    x, res = torch.randn(5, 32).half(), torch.randn(5, 32, requires_grad=True)
+    y = ops.mlp(x, W1, W2, K.ACT_QUICKGELU, residual=res, out_dtype=F32)
+    before = len(linear_stubs)
+    dy = torch.randn(5, 32)
+    (g,) = torch.autograd.grad(y, res, dy)
+    assert torch.equal(g, dy) and len(linear_stubs) == before
+    # both, and x alone, still run their products
+    x.requires_grad_()
+    y = ops.mlp(x, W1, W2, K.ACT_QUICKGELU, residual=res, out_dtype=F32)
+    gx, g = torch.autograd.grad(y, (x, res), dy)
+    assert torch.equal(g, dy) and gx.shape == x.shape and len(linear_stubs) == before + 4
+
+
 @pytest.fixture
 def stubs(monkeypatch):
     """Launchers that return tensors of the right shape and count their calls."""

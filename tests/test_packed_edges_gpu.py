@@ -203,3 +203,17 @@ def test_many_small_weights_beside_a_large_one(cuda, lens, D, dtype):
     within(o, ref, bound + (2.0 ** -25 if dtype == HF else 0.0), "out")          # (half a step of a subnormal output)
     s = (q[2999].double() * k[:3000].double()).sum(-1) * scale
     assert float((lse[:, 2999].double() - torch.logsumexp(s, 0) / math.log(2)).abs().max()) < 2e-5   # (26 in fp32, l to n 2^-24)
+
+
+@pytest.mark.parametrize("int8", [False, True])
+def test_frozen_mlp_with_a_residual_that_alone_wants_a_gradient(cuda, int8):
+    g = gen(470)
+    W1, W2 = (ops.Weights.frozen(randn(g, n, k, mul=k ** -0.5), randn(g, n), HF, int8=int8) for n, k in ((256, 64), (64, 256)))
+    x, res, dy = randn(g, 40, 64, dtype=HF), randn(g, 40, 64).requires_grad_(), randn(g, 40, 64)
+    y = ops.mlp(x, W1, W2, K.ACT_GELU, residual=res, out_dtype=F32)
+    (gr,) = torch.autograd.grad(y, res, dy)
+    assert torch.equal(gr, dy)
+    x2 = x.clone().requires_grad_()
+    y2 = ops.mlp(x2, W1, W2, K.ACT_GELU, residual=res, out_dtype=F32)
+    gx, gr = torch.autograd.grad(y2, (x2, res), dy)
+    assert torch.equal(y2, y) and torch.equal(gr, dy) and bool(gx.any()) and bool(torch.isfinite(gx).all())
