@@ -410,16 +410,17 @@ class _LinearFn(Function):
         cdt = W.sh.dtype
         x = _contig(x)
         rows = x.numel() // W.K
-        y = torch.empty(*x.shape[:-1], W.N, dtype=out_dtype or cdt, device=x.device)
         ctx.drop = (float(drop), _drop_seeds(1)[0]) if drop else None
+        int8 = W.int8 is not None and not ctx.drop and not gn_hw and x.dtype in K.LOWP
+        y = None if int8 else torch.empty(*x.shape[:-1], W.N, dtype=out_dtype or cdt, device=x.device)
         if ctx.drop:                 # y = residual + dropout(x W^T + b)   (vitgan.py:114,133)
             K.gemm(x, W.sh, y, rows, W.N, W.K, ldx=W.K, ldw=W.K, bias=W.bias)
             if residual is not None and (residual.dtype != torch.float32 or y.dtype != torch.float32):
                 raise TypeError("linear(drop>0) with a residual needs the fp32 residual stream")
             K.dropout(y, ctx.drop[0], ctx.drop[1], residual=residual, out=y)
-        elif W.int8 is not None and not gn_hw and x.dtype in K.LOWP:
+        elif int8:
             _f8_twin(x, None)
-            y = K.linear_int8(x, *W.int8, bias=W.bias, residual=residual, out_dtype=y.dtype)
+            y = K.linear_int8(x, *W.int8, bias=W.bias, residual=residual, out_dtype=out_dtype or cdt)
         elif W.fp8 is not None and not gn_hw and x.dtype in K.LOWP:
             f = W.fp8                  # fp8 MFMA path of a frozen layer: quantise the activation, per-tensor delayed scale
             x8 = _f8_twin(x, f["x"])

@@ -61,6 +61,15 @@ def test_mlp_gradient_of_the_residual_alone(linear_stubs, int8):
     assert torch.equal(g, dy) and gx.shape == x.shape and len(linear_stubs) == before + 4
 
 
+def test_linear_with_8_bit_weights_allocates_its_output_once(linear_stubs, monkeypatch):
+    W = Pack(64, 32, HF, True)
+    sizes = []
+    empty = torch.empty
+    monkeypatch.setattr(torch, "empty", lambda *a, **kw: sizes.append(a) or empty(*a, **kw))
+    y = ops.linear(torch.randn(5, 32).half(), W, residual=torch.randn(5, 64), out_dtype=F32)
+    assert y.shape == (5, 64) and y.dtype == F32 and not sizes and len(linear_stubs) == 1
+
+
 @pytest.fixture
 def stubs(monkeypatch):
     """Launchers that return tensors of the right shape and count their calls."""
