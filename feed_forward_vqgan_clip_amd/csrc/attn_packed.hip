@@ -929,7 +929,7 @@ int check_written(const void* ptr, int64_t rs, int64_t hs, const ffvc_attn_packe
   do {                                                                                                                                          \
     static ffvc_lds_once once__;                                                                                                                \
     const int64_t blocks__ = slots * (HEADS);                                                                                                   \
-    FFVC_CHECK_ARG(blocks__ > 0 && blocks__ < (1ll << 31), "ffvc_attn_packed: too many tiles for one launch (%lld)", (long long)blocks__);      \
+    FFVC_CHECK_ARG(ffvc_launch_fits(blocks__, THREADS), "ffvc_attn_packed: too many tiles for one launch (%lld)", (long long)blocks__);         \
     const int rc__ = once__.set((const void*)KERNEL, LDS);                                                                                      \
     if (rc__) return rc__;                                                                                                                      \
     hipLaunchKernelGGL(KERNEL, dim3((unsigned)blocks__), dim3(THREADS), LDS, st, d, slots);                                                     \

@@ -39,6 +39,9 @@ void ffvc_set_error(const char* fmt, ...);
     }                                                                    \
   } while (0)
 
+// A launch takes fewer than 2^32 threads in x.
+inline bool ffvc_launch_fits(int64_t blocks, int threads) { return blocks > 0 && blocks * threads < (1ll << 32); }
+
 // The dynamic-LDS limit of one kernel, raised once per device (a static of each launcher; launchers may run on several threads).
 struct ffvc_lds_once {
   std::atomic<uint64_t> done{0};

@@ -463,6 +463,7 @@ int embed_bwd(const char* who, const void* dout, int dout_dtype, int64_t ld, int
   FFVC_CHECK_ARG(ld >= dim, "%s: rows shorter than dim", who);
   for (int i = 0; i < count; ++i) FFVC_CHECK_ARG(dtable[i] && vocab[i] > 0, "%s: bad args", who);
   FFVC_CHECK_ARG(n < (1ll << 31) && vocab[0] < (1ll << 31) && vocab[1] < (1ll << 31), "%s: token count and vocabulary must stay below 2^31", who);
+  FFVC_CHECK_ARG(ffvc_launch_fits((vocab[0] + ROWS - 1) / ROWS + (vocab[1] + ROWS - 1) / ROWS, 256), "%s: too many table rows for one launch", who);
   Layout lay(n, dim, count, vocab, (char*)ws);
   FFVC_CHECK_ARG((uintptr_t)ws % 16 == 0 && ws_bytes >= lay.bytes, "%s: workspace of %lld bytes needed, got %lld", who, (long long)lay.bytes,
                  (long long)ws_bytes);
@@ -504,7 +505,7 @@ extern "C" int ffvc_embed_fwd(const void* table, int table_dtype, int64_t ld, in
   FFVC_CHECK_ARG(table && ids && out && n > 0 && dim > 0 && vocab > 0, "ffvc_embed_fwd: bad args");
   FFVC_CHECK_ARG(ffvc_dtype_ok(table_dtype) && ffvc_dtype_ok(out_dtype), "ffvc_embed_fwd: bad dtype");
   FFVC_CHECK_ARG(ld >= dim && ldo >= dim && (!pos || (pos_ld >= dim && npos > 0)), "ffvc_embed_fwd: rows shorter than dim");
-  FFVC_CHECK_ARG((n + 3) / 4 < (1ll << 31), "ffvc_embed_fwd: too many tokens for one launch");
+  FFVC_CHECK_ARG(ffvc_launch_fits((n + 3) / 4, 256), "ffvc_embed_fwd: too many tokens for one launch (%lld, at most %lld)", (long long)n, 4 * ((1ll << 24) - 1));
   auto al = [](const void* p, int dt, int64_t l) { return (uintptr_t)p % 16 == 0 && l % (16 / ffvc_dtype_size(dt)) == 0; };
   const bool vec = dim % 8 == 0 && al(table, table_dtype, ld) && al(out, out_dtype, ldo) && (!pos || al(pos, table_dtype, pos_ld));
   const dim3 grid((unsigned)((n + 3) / 4)), block(256);

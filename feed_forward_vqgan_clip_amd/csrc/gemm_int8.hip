@@ -493,7 +493,7 @@ int launch_tile(const I8Args& p, hipStream_t st) {
   constexpr int lds = 3 * BM * BK + 2 * BN * 128;
   const int tiles_n = ceil_div(p.N, BN);
   const int64_t n_tiles = (int64_t)ceil_div(p.M, BM) * tiles_n;
-  FFVC_CHECK_ARG(n_tiles < (1ll << 31), "ffvc_gemm_int8: too many tiles for one launch");
+  FFVC_CHECK_ARG(ffvc_launch_fits(n_tiles, 256), "ffvc_gemm_int8: too many tiles for one launch");
   static ffvc_lds_once once;
   const int rc = once.set((const void*)gemm_int8_kernel<L, YT, ACT, BM>, lds);
   if (rc) return rc;
@@ -616,7 +616,7 @@ extern "C" int ffvc_int8_quant(const void* x, int x_dtype, int64_t ldx, int8_t* 
   FFVC_CHECK_ARG(ffvc_dtype_ok(x_dtype), "ffvc_int8_quant: bad dtype %d", x_dtype);
   FFVC_CHECK_ARG((uintptr_t)x % 16 == 0 && ldx % (16 / ffvc_dtype_size(x_dtype)) == 0 && ldx >= K && (uintptr_t)q % 16 == 0 && ldq % 16 == 0 && (ldq == 0 || ldq >= K),
                  "ffvc_int8_quant: rows must be 16-byte aligned");
-  FFVC_CHECK_ARG((rows + 3) / 4 < (1ll << 31), "ffvc_int8_quant: too many rows");
+  FFVC_CHECK_ARG(ffvc_launch_fits((rows + 3) / 4, 256), "ffvc_int8_quant: too many rows for one launch (%lld, at most %lld)", (long long)rows, 4 * ((1ll << 24) - 1));
   const dim3 grid((unsigned)((rows + 3) / 4)), block(256);
   hipStream_t st = (hipStream_t)stream;
   DISPATCH_DT(x_dtype, T, {

@@ -557,7 +557,7 @@ int ffvc_tokmix_bwd_hidden(const void* xn, const void* dy, const void* w1, const
  * (the causal mask of cloob.py:510-516 makes a prompt's features independent of what stands behind its last token).
  * ------------------------------------------------------------------------- */
 
-/* out[t] = scale * table[ids[t]] + pos[place[t]], t < n (cloob.py:526-528 with a scale).  table: [vocab] rows of dim, `ld` elements apart;
+/* out[t] = scale * table[ids[t]] + pos[place[t]], t < n <= 2^26 - 4 (cloob.py:526-528 with a scale).  table: [vocab] rows of dim, `ld` elements apart;
  * pos (may be NULL): npos rows of table's dtype; place (may be NULL: t itself) int64.  An id / place outside its table reads a zero row. */
 int ffvc_embed_fwd(const void* table, int table_dtype, int64_t ld, int64_t vocab, const int64_t* ids, float scale, const void* pos, int64_t pos_ld,
                    int64_t npos, const int64_t* place, void* out, int out_dtype, int64_t ldo, int64_t n, int dim, void* stream);
@@ -607,7 +607,8 @@ int ffvc_attn_packed_bwd(const ffvc_attn_packed_desc* d, void* stream);
  *   y[m, n]  = act(xs[m] * ws[n] * sum_k x[m, k] w[n, k] + bias[n]) + residual[m, n]
  * ldq: bytes between the rows of q, or 0 for K panels: [ceil(K / 64)][rows][64], the last panel filled up with zeros — the layout in which
  * ffvc_gemm_int8 takes x (M rows per panel); w keeps plain rows of ldw bytes.  The integer sum is exact.  A row with an inf or NaN gets a NaN scale.  act: NONE | GELU | QUICKGELU; actgrad (may be NULL): contiguous
- * [M, N] of lo_dtype <- act'(pre-activation); y / residual fp32 or lo_dtype; K a multiple of 16 up to 131072, any M and N.
+ * [M, N] of lo_dtype <- act'(pre-activation); y / residual fp32 or lo_dtype; K a multiple of 16 up to 131072, any N, up to
+ * 2^26 - 4 rows (a launch takes fewer than 2^32 threads; what needs more is refused).
  * ffvc_linear_int8_few: the same for up to 16 rows and 16384 elements of 16-bit x, quantised inside the launch (ffvc_linear_int8_few_ok). */
 int ffvc_int8_quant(const void* x, int x_dtype, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t rows, int K, void* stream);
 int ffvc_gemm_int8(const int8_t* x, const float* xs, const int8_t* w, int64_t ldw, const float* ws, const float* bias, int act,

@@ -1,11 +1,16 @@
 """Packed-prompt operators without a GPU: what the public entry points do around the launches, with the launchers stubbed, and more refusals."""
+import ctypes
+import os
+
 import pytest
 import torch
 from torch.autograd import forward_ad
 
+from feed_forward_vqgan_clip_amd import _lib
 from feed_forward_vqgan_clip_amd import kernels as K
 from feed_forward_vqgan_clip_amd import ops
 
+built = pytest.mark.skipif(not os.path.exists(_lib.LIB_PATH), reason="libffvc_hip.so not built (run __graft_entry__.build())")
 BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
 
 
@@ -112,3 +117,39 @@ def test_calls_without_a_gradient_make_no_node(stubs):
     with torch.no_grad():
         assert ops.attention_packed(qkv.clone().requires_grad_(), cu, 2).grad_fn is None
     assert stubs == ["attn", "embed", "attn", "embed", "attn"]
+
+
+A = 1 << 12                                                           # an aligned non-null address that nothing may touch
+
+
+def attn_desc(rows=4, seqs=1, heads=2, kv_heads=2, dim=64):
+    d = _lib.AttnPackedDesc()
+    for i, n in enumerate(("q", "k", "v", "out", "lse", "cu", "dout", "dq", "dk", "dv", "delta")):
+        setattr(d, n, A + (i << 40))
+    d.rows, d.seqs, d.heads, d.kv_heads, d.head_dim, d.dtype, d.scale = rows, seqs, heads, kv_heads, dim, _lib.BF16, 1.0
+    for n in ("q", "k", "v", "o", "do", "dq", "dk", "dv"):
+        setattr(d, n + "_rs", dim * heads)
+        setattr(d, n + "_hs", dim)
+    return d
+
+
+def refused(rc, word):
+    return rc != 0 and word in _lib.load().ffvc_last_error().decode()
+
+
+@built
+def test_launches_of_2_to_the_32_threads_are_refused():
+    """Before anything runs, and by name."""
+    lib = _lib.load()
+    n = (1 << 26) - 3
+    assert refused(lib.ffvc_embed_fwd(A, 1, 8, 5, A, 1.0, 0, 0, 0, 0, A, 1, 8, n, 8, None), "too many")
+    ws = lib.ffvc_embed_bwd_ws_bytes(100, n, 8)
+    assert refused(lib.ffvc_embed_bwd(A, 1, 8, A, 100, n, 8, 1.0, A, 1, A, ws, None), "too many")
+    half = 1 << 25
+    ws = lib.ffvc_embed_bwd_pair_ws_bytes(100, half, half, 8)
+    assert refused(lib.ffvc_embed_bwd_pair(A, 1, 8, A, 100, half, 8, 1.0, A, A, half, A, 1, A, ws, None), "too many")
+    assert refused(lib.ffvc_int8_quant(A, 0, 32, A, 32, A, n, 32, None), "too many")
+    assert refused(lib.ffvc_gemm_int8(A, A, A, 16, A, 0, 0, 0, 1, 1 << 14, A, 0, 1 << 14, 0, 0, 1 << 27, 1 << 14, 16, None), "too many")
+    for d in (attn_desc(rows=1 << 30, heads=8, kv_heads=8, dim=8), attn_desc(rows=1 << 30, seqs=1 << 29, heads=1, kv_heads=1, dim=8)):
+        assert refused(lib.ffvc_attn_packed_fwd(ctypes.byref(d), None), "too many")
+        assert refused(lib.ffvc_attn_packed_bwd(ctypes.byref(d), None), "too many")
