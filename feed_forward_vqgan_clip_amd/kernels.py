@@ -1594,13 +1594,13 @@ def _stream_of(t):
 
 
 def _rows2d(name, t):
-    """A 2-d tensor whose rows are contiguous; returns its row stride."""
+    """A 2-d tensor whose rows are contiguous; returns its row stride (a single row's is never taken: its own may be anything)."""
     if t.dim() != 2:
         raise ValueError(f"{name}: expected a 2-d tensor, got {tuple(t.shape)}")
     rows, cols = t.shape
     if cols > 1 and t.stride(1) != 1:
         raise ValueError(f"{name}: the elements of a row must be contiguous (strides {t.stride()})")
-    return t.stride(0) if rows > 1 else max(cols, t.stride(0))
+    return t.stride(0) if rows > 1 else cols
 
 
 def _ids(name, t, n=None):
@@ -1676,7 +1676,7 @@ def _heads3d(name, t, like=None):
     if t.stride(2) != 1 and t.shape[2] > 1:
         raise ValueError(f"{name}: the features of a head must be contiguous (strides {t.stride()})")
     T, H, D = t.shape
-    return (t.stride(0) if T > 1 else max(H * D, t.stride(0))), (t.stride(1) if H > 1 else D)
+    return (t.stride(0) if T > 1 else H * D), (t.stride(1) if H > 1 else D)
 
 
 def _packed_cu(cu):

@@ -217,3 +217,38 @@ def test_frozen_mlp_with_a_residual_that_alone_wants_a_gradient(cuda, int8):
     y2 = ops.mlp(x2, W1, W2, K.ACT_GELU, residual=res, out_dtype=F32)
     gx, gr = torch.autograd.grad(y2, (x2, res), dy)
     assert torch.equal(y2, y) and torch.equal(gr, dy) and bool(gx.any()) and bool(torch.isfinite(gx).all())
+
+
+def test_a_single_row_of_a_wider_buffer(cuda):
+    """One token: the row stride of its tensors is never taken, so an odd one is no reason to refuse the call."""
+    g = gen(570)
+    H, D = 2, 64
+    wide = randn(g, 1, 3 * H * D + 5, dtype=HF)
+    qkv, cu = wide[:, :3 * H * D], offsets([1])
+    assert qkv.stride(0) % 8
+    do = randn(g, 1, H * D, dtype=HF)
+    want = attend(qkv.contiguous(), cu, H, H, do)
+    leaf = wide.clone().requires_grad_()
+    o = ops.attention_packed(leaf[:, :3 * H * D], cu, H)
+    (d,) = torch.autograd.grad(o, leaf, do)
+    for a, b in zip((o.unflatten(1, (H, D)),) + ops._split_heads(d[:, :3 * H * D], H, H), want):
+        assert torch.equal(a, b)
+    assert torch.equal(K.attn_packed_qkv_fwd(qkv, cu, H, H, D ** -0.5)[0], o.detach())
+    q, k, v = ops._split_heads(qkv, H, H)
+    out = torch.zeros(1, H * D + 3, dtype=HF, device="cuda")[:, :H * D].unflatten(1, (H, D))
+    K.attn_packed_fwd(q, k, v, cu, D ** -0.5, out=out)
+    assert torch.equal(out, want[0])
+    # heads apart by more than their width as well: the single row's heads need no room of a row
+    buf = randn(g, 1, 3 * H, 2 * D, dtype=HF)
+    qq, kk, vv = (buf[:, i * H:(i + 1) * H, :D] for i in range(3))
+    o2, _ = K.attn_packed_fwd(qq, kk, vv, cu, D ** -0.5)
+    assert torch.equal(o2, K.attn_packed_fwd(qq.contiguous(), kk.contiguous(), vv.contiguous(), cu, D ** -0.5)[0])
+    # the other operators take such rows as well
+    x = randn(g, 1, 67, dtype=HF)[:, :64]
+    wq, ws = K.int8_quant(randn(g, 24, 64))
+    assert torch.equal(K.linear_int8(x, wq, ws), K.linear_int8(x.contiguous(), wq, ws))
+    assert torch.equal(K.int8_quant(x)[0], K.int8_quant(x.contiguous())[0])
+    table = randn(g, 1, 67)[:, :64]
+    ids = torch.tensor([0, 0, 1], device="cuda")
+    assert torch.equal(K.embed_fwd(ids, table), K.embed_fwd(ids, table.contiguous()))
+    assert torch.equal(K.embed_bwd(x, ids[:1], 3), K.embed_bwd(x.contiguous(), ids[:1], 3))
