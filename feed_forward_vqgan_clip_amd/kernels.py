@@ -1743,13 +1743,20 @@ def attn_packed_bwd(q, k, v, out, dout, lse, cu_seqlens, scale, dq, dk, dv):
             _call("ffvc_attn_packed_bwd", byref(d), _stream_of(q))
 
 
+def _qkv_head_dim(qkv, heads, kv_heads):
+    W = qkv.shape[1]
+    if heads < 1 or kv_heads < 1 or W % (heads + 2 * kv_heads):
+        raise ValueError(f"attn_packed: {W} columns are no projection of {heads} query and 2 x {kv_heads} key / value heads")
+    return W // (heads + 2 * kv_heads)
+
+
 def attn_packed_qkv_fwd(qkv, cu_seqlens, heads, kv_heads, scale, want_lse=False):
     """attn_packed_fwd of a packed projection [rows, (heads + 2 kv_heads) * dh] -> (out [rows, heads * dh], lse or None)."""
     if qkv.dtype not in LOWP:
         raise TypeError(f"attn_packed: 16-bit tensors only (bf16, f16), got {qkv.dtype}")
     ld = _rows2d("attn_packed: qkv", qkv)
     T, W = qkv.shape
-    D = W // (heads + 2 * kv_heads)
+    D = _qkv_head_dim(qkv, heads, kv_heads)
     seqs = _packed_cu(cu_seqlens)
     with _same_device(qkv, cu_seqlens):
         out = torch.empty(T, heads * D, dtype=qkv.dtype, device=qkv.device)
@@ -1765,11 +1772,11 @@ def attn_packed_qkv_fwd(qkv, cu_seqlens, heads, kv_heads, scale, want_lse=False)
 
 def attn_packed_qkv_bwd(qkv, out, dout, lse, cu_seqlens, heads, kv_heads, scale):
     """The gradient [rows, (heads + 2 kv_heads) * dh] of attn_packed_qkv_fwd's projection; dout contiguous like out."""
-    _req(qkv.dtype, out, dout)
-    _req_f32(lse)
     ld = _rows2d("attn_packed: qkv", qkv)
     T, W = qkv.shape
-    D = W // (heads + 2 * kv_heads)
+    D = _qkv_head_dim(qkv, heads, kv_heads)
+    _req(qkv.dtype, out, dout)
+    _req_f32(lse)
     if tuple(out.shape) != (T, heads * D) or tuple(dout.shape) != (T, heads * D) or tuple(lse.shape) != (heads, T):
         raise ValueError("attn_packed_qkv_bwd: shape mismatch")
     seqs = _packed_cu(cu_seqlens)

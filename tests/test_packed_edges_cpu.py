@@ -153,3 +153,17 @@ def test_launches_of_2_to_the_32_threads_are_refused():
     for d in (attn_desc(rows=1 << 30, heads=8, kv_heads=8, dim=8), attn_desc(rows=1 << 30, seqs=1 << 29, heads=1, kv_heads=1, dim=8)):
         assert refused(lib.ffvc_attn_packed_fwd(ctypes.byref(d), None), "too many")
         assert refused(lib.ffvc_attn_packed_bwd(ctypes.byref(d), None), "too many")
+
+
+def test_projections_that_do_not_divide_into_heads_are_refused():
+    """By the launchers too, which would otherwise leave the last columns' gradient unwritten."""
+    cu = torch.tensor([0, 4], dtype=torch.int32)
+    for W, H, G in ((3 * 2 * 64 + 8, 2, 2), (200, 8, 8), (3 * 64, 0, 1), (3 * 64, 1, 0), (3 * 64, -1, 2)):
+        qkv = torch.zeros(4, W, dtype=HF)
+        with pytest.raises(ValueError):
+            K.attn_packed_qkv_fwd(qkv, cu, H, G, 1.0)
+        D = max(W // max(H + 2 * G, 1), 1)
+        o, lse = torch.zeros(4, H * D if H > 0 else 0, dtype=HF), torch.zeros(max(H, 0), 4)
+        with pytest.raises((ValueError, _lib.FFVCError)) as e:
+            K.attn_packed_qkv_bwd(qkv, o, o, lse, cu, H, G, 1.0)
+        assert isinstance(e.value, ValueError)
