@@ -1679,6 +1679,15 @@ def _heads3d(name, t, like=None):
     return (t.stride(0) if T > 1 else H * D), (t.stride(1) if H > 1 else D)
 
 
+def _written_apart(who, written, others):
+    """Tensors that a launch writes share no memory with what it reads: refused where they begin on the same element (other overlaps are the caller's)."""
+    seen = {t.data_ptr(): n for n, t in others}
+    for n, t in written:
+        if t.numel() and t.data_ptr() in seen:
+            raise ValueError(f"{who}: {n} and {seen[t.data_ptr()]} are the same memory")
+        seen[t.data_ptr()] = n
+
+
 def _packed_cu(cu):
     if cu.dtype != torch.int32 or cu.dim() != 1 or cu.numel() < 2 or not cu.is_contiguous():
         raise TypeError("attn_packed: cu_seqlens must be a contiguous int32 vector of at least two offsets")
@@ -1704,7 +1713,8 @@ def _attn_packed_desc(q, k, v, cu, scale):
 def attn_packed_fwd(q, k, v, cu_seqlens, scale, out=None, want_lse=False):
     """Causal attention over packed sequences: q (rows, heads, head_dim), k / v (rows, kv_heads, head_dim), views of one projection included;
     cu_seqlens int32 [sequences + 1] on the device -> (out (rows, heads, head_dim), lse fp32 (heads, rows) or None).  Without `out` the rows of
-    no sequence (before cu_seqlens[0], from cu_seqlens[-1] on) come as zeros; a given `out` keeps what it holds there.  lse is not written there."""
+    no sequence (before cu_seqlens[0], from cu_seqlens[-1] on) come as zeros; a given `out` keeps what it holds there.  lse is not written there.
+    `out` must share no memory with q, k or v: every workgroup reads them while others write."""
     d = _attn_packed_desc(q, k, v, cu_seqlens, scale)
     T, H, D = q.shape
     with _same_device(q, k, v, cu_seqlens, out):
@@ -1713,6 +1723,8 @@ def attn_packed_fwd(q, k, v, cu_seqlens, scale, out=None, want_lse=False):
             out = torch.empty(T, H, D, dtype=q.dtype, device=q.device)
         elif out.dtype != q.dtype:
             raise TypeError(f"attn_packed: out is {out.dtype}, q is {q.dtype}")
+        else:
+            _written_apart("attn_packed", (("out", out),), (("q", q), ("k", k), ("v", v)))
         d.out, (d.o_rs, d.o_hs) = out.data_ptr(), _heads3d("attn_packed: out", out, (T, H, D))
         lse = torch.empty(H, T, dtype=torch.float32, device=q.device) if want_lse else None
         d.lse = _ptr(lse)
@@ -1722,7 +1734,8 @@ def attn_packed_fwd(q, k, v, cu_seqlens, scale, out=None, want_lse=False):
 
 
 def attn_packed_bwd(q, k, v, out, dout, lse, cu_seqlens, scale, dq, dk, dv):
-    """Gradients of attn_packed_fwd into dq, dk, dv (views of one packed gradient included); rows of no sequence become zeros."""
+    """Gradients of attn_packed_fwd into dq, dk, dv (views of one packed gradient included); rows of no sequence become zeros.
+    dq, dk and dv must share no memory with one another or with what is read."""
     d = _attn_packed_desc(q, k, v, cu_seqlens, scale)
     T, H, D = q.shape
     for n, t, like in (("out", out, q), ("dout", dout, q), ("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
@@ -1736,6 +1749,7 @@ def attn_packed_bwd(q, k, v, out, dout, lse, cu_seqlens, scale, dq, dk, dv):
     _req_f32(lse)
     if tuple(lse.shape) != (H, T):
         raise ValueError("attn_packed_bwd: lse does not belong to these tensors")
+    _written_apart("attn_packed_bwd", (("dq", dq), ("dk", dk), ("dv", dv)), (("q", q), ("k", k), ("v", v), ("out", out), ("dout", dout)))
     with _same_device(q, k, v, out, dout, lse, cu_seqlens, dq, dk, dv):
         delta = torch.empty_like(lse)
         d.lse, d.delta, d.zero_tail = lse.data_ptr(), delta.data_ptr(), 1

@@ -252,3 +252,24 @@ def test_a_single_row_of_a_wider_buffer(cuda):
     ids = torch.tensor([0, 0, 1], device="cuda")
     assert torch.equal(K.embed_fwd(ids, table), K.embed_fwd(ids, table.contiguous()))
     assert torch.equal(K.embed_bwd(x, ids[:1], 3), K.embed_bwd(x.contiguous(), ids[:1], 3))
+
+
+def test_outputs_on_top_of_inputs_are_refused(cuda):
+    g = gen(670)
+    T, H, D, cu = 40, 2, 64, offsets([40])
+    q, k, v, do = (randn(g, T, H, D, dtype=HF) for _ in range(4))
+    for t in (q, k, v):
+        with pytest.raises(ValueError):
+            K.attn_packed_fwd(q, k, v, cu, 0.125, out=t)
+    o, lse = K.attn_packed_fwd(q, k, v, cu, 0.125, want_lse=True)
+    new = lambda: torch.empty_like(q)  # noqa: E731
+    one = new()
+    for dq, dk, dv in ((q, new(), new()), (new(), k, new()), (new(), new(), v), (do, new(), new()), (new(), o, new()), (one, one, new()), (one, new(), one), (new(), one, one)):
+        with pytest.raises(ValueError):
+            K.attn_packed_bwd(q, k, v, o, do, lse, cu, 0.125, dq, dk, dv)
+    grads = [new() for _ in range(3)]
+    K.attn_packed_bwd(q, k, v, o, do, lse, cu, 0.125, *grads)
+    assert all(bool(t.any()) for t in grads)
+    both = torch.empty(T, 2 * H, D, dtype=HF, device="cuda")             # interleaved rows of one buffer are no overlap
+    K.attn_packed_bwd(q, k, v, o, do, lse, cu, 0.125, new(), both[:, :H], both[:, H:])
+    assert torch.equal(both[:, :H], grads[1]) and torch.equal(both[:, H:], grads[2])
