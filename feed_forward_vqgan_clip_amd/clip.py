@@ -314,14 +314,17 @@ class CLIP:
 
     def encode_text_packed(self, ids, cu_seqlens, table=None):
         """Features of prompts packed behind one another (pack_tokens): ids int64 [rows], cu_seqlens int32 [B + 1], both on the device ->
-        (B, embed_dim) fp32.  Rows before the first and behind the last prompt are ignored, a prompt without tokens gives the features of a zero row, tokens past the
-        tower's context get no position (the offsets stay on the device: nothing checks them).
+        (B, embed_dim) fp32.  Rows before the first and behind the last prompt are ignored, a prompt without tokens gives the
+        features of a zero row (also where none has any), tokens past the tower's context get no position (the offsets stay on the device: nothing
+        checks them).
         table: a token embedding to use instead of the checkpoint's (vocab, width) fp32; gradients flow to it (and through the frozen tower)."""
         if not self.text_packed:
             raise RuntimeError("this CLIP was built without text_packed=True")
         if ids.dtype != torch.long or ids.dim() != 1 or cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2:
             raise TypeError("encode_text_packed expects int64 ids [rows] and int32 offsets [B + 1]")
         f32 = torch.float32
+        if ids.numel() == 0:                                                        # no token at all: one row that belongs to no prompt
+            ids = ids.new_full((1,), -1)
         first, end = cu_seqlens[:-1].long(), cu_seqlens[1:].long()
         row = torch.arange(ids.numel(), device=ids.device)
         seq = torch.searchsorted(end, row, right=True)                              # the prompt of a row; B behind the last one

@@ -102,11 +102,13 @@ def test_offsets_that_begin_behind_row_0(cuda, lens, H, G, D, first):
     assert bool((grad == 5.0).all())
 
 
+TOWER = dict(embed_dim=64, image_resolution=32, vision_layers=1, vision_width=128, vision_patch_size=8, context_length=77, vocab_size=500,
+             transformer_width=128, transformer_heads=2, transformer_layers=2)
+
+
 def test_packed_text_tower_on_a_slice_of_the_offsets(cuda):
     """Prompts 2 .. of a batch through the whole batch's rows: their features, and no gradient for the tokens of the prompts before them."""
-    cfg = dict(embed_dim=64, image_resolution=32, vision_layers=1, vision_width=128, vision_patch_size=8, context_length=77, vocab_size=500,
-               transformer_width=128, transformer_heads=2, transformer_layers=2)
-    model = fclip.CLIP(fclip.random_state_dict(cfg, 3), HF, text_packed=True)
+    model = fclip.CLIP(fclip.random_state_dict(TOWER, 3), HF, text_packed=True)
     g = torch.Generator().manual_seed(2)
     text = torch.zeros(6, 77, dtype=torch.long)
     for i in range(6):
@@ -273,3 +275,16 @@ def test_outputs_on_top_of_inputs_are_refused(cuda):
     both = torch.empty(T, 2 * H, D, dtype=HF, device="cuda")             # interleaved rows of one buffer are no overlap
     K.attn_packed_bwd(q, k, v, o, do, lse, cu, 0.125, new(), both[:, :H], both[:, H:])
     assert torch.equal(both[:, :H], grads[1]) and torch.equal(both[:, H:], grads[2])
+
+
+@pytest.mark.parametrize("int8", [False, True])
+def test_packed_text_tower_without_a_token(cuda, int8):
+    """Prompts that are all empty: each the features of an empty prompt beside others, and a gradient of zeros."""
+    model = fclip.CLIP(fclip.random_state_dict(TOWER, 3), HF, int8=int8, text_packed=True)
+    ids = torch.tensor([498, 5, 6, 499], device="cuda")
+    mixed = model.encode_text_packed(ids, torch.tensor([0, 4, 4], dtype=torch.int32, device="cuda"))
+    table = model.tok_emb.clone().requires_grad_()
+    got = model.encode_text_packed(ids[:0], torch.zeros(4, dtype=torch.int32, device="cuda"), table)
+    assert got.shape == (3, 64) and torch.allclose(got, mixed[1].expand(3, 64), rtol=1e-5, atol=1e-6)
+    (gt,) = torch.autograd.grad(got.sum(), table)
+    assert gt.shape == table.shape and not bool(gt.any())
