@@ -288,3 +288,26 @@ def test_packed_text_tower_without_a_token(cuda, int8):
     assert got.shape == (3, 64) and torch.allclose(got, mixed[1].expand(3, 64), rtol=1e-5, atol=1e-6)
     (gt,) = torch.autograd.grad(got.sum(), table)
     assert gt.shape == table.shape and not bool(gt.any())
+
+
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("H,G,D", [(2, 2, 64), (4, 2, 128), (96, 96, 64)])
+def test_offsets_of_any_kind_write_nothing_outside(cuda, H, G, D, many):
+    """Offsets that descend or leave the tensor, forward and backward, into views between guard rows and guard columns."""
+    g = gen(770 + D)
+    T = 700
+    qkv, do = randn(g, T, (H + 2 * G) * D, dtype=BF), randn(g, T, H, D, dtype=BF)
+    q, k, v = ops._split_heads(qkv, H, G)
+    cases = [[0, 5000], [-7, 30, 690], [0, 650, 20, 700], [700, 0], [-2 ** 31, 2 ** 31 - 1], [100, 100, 100], [900, 800, -1, 350], [0, 700, 0, 700, 0, 700]]
+    for cu in cases:
+        if many:                                               # more sequences than lanes: the search in place of the order by length
+            cu = cu + [cu[-1]] * 70
+        cu = torch.tensor(cu, dtype=torch.int32, device="cuda")
+        out = torch.full((T + 128, H * D + 64), 7.0, dtype=BF, device="cuda")
+        grad = torch.full((T + 128, (H + 2 * G) * D + 64), 7.0, dtype=BF, device="cuda")
+        o, lse = K.attn_packed_fwd(q, k, v, cu, D ** -0.5, out=out[64:64 + T, :H * D].unflatten(1, (H, D)), want_lse=True)
+        K.attn_packed_bwd(q, k, v, o, do, lse, cu, D ** -0.5, *ops._split_heads(grad[64:64 + T, :-64], H, G))
+        torch.cuda.synchronize()
+        for buf in (out, grad):
+            buf[64:64 + T, :-64] = 7.0
+            assert bool((buf == 7.0).all()), cu[:6]
