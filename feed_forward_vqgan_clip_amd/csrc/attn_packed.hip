@@ -31,6 +31,8 @@ constexpr float NEG_BIG = -3.0e38f;
 constexpr int F16_UP = 15;
 template <typename L>
 constexpr bool IS_F16 = std::is_same<L, f16_t>::value;
+// Exponents from here on are rounded so coarsely that a weight of 1 may come out as another power of two
+constexpr float LONG_EXP = 0x1p20f;
 // 64 lanes x 16 (4) bytes from a bounded buffer into consecutive LDS
 __device__ __forceinline__ void dma16(rsrc_t r, uint32_t off, unsigned char* lds) { __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_vp)lds, 16, off, 0, 0, 0); }
 __device__ __forceinline__ void dma4(rsrc_t r, uint32_t off, float* lds) { __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_vp)lds, 4, off, 0, 0, 0); }
@@ -419,7 +421,16 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_fwd_kernel(const ffvc_
         for (int r = 0; r < 16; ++r) acc[t][r] *= a;
       m = mx;
     }
-    const float mc = IS_F16<L> ? fmaf(m, c, -(float)F16_UP) : m * c;
+    constexpr float UP = IS_F16<L> ? F16_UP : 0.0f;
+    float mc = IS_F16<L> ? fmaf(m, c, -UP) : m * c;
+    if (__builtin_expect(__any(fabsf(mc) > LONG_EXP), 0)) { // the difference first, then: the row's largest weight is 1 (2^UP) whatever the scores are
+      const float sub = fabsf(mc) > LONG_EXP ? m : 0.0f;
+      mc = fabsf(mc) > LONG_EXP ? -UP : mc;
+#pragma unroll
+      for (int kt = 0; kt < NH; ++kt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) S[kt][r] -= sub;
+    }
     float sum = 0.0f;
 #pragma unroll
     for (int kt = 0; kt < NH; ++kt)
@@ -784,6 +795,7 @@ __global__ __launch_bounds__(64 * NW * SPLIT, 2) void attn_packed_dkv_kernel(con
     const int lim = (int)(ki - r0);                           // first query of the tile that sees this lane's key
     const int end = (int)(pl.len - r0 < QB ? pl.len - r0 : QB);       // rows past the sequence are zeros: against a key with an inf they would give NaN
     const bool edge = r0 < kw + 31 || end < QB;
+    const bool lengthy = IS_F16<L> && __any(fabsf(st[lane & (QB - 1)]) > LONG_EXP);     // then no weight may pass 1
 #pragma unroll
     for (int qt = 0; qt < QB / 32; ++qt) {
       if (r0 + 32 * qt + 31 < kw) continue;                  // a half of earlier queries only
@@ -812,6 +824,12 @@ __global__ __launch_bounds__(64 * NW * SPLIT, 2) void attn_packed_dkv_kernel(con
           const int r = 4 * g + j;
           S[r] = __builtin_amdgcn_exp2f(fmaf(S[r], c, -l4[j]));
           dP[r] *= S[r];                                      // ds / scale
+        }
+      }
+      if constexpr (IS_F16<L>) {
+        if (__builtin_expect(lengthy, 0)) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) S[r] = fminf(S[r], 32768.0f);
         }
       }
       if (edge) {

@@ -7,7 +7,7 @@ import torch
 from feed_forward_vqgan_clip_amd import clip as fclip
 from feed_forward_vqgan_clip_amd import kernels as K
 from feed_forward_vqgan_clip_amd import ops
-from test_packed_gpu import attn_reference, within
+from test_packed_gpu import attn_reference, half, within
 
 pytestmark = pytest.mark.gpu
 BF, HF, F32, F64 = torch.bfloat16, torch.float16, torch.float32, torch.float64
@@ -311,3 +311,28 @@ def test_offsets_of_any_kind_write_nothing_outside(cuda, H, G, D, many):
         for buf in (out, grad):
             buf[64:64 + T, :-64] = 7.0
             assert bool((buf == 7.0).all()), cu[:6]
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lens", [[300], [300] + [2] * 20])
+def test_scores_far_beyond_the_exponents(cuda, lens, D, dtype):
+    """Scores of 10^6 to 4 10^9 (exponents whose last place is up to 512), every key far above those before it: a query's output is its own value
+    row, to the rounding of its one weight and of the result."""
+    T = sum(lens)
+    for top in (64.0, 1024.0, 49152.0):
+        q, k = torch.zeros(T, 2, D, dtype=dtype, device="cuda"), torch.zeros(T, 2, D, dtype=dtype, device="cuda")
+        q[:, :, 5] = 49152.0
+        k[:, :, 5] = (torch.arange(T, device="cuda", dtype=F32)[:, None] + 1) * (top / 512)
+        k[:, 0, 5] = k[:, 0, 5].flip(0).neg()                          # negative scores in one head: the order stays
+        v = randn(gen(870), T, 2, D, dtype=dtype)
+        o, lse = K.attn_packed_fwd(q, k, v, offsets(lens), 1.0, want_lse=True)
+        assert bool(torch.isfinite(o).all()) and bool(torch.isfinite(lse).all())
+        if dtype == HF or T <= 256:                                      # (bf16 does not hold so many different keys: equal ones share the weight)
+            assert float(k[:, :, 5].double().diff(dim=0).min()) > 0
+            want = v.double()
+            within(o, want, (2 * half(dtype) + 4 * 2.0 ** -24) * want.abs() * (1 + half(dtype)) + 2.0 ** -25, "out")
+        dq, dk, dv = (torch.empty_like(q) for _ in range(3))
+        K.attn_packed_bwd(q, k, v, o, randn(gen(871), T, 2, D, dtype=dtype), lse, offsets(lens), 1.0, dq, dk, dv)
+        if top == 64.0:                                                  # exponents of 8 10^6: their rounding is below one
+            assert all(bool(torch.isfinite(t).all()) for t in (dq, dk, dv))
