@@ -322,7 +322,7 @@ __device__ __forceinline__ void redo_out(const uint16_t* Q, int64_t q_rs, const 
       const int n = (int)(i - j0 < 63 ? i - j0 + 1 : 64);
       const float s = lane < n ? dot_rows<L>(Q + i * q_rs, K + (j0 + lane) * k_rs, D) : -INFINITY;
       const float mx = fmaxf(m, wave_max(s)), a = __builtin_amdgcn_exp2f((m - mx) * c);
-      const float w = lane < n ? __builtin_amdgcn_exp2f(fmaf(s, c, -(mx * c))) : 0.0f;
+      const float w = lane < n ? __builtin_amdgcn_exp2f((s - mx) * c) : 0.0f;
       m = mx;
       l = l * a + wave_sum(w);
       o[0] *= a;

@@ -336,3 +336,21 @@ def test_scores_far_beyond_the_exponents(cuda, lens, D, dtype):
         K.attn_packed_bwd(q, k, v, o, randn(gen(871), T, 2, D, dtype=dtype), lse, offsets(lens), 1.0, dq, dk, dv)
         if top == 64.0:                                                  # exponents of 8 10^6: their rounding is below one
             assert all(bool(torch.isfinite(t).all()) for t in (dq, dk, dv))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("D", [64, 128])
+def test_scores_far_beyond_the_exponents_beside_a_nan(cuda, D, dtype):
+    """The rows that are summed again without a later NaN keep their one weight as well."""
+    T = 200
+    q, k = torch.zeros(T, 1, D, dtype=dtype, device="cuda"), torch.zeros(T, 1, D, dtype=dtype, device="cuda")
+    q[:] = 49152.0                                                       # every feature: scores of 4 10^10
+    k[:] = (torch.arange(T, device="cuda", dtype=F32)[:, None, None] + 1) * 64
+    v = randn(gen(970), T, 1, D, dtype=dtype)
+    for t in (150, T - 1):
+        x = v.clone()
+        x[t] = float("nan")
+        o, _ = K.attn_packed_fwd(q, k, x, offsets([T]), 1.0)
+        want = v[:t].double()
+        within(o[:t], want, (2 * half(dtype) + 4 * 2.0 ** -24) * want.abs() * (1 + half(dtype)) + 2.0 ** -25, "out")
+        assert bool(torch.isnan(o[t]).all())
