@@ -354,3 +354,22 @@ def test_scores_far_beyond_the_exponents_beside_a_nan(cuda, D, dtype):
         want = v[:t].double()
         within(o[:t], want, (2 * half(dtype) + 4 * 2.0 ** -24) * want.abs() * (1 + half(dtype)) + 2.0 ** -25, "out")
         assert bool(torch.isnan(o[t]).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("scale", [1e-44, 1e-38, 3e-30, 1e-6, 40.0])
+@pytest.mark.parametrize("lens,H,G,D", [([70, 3], 2, 1, 64), ([20, 9], 2, 2, 128), ([300], 2, 2, 64)])
+def test_scales_of_any_size(cuda, lens, H, G, D, scale, dtype):
+    """From scales at which every weight is the same (their smallest is subnormal) to one at which a few keys take all of it."""
+    g = gen(1070 + D)
+    T = sum(lens)
+    qkv, do = randn(g, T, (H + 2 * G) * D, dtype=dtype), randn(g, T, H * D, dtype=dtype)
+    q, k, v = ops._split_heads(qkv, H, G)
+    (o, dq, dk, dv), bounds = attn_reference(q, k, v, lens, scale, do.view(T, H, D))
+    leaf = qkv.clone().requires_grad_()
+    got = ops.attention_packed(leaf, offsets(lens), H, G, scale=scale)
+    (d,) = torch.autograd.grad(got, leaf, do)
+    # fp32 weights end at 2^-126 = 1.2e-38: up to 300 of them, times scale |dp - delta| |q| < 40 * 200 * 6, are less than 1e-30
+    small = 2.0 ** -25 if dtype == HF else 1e-30
+    for name, a, b, c in zip(("out", "dq", "dk", "dv"), (got.view(T, H, D),) + ops._split_heads(d, H, G), (o, dq, dk, dv), bounds):
+        within(a, b, c + small, name)
