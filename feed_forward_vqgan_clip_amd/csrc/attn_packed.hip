@@ -2,7 +2,8 @@
 //
 // The rows cu[b] .. cu[b + 1] - 1 of q / k / v are sequence b.  With c = scale * log2(e), query i of a sequence and its keys j <= i:
 //     s_ij = q_i . k_j        m_i = max_j s_ij        l_i = sum_j 2^(c (s_ij - m_i))        p_ij = 2^(c (s_ij - m_i)) / l_i
-//     o_i  = sum_j p_ij v_j                           lse_i = c m_i + log2 l_i   (kept for the backward: p_ij = 2^(c s_ij - lse_i))
+//     o_i  = sum_j p_ij v_j                           lse_i = c m_i + log2 l_i   (kept for the backward: p_ij = 2^(c s_ij - lse_i),
+//                                                                                 off by 2^-24 |lse_i| relatively)
 //     dv_j = sum_i p_ij do_i      dp_ij = do_i . v_j      delta_i = do_i . o_i      ds_ij = scale p_ij (dp_ij - delta_i)
 //     dq_i = sum_j ds_ij k_j      dk_j = sum_i ds_ij q_i  (over the heads / kv_heads query heads that share key head j's group)
 //
@@ -335,10 +336,11 @@ __device__ __forceinline__ void redo_out(const uint16_t* Q, int64_t q_rs, const 
 }
 
 // ---- forward -------------------------------------------------------------------------------------------------------------------
+// The weights are rounded to the 16-bit type, as the matrix instructions take them; their sum l is not.
 // NW waves x 32 queries; key / value tiles of KB = 64 rows in a ring of NST LDS slots, filled by LDS-DMA NST - 1 tiles ahead.  Every variant takes a
 // row's keys 64 at a time in the same steps, so a sequence's output does not depend on what it is packed with.
-// Bound by the softmax arithmetic beside the matrix instructions at two (128 features) or three waves per SIMD: 8192 rows, 16 heads of 128, 320 us
-// (860 TFLOP/s of visible pairs); two sequences of 16000, 32 heads, 4.2 ms (985); of 64 features 200 us (690).
+// Bound by the softmax arithmetic beside the matrix instructions at two (128 features) or three waves per SIMD: 8192 rows, 16 heads of 128, 337 us
+// (816 TFLOP/s of visible pairs; medians of a kernel trace); two sequences of 16000, 32 heads, 4.26 ms (970); of 64 features 199 us (690).
 template <typename L, int DP, int NW, int NST, int KB>
 __global__ __launch_bounds__(64 * NW, 2) void attn_packed_fwd_kernel(const ffvc_attn_packed_desc p, int64_t slots) {
   constexpr int BM = 32 * NW, NS = DP / 16, ND = DP / 32, TB = KB * DP * 2;
@@ -488,10 +490,12 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_packed_fwd_kernel(const ffvc_
 // ---- the range of f16 in the backward -----------------------------------------------------------------------------------------------------
 // P and dS are rounded to the 16-bit type, for the matrix instructions that multiply them with 16-bit rows: one rounding per weight.  bf16 has the range
 // of fp32; in f16 a dS of 65520 is infinite and one below 2^-24 has no bits left, though the sums that it belongs to fit.  So f16 weights carry a
-// power of two, 2^F16_UP at first, per query (dq) or key (dk, dv): it enters through the exponent, or through the accumulator that the scores start
+// power of two, 2^BWD_UP at first, per query (dq) or key (dk, dv): it enters through the exponent, or through the accumulator that the scores start
 // from, and is taken out of the sums.  A tile whose largest |f dS| passes 2^15 (|dS| > 1: loss-scaled gradients) lowers the factor and what has
 // been summed so far.  Cost, dq + dk / dv of 8192 rows with 16 heads: 516 -> 556 us with 64 features, 967 -> 993 with 128 (the maximum; the branch is
 // taken a few times per walk at most); bf16 compiles without it.
+// (Less than the forward's: a weight of the backward passes 1 by the rounding of its exponent, a power of two from exponents of 2^24 on.)
+constexpr int BWD_UP = 12;
 // 0, or the (negative) power by which the lane's factor has to change; the half-waves share their column
 __device__ __forceinline__ int lower_by(const f32x16_t& t) {
   float mx = 0.0f;
@@ -531,7 +535,7 @@ __device__ __forceinline__ void join_parts(f32x16_t (&acc)[ND], float* mem, int 
         for (int r = 0; r < 16; ++r) acc[t][r] += join[o * NW * W + (t * 16 + r) * 64];
 }
 
-// The forward's walk once more with three products per tile (s, dp, dq): 8192 rows, 16 heads of 128, 395 us (1040 TFLOP/s); of 64 features 200 us.
+// The forward's walk once more with three products per tile (s, dp, dq): 8192 rows, 16 heads of 128, 412 us (1000 TFLOP/s); of 64 features 200 us.
 // SPLIT = 2: twice NW waves, each NW of them take every other key tile of the same queries; the sums join in LDS at the end (run_bwd has the rule).
 template <typename L, int DP, int NW, int NST, int KB, int SPLIT>
 __global__ __launch_bounds__(64 * NW * SPLIT, DP == 64 && SPLIT == 1 ? 3 : 2) void attn_packed_dq_kernel(const ffvc_attn_packed_desc p, int64_t slots) {
@@ -592,7 +596,7 @@ __global__ __launch_bounds__(64 * NW * SPLIT, DP == 64 && SPLIT == 1 ? 3 : 2) vo
   }
   dl += other_half(dl);
   float ls = ok ? p.lse[stat] : 0.0f;
-  if constexpr (IS_F16<L>) ls -= (float)F16_UP;
+  if constexpr (IS_F16<L>) ls -= (float)BWD_UP;
   if (ok && h == 0 && part == 0) p.delta[stat] = -dl;                   // (negative: the accumulator of dp starts from it)
   f32x16_t acc[ND];
 #pragma unroll
@@ -681,10 +685,10 @@ __global__ __launch_bounds__(64 * NW * SPLIT, DP == 64 && SPLIT == 1 ? 3 : 2) vo
 // NW waves x 32 keys of one key / value head; walks the query tiles (QB rows of q and dout, two LDS stages) that see them, for every query head
 // of the group.  K stays in registers as the B operand of s = q k^T.  V, the B operand of dp = do v^T, stays there too at 64 features; at 128 both
 // next to the two accumulators would take more than half the register file, and one wave per SIMD cannot hide its own waits: V lies in LDS
-// (8192 rows, 16 heads of 128: 963 us with V in registers, 560 in LDS) and a step takes 32 queries, not 64.
+// (8192 rows, 16 heads of 128: 963 us with V in registers, 560 to 587 in LDS) and a step takes 32 queries, not 64.
 //
 // SPLIT > 1: SPLIT * NW waves, each NW of them take every SPLIT-th (head, query tile) of the same keys; the sums join in LDS at the end, in order.
-// (run_bwd has the rule and its figures.)  Four products per tile: 8192 rows, 16 heads of 128, 565 us (970 TFLOP/s).
+// (run_bwd has the rule and its figures.)  Four products per tile: 8192 rows, 16 heads of 128, 587 us (936 TFLOP/s).
 template <typename L, int DP, int NW, int NST, int QB, bool VLDS, int SPLIT>
 __global__ __launch_bounds__(64 * NW * SPLIT, 2) void attn_packed_dkv_kernel(const ffvc_attn_packed_desc p, int64_t slots) {
   constexpr int BM = 32 * NW, NS = DP / 16, ND = DP / 32, TB = QB * DP * 2, VB = VLDS ? BM * DP * 2 : 0;
@@ -779,7 +783,7 @@ __global__ __launch_bounds__(64 * NW * SPLIT, 2) void attn_packed_dkv_kernel(con
     zero16(aV[t]);
   }
   const bool ranged = IS_F16<L> && c > 0x1p-100f;
-  float up = ranged ? F16_UP / c : 0.0f;                     // the scores start from `up`: the lane's factor is 2^(c up)
+  float up = ranged ? BWD_UP / c : 0.0f;                     // the scores start from `up`: the lane's factor is 2^(c up)
 #pragma unroll 1
   for (int it = 0; it < steps; ++it) {
     arrive<(NST - 2) * PIECES>();
@@ -795,7 +799,6 @@ __global__ __launch_bounds__(64 * NW * SPLIT, 2) void attn_packed_dkv_kernel(con
     const int lim = (int)(ki - r0);                           // first query of the tile that sees this lane's key
     const int end = (int)(pl.len - r0 < QB ? pl.len - r0 : QB);       // rows past the sequence are zeros: against a key with an inf they would give NaN
     const bool edge = r0 < kw + 31 || end < QB;
-    const bool lengthy = IS_F16<L> && __any(fabsf(st[lane & (QB - 1)]) > LONG_EXP);     // then no weight may pass 1
 #pragma unroll
     for (int qt = 0; qt < QB / 32; ++qt) {
       if (r0 + 32 * qt + 31 < kw) continue;                  // a half of earlier queries only
@@ -824,12 +827,6 @@ __global__ __launch_bounds__(64 * NW * SPLIT, 2) void attn_packed_dkv_kernel(con
           const int r = 4 * g + j;
           S[r] = __builtin_amdgcn_exp2f(fmaf(S[r], c, -l4[j]));
           dP[r] *= S[r];                                      // ds / scale
-        }
-      }
-      if constexpr (IS_F16<L>) {
-        if (__builtin_expect(lengthy, 0)) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) S[r] = fminf(S[r], 32768.0f);
         }
       }
       if (edge) {
@@ -956,7 +953,11 @@ int check_written(const void* ptr, int64_t rs, int64_t hs, const ffvc_attn_packe
 
 // Short sequences on average: one wave per workgroup, so that a prompt does not pay for rows it has not.  Forward, four waves / one, us, 256 sequences with
 // 8 heads, of 20 / 48 / 64 / 100 / 128 rows: 20 / 9.7, 28 / 17, 26 / 20, 37 / 32, 62 / 36 with 64 features; 26 / 18, 32 / 31, 35 / 35, 53 / 66, 89 / 68 with 128 (and
-// 128 of 200 rows 38 / 36, 56 / 69).  A long sequence among short ones costs little: one of 4096 rows and 63 of 10, 74 / 79 and 105 / 115.
+// 128 of 200 rows 38 / 36, 56 / 69).  Backward, dq + dk / dv, 256 sequences of 20 / 48 / 64 / 100: 43 / 24, 54 / 43, 60 / 50, 95 / 83; 61 / 44, 90 / 86, 103 / 98, 186 / 209.
+// The mean says nothing about the longest sequence, and the lengths are not known here.  A long one among short or empty ones goes through one-wave
+// tiles whose walks nobody splits; four waves / one, forward and backward, 8 heads: one of 2048 rows and 63 of 10 39 / 39 and 66 / 104 (128 features 53 / 56,
+// 155 / 165); one of 4096 and 127 of 10 73 / 75, 183 / 200 (103 / 120, 327 / 338; with 16 / 4 heads of 64 85 / 90, 226 / 539); one of 8000 in 256 slots 130 / 164,
+// 348 / 398 (192 / 241, 634 / 841).  The rule stands for what it serves, prompts of like lengths, which the four-wave form takes twice as long for.
 inline bool short_rows(const ffvc_attn_packed_desc& d, int rows) { return d.rows <= rows * (int64_t)d.seqs; }
 
 template <typename L, int DP>
@@ -986,8 +987,8 @@ int run_bwd(const ffvc_attn_packed_desc& d, hipStream_t st) {
   } else {
     constexpr int NW = 4, NST = 2, KB = 64, QB = DP == 64 ? 64 : 32;
     const int64_t slots = d.rows / (32 * NW) + d.seqs + 2;
-    // (Tiles are counted as rows / 128 + seqs + 1 per head.)  Few query tiles for the chip's places: each split over two halves of its keys, tiles of 64 queries.  Measured (1 / 2 parts), us: 560 tiles, 8 ragged
-    // sequences with 16 heads 28 / 22, 128 features 42 / 37; 288 tiles, one of 2048 rows 39 / 30, 62 / 43; but 1056 tiles, one of 8192 198 / 217,
+    // (Tiles are counted as rows / 128 + seqs + 1 per head.)  Few query tiles for the chip's places: each split over two halves of its keys, tiles of 64
+    // queries.  Measured (1 / 2 parts), us: 560 tiles, 8 ragged sequences with 16 heads 28 / 22, 128 features 42 / 37; 288 tiles, one of 2048 rows 39 / 30, 62 / 43; but 1056 tiles, one of 8192 198 / 217,
     // 380 / 394; 2064 tiles, 24 ragged ones 72 / 90, 128 / 157 (the halves fetch every key and value twice as often).
     if ((slots - 1) * d.heads < 768) {
       const int64_t slots = d.rows / 64 + d.seqs + 2;
