@@ -411,8 +411,8 @@ __device__ __forceinline__ float act_gelu_grad_fast(float x) {
   gelu_parts_fast(x, cdf, e);
   return cdf + x * 0.39894228040143267794f * e;
 }
-// Two-at-a-time variants for bf16-storage epilogues: the polynomial parts compile to v_pk_*_f32 (two lanes of fp32
-// per issue slot) and the reciprocal is the 1-ulp v_rcp_f32 instead of the ~11-instruction IEEE division.
+// Two-at-a-time variants for bf16-storage epilogues: the reciprocal is the 1-ulp v_rcp_f32 instead of the ~11-instruction IEEE
+// division.  (The pairs are a way of writing: the build has no packed fp32 instructions, each half is an instruction of its own.)
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ f32x2_t rcp2_(f32x2_t v) {
   f32x2_t r;

@@ -774,8 +774,8 @@ __device__ __forceinline__ void gemm_epilogue_perm16(const ffvc_gemm_desc& p, f3
           epilogue_oct<T, EPI>(p, v, n, rcur.y, rcur.r, rcur.a, flags);      // the ordinary store of dy (bias / residual as asked)
           pre_cur = unpack8<T>(gb_raw[(2 * b + pp) % GD]);
           if (2 * b + pp + GD < 4 * MT) gb_raw[(2 * b + pp) % GD] = gnb_fetch(2 * b + pp + GD);
-          // two columns at a time on packed fp32 (v_pk_fma / v_pk_mul: the epilogue's VALU time is what the fusion costs — 4 cycles per
-          // wave instruction, 16 per transcendental); the fp32 value is used as it is (its 16-bit rounding moves a sum by ~1e-4 of
+          // two columns at a time (the epilogue's VALU time is what the fusion costs — 4 cycles per wave instruction, 16 per
+          // transcendental; the build has no packed fp32 instructions); the fp32 value is used as it is (its 16-bit rounding moves a sum by ~1e-4 of
           // the rounding noise of its terms)
 #pragma unroll
           for (int j = 0; j < 8; j += 2) {

@@ -506,7 +506,8 @@ template <typename L, typename YT, int ACT>
 int launch_gemm(const I8Args& p, hipStream_t st) {
   if (few_outputs(p.M, p.N)) return launch_skinny<L, YT>(p, st);
   // 256-row tiles from one per CU on (2056 x 4096 x 1024, 256 whole tiles: 19.3 against 22.8 us with 128 rows; 4617 x 512 x 2048, 72 tiles: 20.6
-  // against 13.5).  Up to 64 rows past the last whole tile go to the kernel above where the whole tiles fill the chip's two places per CU (16448 x
+  // against 13.5).  Just above the border a short K gains nothing: 4617 x 2048 x 512, 288 whole tiles, 15.6 against 15.1; 8192 x 2048 x 512, 512 tiles, 19.3
+  // against 19.8.  Up to 64 rows past the last whole tile go to the kernel above where the whole tiles fill the chip's two places per CU (16448 x
   // 4096 x 1024: 100 against 108 us; but 224 rows of 12000 x 2048 x 1024 45 against 38); with fewer they run beside the others anyway.
   const int64_t whole = (int64_t)(p.M / 256) * ceil_div(p.N, BN);
   if (whole < 256) return launch_tile<L, YT, ACT, 128>(p, st);

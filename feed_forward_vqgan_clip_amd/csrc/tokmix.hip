@@ -456,7 +456,7 @@ __global__ __launch_bounds__(512, 2) void tokmix_bwd_hidden_kernel(const uint16_
       for (int i = 0; i < 16; ++i) n1[i] = n2[i] = 0.0f;
       constexpr int KPG = NK1 / 8;             // k-steps of the next chunk per GELU pair
 #pragma unroll
-      for (int r = 0; r < 16; r += 2) {        // two hidden rows at a time: the erf / pdf polynomial runs on v_pk_*_f32
+      for (int r = 0; r < 16; r += 2) {        // two hidden rows at a time (in fp32 instructions of one value each)
         // the next chunk's fragments are read one VALU block ahead of the MFMAs that consume them: the LDS latency hides
         // under the GELU arithmetic instead of sitting in front of every MFMA (one k-step = 8 VGPRs in flight)
         static_assert(KPG == 1 || KPG == 2, "k-steps per GELU pair");
