@@ -174,3 +174,36 @@ def test_8_bit_layers_pass_gradients_straight_through(cuda, dtype, act):
     eh = ag.double().abs() * (2 * D * E) * (dy.double().abs() @ a2.abs()) + u * hid.abs() * (1 + u)        # the hidden gradient is stored in 16 bits
     want = hid @ a1
     within(dx, want, (eh @ a1.abs()) * (1 + u) + u * want.abs() * (1 + u) + 2 * Hd * E * (hid.abs() @ a1.abs()), "mlp dx")
+
+
+@pytest.mark.parametrize("int8", [False, True])
+def test_packed_tower_captured_and_replayed(cuda, int8):
+    """A fixed buffer of ids and offsets: one capture serves batches of other lengths, also with empty prompts and rows before the first one."""
+    cfg = dict(embed_dim=64, image_resolution=32, vision_layers=1, vision_width=128, vision_patch_size=8, context_length=77, vocab_size=500,
+               transformer_width=128, transformer_heads=2, transformer_layers=2)
+    model = fclip.CLIP(fclip.random_state_dict(cfg, 3), HF, int8=int8, text_packed=True)
+    rows, B = 200, 6
+    g = torch.Generator(device="cuda").manual_seed(31)
+    ids, cu = torch.zeros(rows, dtype=torch.long, device="cuda"), torch.zeros(B + 1, dtype=torch.int32, device="cuda")
+    batches = [[0, 10, 30, 31, 90, 150, 200], [0, 0, 77, 77, 100, 101, 140], [17, 40, 50, 90, 91, 92, 199], [0, 33, 66, 99, 132, 165, 198]]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.no_grad(), torch.cuda.stream(side):
+        for _ in range(2):
+            model.encode_text_packed(ids, cu)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.cuda.graph(graph):
+        got = model.encode_text_packed(ids, cu)
+    for r in range(2):
+        for c in batches:
+            new = torch.randint(0, 500, (rows,), generator=g, device="cuda")
+            off = torch.tensor(c, dtype=torch.int32, device="cuda")
+            ids.copy_(new)
+            cu.copy_(off)
+            graph.replay()
+            with torch.no_grad():
+                want = model.encode_text_packed(new, off)
+            torch.cuda.synchronize()
+            assert torch.allclose(got, want, rtol=1e-5, atol=1e-6), (r, c)
+            assert bool(torch.isfinite(got).all())
