@@ -535,6 +535,8 @@ __device__ __forceinline__ void join_parts(f32x16_t (&acc)[ND], float* mem, int 
         for (int r = 0; r < 16; ++r) acc[t][r] += join[o * NW * W + (t * 16 + r) * 64];
 }
 
+// delta is taken from the output as it is stored, in 16 bits: the exact one would need the output in 32 bits or another walk.  In bf16 gradients are then
+// off by 0.0025 (relative norm), by 0.0023 with the exact delta, by 0.0017 with nothing rounded but themselves; the rest is P's and dS's rounding.
 // The forward's walk once more with three products per tile (s, dp, dq): 8192 rows, 16 heads of 128, 412 us (1000 TFLOP/s); of 64 features 200 us.
 // SPLIT = 2: twice NW waves, each NW of them take every other key tile of the same queries; the sums join in LDS at the end (run_bwd has the rule).
 template <typename L, int DP, int NW, int NST, int KB, int SPLIT>
@@ -988,8 +990,9 @@ int run_bwd(const ffvc_attn_packed_desc& d, hipStream_t st) {
     constexpr int NW = 4, NST = 2, KB = 64, QB = DP == 64 ? 64 : 32;
     const int64_t slots = d.rows / (32 * NW) + d.seqs + 2;
     // (Tiles are counted as rows / 128 + seqs + 1 per head.)  Few query tiles for the chip's places: each split over two halves of its keys, tiles of 64
-    // queries.  Measured (1 / 2 parts), us: 560 tiles, 8 ragged sequences with 16 heads 28 / 22, 128 features 42 / 37; 288 tiles, one of 2048 rows 39 / 30, 62 / 43; but 1056 tiles, one of 8192 198 / 217,
-    // 380 / 394; 2064 tiles, 24 ragged ones 72 / 90, 128 / 157 (the halves fetch every key and value twice as often).
+    // queries.  Measured (1 / 2 parts), us: 560 tiles, 8 ragged sequences with 16 heads 28 / 22, 128 features 42 / 37; 288 tiles, one of 2048 rows 39 / 30,
+    // 62 / 43; but 1056 tiles, one of 8192 198 / 217, 380 / 394; 2064 tiles, 24 ragged ones 72 / 90, 128 / 157 (the halves fetch every key and value
+    // twice as often).
     if ((slots - 1) * d.heads < 768) {
       const int64_t slots = d.rows / 64 + d.seqs + 2;
       LAUNCH_PACKED((attn_packed_dq_kernel<L, DP, 2, 2, 32, 2>), 2 * 2 * 2 * 32 * DP * 2, d.heads, 256);

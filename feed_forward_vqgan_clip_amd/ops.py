@@ -557,7 +557,7 @@ class _MLPFn(Function):
         W1, W2, rows = ctx.W1, ctx.W2, ctx.rows
         cdt = W1.sh.dtype
         if not ctx.train and not ctx.needs_input_grad[0]:             # the residual alone: its gradient is dy (and the 8-bit form kept no act'(pre))
-            return None, None, None, None, None, (dy if ctx.has_res else None), None, None, None, None, None
+            return None, None, None, None, None, (_contig(dy) if ctx.has_res else None), None, None, None, None, None
         x, h_pre, h = ctx.saved_tensors
         dy = _contig(dy)
         f8_bwd = ctx.fp8 and W2.fp8["sht"] is not None and W1.fp8["sht"] is not None
